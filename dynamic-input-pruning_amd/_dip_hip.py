@@ -13,10 +13,13 @@ other, like the reference's SharedBuffers, dip_stream_predispatch.py:123-138).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 import os
 import threading
 from pathlib import Path
+from typing import NamedTuple
 
 import torch
 
@@ -93,6 +96,22 @@ _SIGS = {
                                     ctypes.c_float, ctypes.c_float, _p], _i32),
     "dip_decode_attention": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _sz,
                               _p], _i32),
+    "dip_kv4_write": ([_p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64,
+                       _p], _i32),
+    "dip_kv4_read": ([_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p], _i32),
+    "dip_qk_norm_rope_kv4": ([_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                              ctypes.c_float, _p], _i32),
+    "dip_qk_norm_rope_kv4_rows": ([_p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64,
+                                   _i64, _i64, ctypes.c_float, _p], _i32),
+    "dip_kv4_decode_attention_workspace_size": ([_i64, _i64, _i64, _i64], _sz),
+    "dip_kv4_decode_attention": ([_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, ctypes.c_float,
+                                  _p, _sz, _p], _i32),
+    "dip_kv4_prompt_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64], _sz),
+    "dip_kv4_prompt_attention": ([_p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
+                                  ctypes.c_float, _p, _sz, _p], _i32),
+    "dip_sample_workspace_size": ([_i64, _i64], _sz),
+    "dip_sample": ([_p, _i32, _i64, _i64, _i64, _p, ctypes.c_double, _i64, ctypes.c_double,
+                    ctypes.c_double, _p, _p, _p, _sz, _p], _i32),
     "dip_set_tuning": ([_i32, _i32], _i32),
     "dip_timeline_read": ([_i32, _p], _i32),
     "dip_get_tuning": ([_i32], _i32),
@@ -100,7 +119,7 @@ _SIGS = {
 # The argument lists above follow this version of include/dip_hip.h
 # (DIP_VERSION); a library built from another one would be called with
 # shifted arguments, or lack an entry point, so it is refused here.
-ABI_VERSION = 305
+ABI_VERSION = 306
 if lib.dip_version() != ABI_VERSION:
     raise ImportError(f"{LIB_PATH} reports ABI version {lib.dip_version()}, these bindings "
                       f"are written for {ABI_VERSION}; rebuild the library")
@@ -844,6 +863,275 @@ def decode_attention_fused(qkv, q_norm_w, k_norm_w, cos, sin, pos, k_cache, v_ca
                                           float(eps), float(scale), _stream(dev)),
            "dip_decode_attention_fused")
     return out
+
+
+# ---------------------------------------------------------------------------
+# the 4-bit key/value cache, its attention, and drawing a token
+# ---------------------------------------------------------------------------
+KV4_GROUP = 32   # dimensions of a row that share a scale
+KV4_BLOCK = 32   # rows of a block: max_len is a multiple
+
+
+class KV4Cache(NamedTuple):
+    """A 4-bit key/value cache (kv4_cache makes one): one layer's arrays, or
+    with a leading dimension every layer's (``layer(i)`` is one of them)."""
+    k: torch.Tensor       # int8 [n_kv_heads, max_len, 64]
+    v: torch.Tensor       # int8 [n_kv_heads, max_len / 32, 2048]
+    scales: torch.Tensor  # bf16 [n_kv_heads, max_len, 2, 4]
+
+    def layer(self, i: int) -> "KV4Cache":
+        return KV4Cache(self.k[i], self.v[i], self.scales[i])
+
+    @property
+    def max_len(self) -> int:
+        return self.k.shape[-2]
+
+
+def kv4_cache(n_kv_heads: int, max_len: int, device="cuda", layers=None) -> KV4Cache:
+    """An empty (zero) 4-bit cache of at least max_len rows (rounded up to a
+    multiple of 32), for one layer, or for `layers` of them."""
+    if n_kv_heads < 1 or max_len < 1 or (layers is not None and layers < 1):
+        raise RuntimeError("a cache needs at least one head, row and layer")
+    rows = -(-int(max_len) // KV4_BLOCK) * KV4_BLOCK
+    lead = (n_kv_heads,) if layers is None else (layers, n_kv_heads)
+    return KV4Cache(torch.zeros(*lead, rows, 64, dtype=torch.int8, device=device),
+                    torch.zeros(*lead, rows // KV4_BLOCK, 2048, dtype=torch.int8, device=device),
+                    torch.zeros(*lead, rows, 2, 4, dtype=torch.bfloat16, device=device))
+
+
+def _kv4(cache: KV4Cache, *ts):
+    """(device, n_kv_heads, max_len) of one layer's cache, all on one device."""
+    k, v, sc = cache
+    dev = _dev(k, v, sc, *ts)
+    if k.dim() != 3 or k.shape[1] % KV4_BLOCK or k.shape[2] != 64:
+        raise RuntimeError("cache must be one layer's arrays, as kv4_cache makes them")
+    nkv, max_len, _ = k.shape
+    for t, dt, shape in ((k, torch.int8, (nkv, max_len, 64)),
+                         (v, torch.int8, (nkv, max_len // KV4_BLOCK, 2048)),
+                         (sc, torch.bfloat16, (nkv, max_len, 2, 4))):
+        if t.dtype != dt or t.shape != shape or not t.is_contiguous() or t.data_ptr() % 16:
+            raise RuntimeError("cache must be one layer's arrays, as kv4_cache makes them")
+    return dev, nkv, max_len
+
+
+def _on(dev: torch.device):
+    """The device the library launches on, where it is not the current one."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _rows_in(start: int, n: int, max_len: int):
+    start, n = int(start), int(n)
+    if start < 0 or n < 0 or start + n > max_len:
+        raise RuntimeError(f"rows {start} .. {start + n} outside the cache's {max_len}")
+    return start, n
+
+
+def kv4_write(k, v, cache: KV4Cache, start: int = 0) -> None:
+    """Quantise k and v (bf16 [tokens, n_kv_heads, 128], any strides of the first
+    two dimensions) into rows start .. of one layer's cache."""
+    dev, nkv, max_len = _kv4(cache, k, v)
+    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (nkv, 128) \
+            or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise RuntimeError(f"k and v must be bf16 [tokens, {nkv}, 128]")
+    start, n = _rows_in(start, k.shape[0], max_len)
+    if n == 0:
+        return
+    # a last dimension that is not dense, odd strides and pointers: a dense copy
+    k, v = (t if t.stride(2) == 1 and not (t.stride(0) | t.stride(1)) & 1
+            and not t.data_ptr() & 3 else t.clone(memory_format=torch.contiguous_format)
+            for t in (k, v))
+    with _on(dev):
+        _check(lib.dip_kv4_write(_ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0),
+                                 v.stride(1), _ptr(cache.k), _ptr(cache.v), _ptr(cache.scales),
+                                 start, n, nkv, 128, max_len, _stream(dev)), "dip_kv4_write")
+
+
+def kv4_read(cache: KV4Cache, start: int = 0, rows=None):
+    """(k, v) bf16 [rows, n_kv_heads, 128]: what rows start .. (to the end of the
+    cache by default) of one layer's cache stand for, exactly."""
+    dev, nkv, max_len = _kv4(cache)
+    start, n = _rows_in(start, max_len - int(start) if rows is None else rows, max_len)
+    k, v = torch.empty(2, n, nkv, 128, dtype=torch.bfloat16, device=dev)
+    with _on(dev):
+        _check(lib.dip_kv4_read(_ptr(cache.k), _ptr(cache.v), _ptr(cache.scales), _ptr(k), _ptr(v),
+                                start, n, nkv, 128, max_len, _stream(dev)), "dip_kv4_read")
+    return k, v
+
+
+def _qk_kv4_check(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads, n_kv_heads, tokens):
+    dev, nkv, max_len = _kv4(cache, qkv, q_norm_w, k_norm_w, cos, sin, q_out)
+    if n_kv_heads != nkv or n_heads < 1:
+        raise RuntimeError(f"the cache has {nkv} kv heads, the call {n_kv_heads}")
+    _bf16_vec(qkv, tokens * (n_heads + 2 * nkv) * 128, "qkv")
+    _bf16_vec(q_norm_w, 128, "q_norm_w")
+    _bf16_vec(k_norm_w, 128, "k_norm_w")
+    _bf16_vec(q_out, tokens * n_heads * 128, "q_out")
+    for name, t in (("cos", cos), ("sin", sin)):
+        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape[-1] != 128:
+            raise RuntimeError(f"{name} must be a contiguous bf16 [rows, 128] table")
+    if cos.shape != sin.shape:
+        raise RuntimeError("cos and sin must have as many rows")
+    return dev, max_len, cos.numel() // 128
+
+
+def qk_norm_rope_kv4(qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out, cache: KV4Cache,
+                     n_heads: int, n_kv_heads: int, eps: float):
+    """qk_norm_rope_cache into one layer's 4-bit cache: one token's q|k|v at the
+    position in `pos` (int64, on the device); the tables must have the cache's
+    rows."""
+    dev, max_len, table = _qk_kv4_check(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads,
+                                        n_kv_heads, 1)
+    if table < max_len:
+        raise RuntimeError(f"cos and sin have {table} rows, the cache {max_len}")
+    _pos_tensor(pos, dev)
+    with _on(dev):
+        _check(lib.dip_qk_norm_rope_kv4(_ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos),
+                                        _ptr(sin), _ptr(pos), _ptr(q_out), _ptr(cache.k),
+                                        _ptr(cache.v), _ptr(cache.scales), n_heads, n_kv_heads,
+                                        128, max_len, float(eps), _stream(dev)),
+               "dip_qk_norm_rope_kv4")
+    return q_out
+
+
+def qk_norm_rope_kv4_rows(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache: KV4Cache,
+                          n_heads: int, n_kv_heads: int, eps: float, start: int = 0):
+    """qk_norm_rope_kv4 for a prompt's tokens: row t of qkv [tokens, ..] at
+    position start + t, q to row t of q_out."""
+    tokens = qkv.shape[0]
+    dev, max_len, table = _qk_kv4_check(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads,
+                                        n_kv_heads, tokens)
+    start, tokens = _rows_in(start, tokens, min(max_len, table))
+    with _on(dev):
+        _check(lib.dip_qk_norm_rope_kv4_rows(_ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos),
+                                             _ptr(sin), start, _ptr(q_out), _ptr(cache.k),
+                                             _ptr(cache.v), _ptr(cache.scales), tokens, n_heads,
+                                             n_kv_heads, 128, max_len, float(eps), _stream(dev)),
+               "dip_qk_norm_rope_kv4_rows")
+    return q_out
+
+
+def _attn_out(q, out, n: int, dev):
+    if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.data_ptr() % 16:
+        raise RuntimeError("q must be a contiguous, 16-byte aligned bf16 tensor")
+    if out is None:
+        return torch.empty_like(q)
+    if out.device != dev:
+        raise RuntimeError("out must be on q's device")
+    return _bf16_vec(out, n, "out")
+
+
+def _scratch(nbytes: int, ws, dev, name: str):
+    """The caller's workspace, or the caching allocator's, so that calls on several
+    streams and captured graphs each have their own (nothing has to be cleared)."""
+    if ws is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    if ws.device != dev or not ws.is_contiguous() or ws.numel() * ws.element_size() < nbytes:
+        raise RuntimeError(f"{name} workspace too small")
+    return ws
+
+
+def _nbytes(ws) -> int:
+    return 0 if ws is None else ws.numel() * ws.element_size()
+
+
+def kv4_decode_attention_workspace_bytes(n_heads: int, n_kv_heads: int, max_len: int) -> int:
+    return lib.dip_kv4_decode_attention_workspace_size(n_heads, n_kv_heads, 128, max_len)
+
+
+def kv4_decode_attention(q, cache: KV4Cache, pos, out, scale: float, ws=None):
+    """Grouped-query attention of one token (q, n_heads * 128 values) over rows
+    0 .. pos of one layer's 4-bit cache -> out (new if None)."""
+    dev, nkv, max_len = _kv4(cache, q)
+    nh = q.numel() // 128
+    if q.numel() != nh * 128 or nh < 1 or nh % nkv:
+        raise RuntimeError(f"q must hold a multiple of {nkv} heads of 128 values")
+    _pos_tensor(pos, dev)
+    out = _attn_out(q, out, nh * 128, dev)
+    with _on(dev):
+        ws = _scratch(kv4_decode_attention_workspace_bytes(nh, nkv, max_len), ws, dev,
+                      "attention")
+        _check(lib.dip_kv4_decode_attention(_ptr(q), _ptr(cache.k), _ptr(cache.v),
+                                            _ptr(cache.scales), _ptr(pos), _ptr(out), nh, nkv,
+                                            128, max_len, float(scale), _ptr(ws), _nbytes(ws),
+                                            _stream(dev)), "dip_kv4_decode_attention")
+    return out
+
+
+def kv4_prompt_attention(q, cache: KV4Cache, start: int, out, scale: float, ws=None):
+    """Grouped-query attention of a prompt's tokens (q [tokens, n_heads * 128] at
+    positions start ..), token t over rows 0 .. start + t of one layer's 4-bit
+    cache -> out (new if None)."""
+    dev, nkv, max_len = _kv4(cache, q)
+    if q.dim() != 2 or q.shape[1] % (128 * nkv) or not q.shape[1]:
+        raise RuntimeError(f"q must be [tokens, a multiple of {nkv} heads of 128 values]")
+    tokens, nh = q.shape[0], q.shape[1] // 128
+    start, tokens = _rows_in(start, tokens, max_len)
+    out = _attn_out(q, out, q.numel(), dev)
+    if tokens == 0:
+        return out
+    with _on(dev):
+        ws = _scratch(lib.dip_kv4_prompt_attention_workspace_size(tokens, start, nh, nkv, 128), ws,
+                      dev, "attention")
+        _check(lib.dip_kv4_prompt_attention(_ptr(q), _ptr(cache.k), _ptr(cache.v),
+                                            _ptr(cache.scales), start, _ptr(out), tokens, nh,
+                                            nkv, 128, max_len, float(scale), _ptr(ws),
+                                            _nbytes(ws), _stream(dev)),
+               "dip_kv4_prompt_attention")
+    return out
+
+
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def check_sampling(temperature: float, top_k: int, top_p: float, min_p: float) -> None:
+    """Raise where sample would."""
+    if not (math.isfinite(temperature) and temperature >= 0):
+        raise RuntimeError(f"temperature must be finite and >= 0, got {temperature}")
+    if top_k < 0 or int(top_k) != top_k:
+        raise RuntimeError(f"top_k must be a whole number >= 0, got {top_k}")
+    if not 0 < top_p <= 1:
+        raise RuntimeError(f"top_p must be in (0, 1], got {top_p}")
+    if not 0 <= min_p <= 1:
+        raise RuntimeError(f"min_p must be in [0, 1], got {min_p}")
+
+
+def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+           min_p: float = 0.0, out=None, prob=None, ws=None):
+    """(token int64 [rows], its probability fp32 [rows]): one token drawn from each
+    row of logits [rows, vocab] (bf16, fp16 or fp32; dense rows, any row stride)
+    with the numbers u (fp32 [rows], in [0, 1)).
+
+    Of the tokens in the order (logit descending, index ascending), with weights
+    exp((logit - max) / temperature): the first top_k are kept (0: all), of those
+    the fewest whose weights reach top_p of their sum, of those the ones with at
+    least min_p of the largest weight.  The token is where the running sum of the
+    kept weights, by index, exceeds u times their sum.  temperature 0 is greedy.
+    NaN counts as -inf; a row of nothing else gives token 0, probability 0."""
+    check_sampling(temperature, top_k, top_p, min_p)
+    dev = _dev(logits, u)
+    if logits.dtype not in _LOGIT_TYPES or logits.dim() != 2 or logits.shape[1] < 1:
+        raise RuntimeError("logits must be bf16, fp16 or fp32 [rows, vocab]")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1 or logits.stride(0) < 0:
+        logits = logits.contiguous()
+    u = _want(u.reshape(-1), torch.float32, "u", (rows,))
+    token = torch.empty(rows, dtype=torch.int64, device=dev) if out is None else out
+    prob = torch.empty(rows, dtype=torch.float32, device=dev) if prob is None else prob
+    for name, t, dt in (("out", token, torch.int64), ("prob", prob, torch.float32)):
+        if t.dtype != dt or t.numel() != rows or not t.is_contiguous() or t.device != dev:
+            raise RuntimeError(f"{name} must be a contiguous {dt} tensor of {rows} values on the "
+                               "logits' device")
+    if rows == 0:
+        return token, prob
+    with _on(dev):
+        ws = _scratch(lib.dip_sample_workspace_size(rows, vocab), ws, dev, "sampling")
+        _check(lib.dip_sample(_ptr(logits), _LOGIT_TYPES[logits.dtype], rows, vocab,
+                              logits.stride(0), _ptr(u), float(temperature), int(top_k),
+                              float(top_p), float(min_p), _ptr(token), _ptr(prob), _ptr(ws),
+                              _nbytes(ws), _stream(dev)), "dip_sample")
+    return token, prob
 
 
 def mlp_decode_rmsnorm(gate_qw, gate_sc, up_qw, up_sc, down_t_qw, down_t_sc, res, add, norm_w,

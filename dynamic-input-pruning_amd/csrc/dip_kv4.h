@@ -1,0 +1,100 @@
+// dip_kv4.h — the 4-bit key/value cache: its layout in memory and the device
+// code that packs and unpacks it.
+//
+// Values.  Each row (position) of each key/value head has 128 keys and 128
+// values, in groups of 32 consecutive dimensions.  A group is a bf16 scale s
+// and whole numbers q in [-7, 7] (4 bits, two's complement) and stands for
+// q * s.  With a the group's largest magnitude,
+//   s = a / 7 with the significand cut to 5 bits (0 below 2^-100),
+//   q = rint(x / s).
+// Cutting s keeps 7 s <= a (nothing overflows) and a / s < 7.5, so every error
+// is at most s / 2; and |q| <= 7 has 3 bits, so q * s has at most 8: it is a
+// bf16 number, and every reader of the cache computes with the same values.
+// A group that holds a NaN or an infinity has s = NaN and stands for NaN.
+//
+// Layout (per key/value head; max_len a multiple of 32):
+//   scales bf16 [max_len][2][4]: a row's 4 key scales, then its 4 value scales.
+//   keys   [max_len][16 words]: word 4 c + g of a row holds dimensions
+//          32 g + 8 c .. + 7, so one 16-byte load per lane is the A operand of
+//          four 16x16x32 MFMAs (lane quarter c, 16 rows), one per group: a
+//          group's scale then multiplies a finished product.
+//   values [max_len / 32][512 words]: 32 rows together.  Word
+//          256 (d / 64) + 64 c + 4 (d % 16) + (d / 16) % 4 holds dimension d of
+//          the rows 4 c .. 4 c + 3 and 16 + 4 c .. 16 + 4 c + 3: as many rows as
+//          a lane of quarter c has scores of in the result of the key MFMAs, so
+//          the softmax's weights are the value MFMA's B operand where they are.
+// In a word, element j (a dimension of a key, a row of a value) is nibble
+// j / 2 + 4 (j % 2): v_bitop3 turns nibbles m and m + 4 into one register of the
+// operand (elements 2 m and 2 m + 1).
+#pragma once
+
+#include "dip_common.h"
+#include "dip_internal.h"
+
+namespace dip {
+
+constexpr int kKvHeadDim = 128;
+constexpr int kKvGroups = 4;           // scale groups of a row
+constexpr int kKvKeyBytes = 64;        // a row's packed keys
+constexpr int kKvScaleVals = 8;        // a row's scales (keys, then values)
+constexpr int kKvBlock = 32;           // rows of a value block
+constexpr int kKvBlockWords = 512;
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+// Element j of a word, as a shift.
+DIP_DEV int kv4_shift(int j) { return 4 * ((j >> 1) + 4 * (j & 1)); }
+// The word of a value block that holds dimension d for lane quarter c.
+DIP_DEV int kv4_value_word(int d, int c) {
+  return 256 * (d >> 6) + 64 * c + 4 * (d & 15) + ((d >> 4) & 3);
+}
+// Row r (0 .. 31) of a block: lane quarter and element of the word.
+DIP_DEV int kv4_row_quarter(int r) { return (r >> 2) & 3; }
+DIP_DEV int kv4_row_elem(int r) { return 4 * (r >> 4) + (r & 3); }
+
+// One word as an MFMA operand of 8 bf16 values 1.5 + q / 16 (exact).
+DIP_DEV bf16x8_t kv4_biased(uint32_t w) {
+  u32x4_t r;
+  r.x = ((w << 3) & kPairMask) ^ kPairMagicFlip;
+  r.y = ((w >> 1) & kPairMask) ^ kPairMagicFlip;
+  r.z = ((w >> 5) & kPairMask) ^ kPairMagicFlip;
+  r.w = ((w >> 9) & kPairMask) ^ kPairMagicFlip;
+  return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// Nibble at `shift` as a signed number.
+DIP_DEV int kv4_nibble(uint32_t w, int shift) { return (int)(w << (28 - shift)) >> 28; }
+
+// Max over aligned groups of 16 lanes of whole numbers.
+DIP_DEV uint32_t group_umax16(uint32_t v) {
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+  v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));
+  return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));
+}
+
+// A pair of bf16 values per lane, 16 lanes to a group: the group's scale (bf16
+// bits) and the pair's numbers as nibbles.
+struct Kv4Pair {
+  uint32_t scale, q0, q1;
+};
+
+DIP_DEV Kv4Pair kv4_quantize(uint32_t pair) {
+  const float x0 = bf16_to_f32(pair & 0xFFFFu), x1 = __uint_as_float(pair & 0xFFFF0000u);
+  const uint32_t a =
+      group_umax16(max((pair << 16) & 0x7FFFFFFFu, pair & 0x7FFF0000u));  // |x| orders as its bits
+  uint32_t sb = __float_as_uint(__uint_as_float(a) / 7.0f) & 0xFFF80000u;
+  if (sb < 0x0D800000u) sb = 0u;         // below 2^-100
+  if (a >= 0x7F800000u) sb = 0x7FC00000u;  // an infinity or a NaN in the group
+  const float s = __uint_as_float(sb);
+  Kv4Pair r;
+  r.scale = sb >> 16;
+  const bool some = s > 0.f;
+  const float q0 = some ? rintf(x0 / s) : 0.f, q1 = some ? rintf(x1 / s) : 0.f;
+  r.q0 = (uint32_t)(int)fminf(fmaxf(q0, -7.f), 7.f) & 15u;
+  r.q1 = (uint32_t)(int)fminf(fmaxf(q1, -7.f), 7.f) & 15u;
+  return r;
+}
+
+}  // namespace dip

@@ -52,7 +52,8 @@ const char* dip_status_string(int status);
  * Library version as an integer (major * 10000 + minor * 100 + patch).  The
  * minor number changes whenever an entry point's argument list changes, so
  * a binding written against this header checks dip_version() == DIP_VERSION
- * before its first call.  0.3.5 adds dip_int4_gemm_swiglu, dip_swiglu,
+ * before its first call.  0.3.6 adds the 4-bit key/value cache (dip_kv4_*,
+ * dip_qk_norm_rope_kv4*) and dip_sample.  0.3.5 adds dip_int4_gemm_swiglu, dip_swiglu,
  * dip_dequant_t, dip_stream_rows, dip_add_rmsnorm_rows and
  * dip_qk_norm_rope_cache_rows.  0.3.4: dip_int4_gather_down_by_channel takes
  * indices == NULL (every row in order; it was an error).  0.3.3 adds the
@@ -63,7 +64,7 @@ const char* dip_status_string(int status);
  * down_t_sc_gm to the decode and gather-down entry points and g_len to
  * dip_ca_fused_gemv.
  */
-#define DIP_VERSION 305
+#define DIP_VERSION 306
 int dip_version(void);
 
 /* Highest row count the top-k supports (its keys are staged in LDS). */
@@ -610,6 +611,107 @@ int dip_decode_attention(const uint16_t* q, const uint16_t* k_cache, const uint1
                          const int64_t* pos, uint16_t* out, int64_t n_heads, int64_t n_kv_heads,
                          int64_t head_dim, int64_t max_len, float scale, void* workspace,
                          size_t ws_bytes, void* stream);
+
+/*
+ * The 4-bit key/value cache.  The reference keeps its keys and values in
+ * transformers' bf16 cache and has no counterpart of these.
+ *
+ * Per row (position) and kv head, groups of 32 consecutive dimensions of the
+ * key and of the value share a bf16 scale s and hold whole numbers q in
+ * [-7, 7], standing for q * s.  With a the group's largest magnitude s is a / 7
+ * cut to a 5-bit significand (0 below 2^-100) and q = rint(x / s), so every
+ * q * s is a bf16 number and off by s / 2 at most.  A group with an infinity
+ * or a NaN stands for NaN.  A layer's cache is three device arrays (the
+ * packing of their words is csrc/dip_kv4.h's):
+ *   k_cache   int8 [n_kv_heads, max_len, 64]
+ *   v_cache   int8 [n_kv_heads, max_len / 32, 2048]
+ *   kv_scales bf16 [n_kv_heads, max_len, 2, 4]
+ * max_len a multiple of 32 (else DIP_ERR_SHAPE), head_dim 128 (else
+ * DIP_ERR_UNSUPPORTED); 144 bytes per row and kv head, where bf16 takes 512.
+ * They must hold finite or any bits, but allocated ones, for every row: rows
+ * behind a token's position are read and do not count.  Writers change the
+ * rows they are given and no others; two that write rows of one block of 32
+ * must be ordered on a stream.
+ *
+ * dip_kv4_write: k and v bf16, token t's head h at k + t * k_tok_stride +
+ * h * k_head_stride (in values; even, pointers 4-byte aligned), into rows
+ * start .. start + tokens - 1, which the cache must have.
+ */
+int dip_kv4_write(const uint16_t* k, const uint16_t* v, int64_t k_tok_stride,
+                  int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride,
+                  int8_t* k_cache, int8_t* v_cache, uint16_t* kv_scales, int64_t start,
+                  int64_t tokens, int64_t n_kv_heads, int64_t head_dim, int64_t max_len,
+                  void* stream);
+
+/* k_out, v_out bf16 [rows, n_kv_heads, head_dim]: what rows start ..
+ * start + rows - 1 stand for, exactly. */
+int dip_kv4_read(const int8_t* k_cache, const int8_t* v_cache, const uint16_t* kv_scales,
+                 uint16_t* k_out, uint16_t* v_out, int64_t start, int64_t rows,
+                 int64_t n_kv_heads, int64_t head_dim, int64_t max_len, void* stream);
+
+/* dip_qk_norm_rope_cache and its rows form with the 4-bit cache: the token at
+ * the device-side position (outside [0, max_len): q_out with row 0 of the
+ * tables, no cache row), and a prompt's tokens at positions start ..
+ * start + tokens - 1, which the cache must have.  The norm's mean and root are
+ * taken in 64 bits, so a row of the cache depends on its token alone. */
+int dip_qk_norm_rope_kv4(const uint16_t* qkv, const uint16_t* q_norm_w, const uint16_t* k_norm_w,
+                         const uint16_t* cos_table, const uint16_t* sin_table,
+                         const int64_t* pos, uint16_t* q_out, int8_t* k_cache, int8_t* v_cache,
+                         uint16_t* kv_scales, int64_t n_heads, int64_t n_kv_heads,
+                         int64_t head_dim, int64_t max_len, float eps, void* stream);
+int dip_qk_norm_rope_kv4_rows(const uint16_t* qkv, const uint16_t* q_norm_w,
+                              const uint16_t* k_norm_w, const uint16_t* cos_table,
+                              const uint16_t* sin_table, int64_t start, uint16_t* q_out,
+                              int8_t* k_cache, int8_t* v_cache, uint16_t* kv_scales,
+                              int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                              int64_t head_dim, int64_t max_len, float eps, void* stream);
+
+/*
+ * dip_kv4_decode_attention: dip_decode_attention over the 4-bit cache, for any
+ * n_heads (at most 4096) that n_kv_heads divides.  A position before the first
+ * row attends nothing and gives zeros; one behind the last attends every row.
+ * dip_kv4_prompt_attention: the tokens of q [tokens, n_heads, head_dim] at
+ * positions start .. start + tokens - 1, token t over rows 0 .. start + t, into
+ * out [tokens, n_heads, head_dim].
+ * Products of bf16 numbers summed in fp32, softmax and its sums in fp32, the
+ * weights (times the values' scales) rounded to bf16, bf16 results.  The
+ * workspaces need no clearing.
+ */
+size_t dip_kv4_decode_attention_workspace_size(int64_t n_heads, int64_t n_kv_heads,
+                                               int64_t head_dim, int64_t max_len);
+int dip_kv4_decode_attention(const uint16_t* q, const int8_t* k_cache, const int8_t* v_cache,
+                             const uint16_t* kv_scales, const int64_t* pos, uint16_t* out,
+                             int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                             int64_t max_len, float scale, void* workspace, size_t ws_bytes,
+                             void* stream);
+size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_t start, int64_t n_heads,
+                                               int64_t n_kv_heads, int64_t head_dim);
+int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache, const int8_t* v_cache,
+                             const uint16_t* kv_scales, int64_t start, uint16_t* out,
+                             int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                             int64_t head_dim, int64_t max_len, float scale, void* workspace,
+                             size_t ws_bytes, void* stream);
+
+/*
+ * token[r] (int64) drawn from row r of logits [rows, vocab] (DIP_BF16, DIP_F16
+ * or DIP_F32; rows row_stride values apart) with the number u[r] in [0, 1), and
+ * prob[r] (fp32, may be NULL) its probability.  With the tokens ordered by
+ * (logit descending, index ascending) and w = exp((logit - max) / temperature):
+ * the first top_k tokens are kept (0: all), of those the fewest whose weights
+ * reach top_p times their sum, of those the ones with w >= min_p; the token is
+ * the first by index at which the running sum of the kept weights exceeds u
+ * times their sum (the last kept one for u beyond 1 or NaN).  temperature 0: the
+ * largest logit, the lowest index among equals.  NaN counts as -inf, -inf is never
+ * drawn; a row of nothing else gives token 0 with probability 0.  Sums and
+ * weights in 64 bits.  temperature >= 0, top_k >= 0, top_p in (0, 1], min_p in
+ * [0, 1] (else DIP_ERR_ARG).  The reference decodes greedily
+ * (gen_utils.py:40-46) and has no counterpart.
+ */
+enum { DIP_BF16 = 0, DIP_F16 = 1, DIP_F32 = 2 };
+size_t dip_sample_workspace_size(int64_t rows, int64_t vocab);
+int dip_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+               const float* u, double temperature, int64_t top_k, double top_p, double min_p,
+               int64_t* token, float* prob, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }  // extern "C"
