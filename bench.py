@@ -136,7 +136,8 @@ def whole_model(args) -> int:
           f"keep={args.keep}", file=sys.stderr, flush=True)
     model, mods = synthetic_model(cfg, args.keep, dev, seed=0)
     plen, gen_new = 32, 64
-    dec = DIPDecoder(model, max_len=plen + max(args.warmup + args.steps, gen_new) + 1)
+    dec = DIPDecoder(model, max_len=plen + max(args.warmup + args.steps, gen_new) + 1,
+                     kv_bits=args.kv_bits)
     prompt = torch.randint(0, cfg.vocab_size, (1, plen), generator=torch.Generator().manual_seed(0))
     print("[bench] model built; prefill + warmup", file=sys.stderr, flush=True)
     dec.prefill(prompt)
@@ -177,7 +178,7 @@ def whole_model(args) -> int:
         "higher_is_better": True, "dtype": "bf16", "data": "synthetic",
         "config": {"workload": f"{args.shape}-shape whole model, batch 1, prompt {plen}, "
                                "HIP-graph decode step", "layers": cfg.num_hidden_layers,
-                   "keep": args.keep, "k": k},
+                   "keep": args.keep, "k": k, "kv_bits": args.kv_bits},
         "reference_method_tok_s": round(sum(runs) / len(runs), 2),
         "reference_method": f"greedy generate of {gen_new} tokens incl. {plen}-token prefill, "
                             "wall clock, mean of 3 after 1 warmup",
@@ -612,6 +613,8 @@ def main(argv=None):
     ap.add_argument("--eager", action="store_true",
                     help="launch every kernel eagerly instead of replaying the captured graph "
                          "(for counter collection, which profiles each dispatch)")
+    ap.add_argument("--kv-bits", type=int, choices=(4, 16), default=16,
+                    help="with --whole-model: bits of the cached keys and values")
     ap.add_argument("--whole-model", action="store_true",
                     help="instead of the MLP stack, time greedy decode of a whole synthetic "
                          "Qwen3 of --shape (attention, DIP MLPs, lm_head) with the HIP-graph "

@@ -8,7 +8,8 @@ swap each decoder MLP for a DIP module, then load every other tensor of
 model_int4.safetensors.  One MI355X holds the whole model in HBM, so every
 tensor goes to one device; there is no offload map.
 
-``DIPDecoder`` runs greedy decoding.  The prompt runs like the HF forward (the
+``DIPDecoder`` decodes, greedily or drawing tokens (temperature, top-k, top-p,
+min-p), with its keys and values in bf16 or in 4 bits.  The prompt runs like the HF forward (the
 reference's prefill: the DIP modules take their dense route for sequences
 longer than one token), on this library's kernels around the projections and
 MLPs where the model fits them, and leaves its keys and values in a static
@@ -204,9 +205,16 @@ def _rotate_half(x: torch.Tensor) -> torch.Tensor:
     return torch.cat((-x[..., h:], x[..., :h]), dim=-1)
 
 
+# Tokens of a prompt that go through the layers together where the cache is in 4
+# bits: its attention takes up a prompt at any row, so a long one's activations
+# (three times the MLP's width per token) need not be held at once.
+_PROMPT_CHUNK = 8192
+
+
 class DIPDecoder:
-    """Greedy decoding of a Qwen3 causal LM with a static key/value cache and
-    a HIP-graph decode step.  Batch size 1, as the reference's decode.
+    """Decoding of a Qwen3 causal LM, greedy or drawing tokens, with a static
+    key/value cache and a HIP-graph decode step.  Batch size 1, as the
+    reference's decode.
 
     Args:
       model:     a Qwen3ForCausalLM-shaped model (model.model.layers[i] with
@@ -229,10 +237,16 @@ class DIPDecoder:
                  folded into the DIP MLP's gate (7 launches per layer, 9 for
                  long caches).  None: whenever the model fits them (GPU,
                  bf16, head_dim 128, int4 attention projections).
+      kv_bits:   16: keys and values in the model's type.  4: in 4 bits with a
+                 scale per 32 dimensions (144 bytes per row and kv head instead
+                 of 512), for long sequences; needs the fused kernels.  The
+                 prompt's attention then reads the 4-bit rows too, so it sees
+                 what later tokens see (through the HF forward, where the model
+                 has other modules, hooks or modes, it does not).
     """
 
     def __init__(self, model: nn.Module, max_len: int = 1024, use_graph: bool = True,
-                 fused=None):
+                 fused=None, kv_bits: int = 16):
         inner = model.model
         cfg = model.config
         self.model = model
@@ -249,18 +263,32 @@ class DIPDecoder:
         if rot.rope_type not in _STATIC_ROPE:
             raise ValueError(f"rope type {rot.rope_type!r}: frequencies change with length")
         self.max_len = int(max_len)
-        pos = torch.arange(self.max_len, dtype=torch.float32, device=self.device)
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
+        self.kv_bits = kv_bits
+        supported = self._fused_supported()
+        if kv_bits == 4 and (not supported or (fused is not None and not fused)):
+            raise ValueError("a 4-bit cache needs the fused decode: a GPU, bf16 weights, head_dim "
+                             "128, int4 attention projections and a supported head grouping")
+        rows = self.max_len
+        if kv_bits == 4:
+            import _dip_hip as K
+            self.kv4 = K.kv4_cache(self.nkv, self.max_len, self.device, layers=len(self.layers))
+            self._kv4 = [self.kv4.layer(i) for i in range(len(self.layers))]
+            rows = self.kv4.max_len
+        pos = torch.arange(rows, dtype=torch.float32, device=self.device)
         freqs = pos[:, None] * rot.inv_freq.to(self.device, torch.float32)[None, :]
         table = torch.cat((freqs, freqs), dim=-1)
         self.cos = (table.cos() * rot.attention_scaling).to(self.dtype)
         self.sin = (table.sin() * rot.attention_scaling).to(self.dtype)
-        shape = (len(self.layers), self.nkv, self.max_len, self.hd)
-        self.k_cache = torch.zeros(shape, dtype=self.dtype, device=self.device)
-        self.v_cache = torch.zeros(shape, dtype=self.dtype, device=self.device)
+        if kv_bits == 16:
+            shape = (len(self.layers), self.nkv, self.max_len, self.hd)
+            self.k_cache = torch.zeros(shape, dtype=self.dtype, device=self.device)
+            self.v_cache = torch.zeros(shape, dtype=self.dtype, device=self.device)
         self._cols = torch.arange(self.max_len, device=self.device)
         self.tok = torch.zeros(1, dtype=torch.long, device=self.device)
         self.pos = torch.zeros(1, dtype=torch.long, device=self.device)
-        supported = self._fused_supported()
+        self._draw = None  # how generate draws its tokens; None: greedy
         if fused and not supported:
             raise ValueError("fused decode needs a GPU, bf16 weights, head_dim 128, int4 "
                              "attention projections and a supported head grouping")
@@ -336,9 +364,10 @@ class DIPDecoder:
         self._qkv = torch.empty((self.nh + 2 * self.nkv) * self.hd, dtype=bf, device=dev)
         self._q = torch.empty(self.nh * self.hd, dtype=bf, device=dev)
         self._o = torch.empty(self.nh * self.hd, dtype=bf, device=dev)
-        self._attn_ws = torch.zeros(K.decode_attention_workspace_bytes(self.nh, self.hd,
-                                                                       self.max_len),
-                                    dtype=torch.uint8, device=dev)
+        nbytes = (K.kv4_decode_attention_workspace_bytes(self.nh, self.nkv, self.kv4.max_len)
+                  if self.kv_bits == 4 else
+                  K.decode_attention_workspace_bytes(self.nh, self.hd, self.max_len))
+        self._attn_ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
         # short caches: norm + rotary + cache write + attention in one launch
         # (one workgroup per kv head); longer ones split the cache over many
         # workgroups (three launches)
@@ -365,7 +394,13 @@ class DIPDecoder:
             else:
                 K.add_rmsnorm(h, y, n_in.weight, self._x, n_in.variance_epsilon)
                 K.int4_gemv(qw, sc, self._x, out=self._qkv)
-            if self._attn_one_launch:
+            if self.kv_bits == 4:
+                K.qk_norm_rope_kv4(self._qkv, a.q_norm.weight, a.k_norm.weight, self.cos, self.sin,
+                                   self.pos, self._q, self._kv4[i], self.nh, self.nkv,
+                                   a.q_norm.variance_epsilon)
+                K.kv4_decode_attention(self._q, self._kv4[i], self.pos, self._o, a.scaling,
+                                       ws=self._attn_ws)
+            elif self._attn_one_launch:
                 K.decode_attention_fused(self._qkv, a.q_norm.weight, a.k_norm.weight, self.cos,
                                          self.sin, self.pos, self.k_cache[i], self.v_cache[i],
                                          self._o, self.nh, self.nkv, a.q_norm.variance_epsilon,
@@ -474,7 +509,23 @@ class DIPDecoder:
         """prefill with the decode kernels' prompt forms around the
         projections: one q|k|v product; q/k norm, rotary embedding and the
         static cache's rows in one launch; residual add and RMSNorm in one; and
-        the head for the last token alone."""
+        the head for the last token alone.  With a 4-bit cache the prompt goes
+        through the layers in parts of even length."""
+        K, plen = self._K, ids.shape[1]
+        parts = 1 if self.kv_bits == 16 else -(-plen // _PROMPT_CHUNK)
+        ends = [plen * (j + 1) // parts for j in range(parts)]
+        for start, end in zip([0] + ends, ends):
+            h, y = self._prefill_part(ids[:, start:end], start)
+        n = self.model.model.norm
+        last = torch.empty(self.hidden, dtype=self.dtype, device=self.device)
+        K.add_rmsnorm(h[-1], y[-1], n.weight, last, n.variance_epsilon)
+        logits = self._head(last.view(1, 1, -1))
+        self.pos.fill_(plen)
+        return logits
+
+    def _prefill_part(self, ids: torch.Tensor, start: int):
+        """The tokens of a prompt from position `start` through every layer
+        (start 0 with a bf16 cache); (residual, last MLP's output)."""
         from qlinear import int4_linear
         K, inner, hd, nh = self._K, self.model.model, self.hd, self.nh
         plen = ids.shape[1]
@@ -483,26 +534,30 @@ class DIPDecoder:
         x = y = None
         for i, L in enumerate(self.layers):
             a, n_in, pn = L.self_attn, L.input_layernorm, L.post_attention_layernorm
-            kc, vc = self.k_cache[i], self.v_cache[i]
             # a layer's own, as who calls its MLP may keep it; else the same memory again
             x = None
             x = torch.empty_like(h)
             K.add_rmsnorm_rows(h, y, n_in.weight, x, n_in.variance_epsilon)
             qkv = int4_linear(x, *self._qkv_w[i])
-            K.qk_norm_rope_cache_rows(qkv, a.q_norm.weight, a.k_norm.weight, self.cos, self.sin, q,
-                                      kc, vc, nh, self.nkv, a.q_norm.variance_epsilon)
-            o = F.scaled_dot_product_attention(
-                q.view(1, plen, nh, hd).transpose(1, 2), kc[None, :, :plen], vc[None, :, :plen],
-                is_causal=plen > 1, scale=a.scaling, enable_gqa=nh != self.nkv)
-            o = a.o_proj(o.transpose(1, 2).reshape(1, plen, nh * hd))
+            if self.kv_bits == 4:
+                K.qk_norm_rope_kv4_rows(qkv, a.q_norm.weight, a.k_norm.weight, self.cos, self.sin,
+                                        q, self._kv4[i], nh, self.nkv, a.q_norm.variance_epsilon,
+                                        start=start)
+                o = K.kv4_prompt_attention(q, self._kv4[i], start, None, a.scaling)
+                o = a.o_proj(o.view(1, plen, nh * hd))
+            else:
+                kc, vc = self.k_cache[i], self.v_cache[i]
+                K.qk_norm_rope_cache_rows(qkv, a.q_norm.weight, a.k_norm.weight, self.cos,
+                                          self.sin, q, kc, vc, nh, self.nkv,
+                                          a.q_norm.variance_epsilon)
+                o = F.scaled_dot_product_attention(
+                    q.view(1, plen, nh, hd).transpose(1, 2), kc[None, :, :plen],
+                    vc[None, :, :plen], is_causal=plen > 1, scale=a.scaling,
+                    enable_gqa=nh != self.nkv)
+                o = a.o_proj(o.transpose(1, 2).reshape(1, plen, nh * hd))
             K.add_rmsnorm_rows(h, o.reshape(plen, -1), pn.weight, x, pn.variance_epsilon)
             y = L.mlp(x.view(1, plen, -1)).reshape(plen, -1)
-        n = inner.norm
-        last = torch.empty(self.hidden, dtype=self.dtype, device=self.device)
-        K.add_rmsnorm(h[-1], y[-1], n.weight, last, n.variance_epsilon)
-        logits = self._head(last.view(1, 1, -1))
-        self.pos.fill_(plen)
-        return logits
+        return h, y
 
     # -- one decode step (device-side token and position) ---------------------
     def _body(self) -> torch.Tensor:
@@ -541,13 +596,23 @@ class DIPDecoder:
         return inner.norm(h)
 
     def _head(self, h: torch.Tensor) -> torch.Tensor:
-        """lm_head and the greedy choice, outside any graph: over a full
+        """lm_head and the choice of the token, outside any graph: over a full
         vocabulary both are library calls (a GEMV and a many-workgroup
         reduction) that may clear their own scratch with a memset, which a
         captured graph does not replay reliably."""
         logits = self.model.lm_head(h).view(-1)
-        self.tok.copy_(logits.argmax().view(1))
+        self._choose(logits)
         return logits
+
+    def _choose(self, logits: torch.Tensor) -> None:
+        """The token of `logits`: the largest, or the one that generate's next
+        number draws."""
+        if self._draw is None:
+            self.tok.copy_(logits.argmax().view(1))
+            return
+        import _dip_hip as K
+        numbers, how = self._draw
+        K.sample(logits.view(1, -1), next(numbers), out=self.tok, **how)
 
     @torch.no_grad()
     def step(self) -> torch.Tensor:
@@ -588,20 +653,46 @@ class DIPDecoder:
         cache = DynamicCache(config=self.model.config)
         out = self.model(input_ids=ids, past_key_values=cache, use_cache=True)
         for i, layer in enumerate(cache.layers):
+            if self.kv_bits == 4:
+                self._K.kv4_write(layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1),
+                                  self._kv4[i])
+                continue
             self.k_cache[i, :, :plen].copy_(layer.keys[0])
             self.v_cache[i, :, :plen].copy_(layer.values[0])
         logits = out.logits[0, -1]
-        self.tok.copy_(logits.argmax().view(1))
+        self._choose(logits)
         self.pos.fill_(plen)
         return logits
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id=None,
-                 return_logits: bool = False):
-        """Greedy continuation of `input_ids` [1, P]: the prompt followed by up
-        to `max_new_tokens` tokens (cut after the first `eos_token_id`), as
-        HF's generate(do_sample=False) returns it for batch 1.  With
-        `return_logits` also the logits of every generated token."""
+                 return_logits: bool = False, do_sample: bool = False, temperature: float = 1.0,
+                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, generator=None):
+        """Continuation of `input_ids` [1, P]: the prompt followed by up to
+        `max_new_tokens` tokens (cut after the first `eos_token_id`), as HF's
+        generate returns it for batch 1.  Greedy, or with `do_sample` drawn with
+        numbers of `generator` (the device's default one if None): after
+        `temperature`, of the `top_k` likeliest tokens (0: all) the fewest that
+        reach `top_p` of the probability, of those the ones with at least
+        `min_p` of the largest (_dip_hip.sample).  With `return_logits` also the
+        logits of every generated token, before any of these."""
+        if not do_sample:
+            return self._generate(input_ids, max_new_tokens, eos_token_id, return_logits)
+        if self.device.type != "cuda":
+            raise ValueError("drawing tokens needs a GPU")
+        import _dip_hip as K
+        how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        K.check_sampling(**how)
+        u = torch.rand(max(max_new_tokens, 1), generator=generator,
+                       device=self.device if generator is None else generator.device)
+        self._draw = iter(u.to(self.device).split(1)), how
+        try:
+            return self._generate(input_ids, max_new_tokens, eos_token_id, return_logits)
+        finally:
+            self._draw = None
+
+    def _generate(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id,
+                  return_logits: bool):
         ids = input_ids.to(self.device).view(1, -1)
         plen = ids.shape[1]
         if plen + max_new_tokens > self.max_len:
