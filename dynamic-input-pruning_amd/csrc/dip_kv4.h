@@ -24,8 +24,9 @@
 //          a lane of quarter c has scores of in the result of the key MFMAs, so
 //          the softmax's weights are the value MFMA's B operand where they are.
 // In a word, element j (a dimension of a key, a row of a value) is nibble
-// j / 2 + 4 (j % 2): v_bitop3 turns nibbles m and m + 4 into one register of the
-// operand (elements 2 m and 2 m + 1).
+// n = j / 2 + 4 (j % 2), at the bits 4 n + 3 .. of the word (modulo 32): v_bitop3
+// turns nibbles m and m + 4 into one register of the operand (elements 2 m and
+// 2 m + 1), the first pair where it lies, the others after one shift.
 #pragma once
 
 #include "dip_common.h"
@@ -43,8 +44,9 @@ constexpr int kKvBlockWords = 512;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-// Element j of a word, as a shift.
-DIP_DEV int kv4_shift(int j) { return 4 * ((j >> 1) + 4 * (j & 1)); }
+// Element j of a word, as a shift; the last one's nibble wraps around.
+DIP_DEV int kv4_shift(int j) { return 4 * ((j >> 1) + 4 * (j & 1)) + 3; }
+DIP_DEV uint32_t kv4_rotl(uint32_t v, int s) { return __builtin_rotateleft32(v, (uint32_t)s); }
 // The word of a value block that holds dimension d for lane quarter c.
 DIP_DEV int kv4_value_word(int d, int c) {
   return 256 * (d >> 6) + 64 * c + 4 * (d & 15) + ((d >> 4) & 3);
@@ -56,15 +58,17 @@ DIP_DEV int kv4_row_elem(int r) { return 4 * (r >> 4) + (r & 3); }
 // One word as an MFMA operand of 8 bf16 values 1.5 + q / 16 (exact).
 DIP_DEV bf16x8_t kv4_biased(uint32_t w) {
   u32x4_t r;
-  r.x = ((w << 3) & kPairMask) ^ kPairMagicFlip;
-  r.y = ((w >> 1) & kPairMask) ^ kPairMagicFlip;
-  r.z = ((w >> 5) & kPairMask) ^ kPairMagicFlip;
-  r.w = ((w >> 9) & kPairMask) ^ kPairMagicFlip;
+  r.x = (w & kPairMask) ^ kPairMagicFlip;
+  r.y = ((w >> 4) & kPairMask) ^ kPairMagicFlip;
+  r.z = ((w >> 8) & kPairMask) ^ kPairMagicFlip;
+  r.w = (__builtin_amdgcn_alignbit(w, w, 12) & kPairMask) ^ kPairMagicFlip;
   return __builtin_bit_cast(bf16x8_t, r);
 }
 
 // Nibble at `shift` as a signed number.
-DIP_DEV int kv4_nibble(uint32_t w, int shift) { return (int)(w << (28 - shift)) >> 28; }
+DIP_DEV int kv4_nibble(uint32_t w, int shift) {
+  return (int)kv4_rotl(w, (28 - shift) & 31) >> 28;
+}
 
 // Max over aligned groups of 16 lanes of whole numbers.
 DIP_DEV uint32_t group_umax16(uint32_t v) {

@@ -71,9 +71,9 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
       if (!in[j]) continue;
       const int64_t row = block * kKvBlock + 16 * (j >> 2) + 4 * c + (j & 3);
       const Kv4Pair p = kv4_quantize(pair[j]);
-      word[0] |= p.q0 << kv4_shift(j);
-      word[1] |= p.q1 << kv4_shift(j);
-      mask |= 15u << kv4_shift(j);
+      word[0] |= kv4_rotl(p.q0, kv4_shift(j));
+      word[1] |= kv4_rotl(p.q1, kv4_shift(j));
+      mask |= kv4_rotl(15u, kv4_shift(j));
       if ((l & 15) == 0)
         a.sc[((size_t)head * a.max_len + row) * kKvScaleVals + kKvGroups + (l >> 4)] =
             (uint16_t)p.scale;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
   const int kvh = kNorm ? head - a.nh : head;
   const Kv4Pair p = kv4_quantize(pair);
   // dimensions 8 (l / 4) .. + 7 are four lanes' pairs
-  uint32_t w = (p.q0 << kv4_shift(2 * (l & 3))) | (p.q1 << kv4_shift(2 * (l & 3) + 1));
+  uint32_t w = kv4_rotl(p.q0 | (p.q1 << 16), kv4_shift(2 * (l & 3)));
   w |= (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0xB1, 0xF, 0xF, true);
   w |= (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x4E, 0xF, 0xF, true);
   const size_t at = (size_t)kvh * a.max_len + row;

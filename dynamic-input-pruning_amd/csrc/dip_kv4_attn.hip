@@ -3,6 +3,8 @@
 // tokens.
 #include "dip_kv4.h"
 
+#include <type_traits>
+
 namespace dip {
 namespace {
 
@@ -40,6 +42,8 @@ DIP_DEV int blocks_per_wave(int rows, int waves) {
   return max(1, (blocks + waves - 1) / waves);
 }
 
+// 2^x; results below the normal range are 0.
+DIP_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 DIP_DEV float scale_lo(uint32_t w) { return __uint_as_float(w << 16); }
 DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
@@ -79,10 +83,9 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
   const int tok = col / a.group, head = kvh * a.group + col % a.group;
   const bool on = tok < a.tokens;
   const int limit = on ? rows_at(first + tok, a.max_len) : 0;
-  // rows that every column of the tile attends
-  const int sure = on && tile * kCols + kCols <= a.tokens * a.group
-                       ? rows_at(first + tile * kCols / a.group, a.max_len)
-                       : 0;
+  // rows that every column of the tile attends (columns without a token, whose
+  // queries are 0, take them too: nothing reads their sums)
+  const int sure = rows_at(first + tile * kCols / a.group, a.max_len);
   bf16x8_t bq[kKvGroups];
   float qs[kKvGroups];
   {
@@ -113,16 +116,22 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
   for (int g = 0; g < kKvGroups; ++g) bias[g] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, den = 0.f;  // den: this lane's rows only
 
-  for (int b = b0; b < b1; ++b) {
+  struct Raw {
     uint4 kw[2], vw[2], sw[2][4];
+  };
+  auto load = [&](Raw& x, int b) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      kw[t] = reinterpret_cast<const uint4*>(kc)[(size_t)(b * kKvBlock + 16 * t + l16) * 4 + c];
-      vw[t] = reinterpret_cast<const uint4*>(vc)[(size_t)b * (kKvBlockWords / 4) + 64 * t + l];
+      x.kw[t] = reinterpret_cast<const uint4*>(kc)[(size_t)(b * kKvBlock + 16 * t + l16) * 4 + c];
+      x.vw[t] = reinterpret_cast<const uint4*>(vc)[(size_t)b * (kKvBlockWords / 4) + 64 * t + l];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sw[t][r] = sc[b * kKvBlock + 16 * t + 4 * c + r];
+      for (int r = 0; r < 4; ++r) x.sw[t][r] = sc[b * kKvBlock + 16 * t + 4 * c + r];
     }
-    const bool full = (b + 1) * kKvBlock <= sure;
+  };
+  auto block = [&](const Raw& x, int b, auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
+    const uint4(&kw)[2] = x.kw, (&vw)[2] = x.vw;
+    const uint4(&sw)[2][4] = x.sw;
     float s[2][4];
     bool ok[2][4];
     float mx = -INFINITY;
@@ -142,14 +151,14 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        ok[t][r] = full || b * kKvBlock + 16 * t + 4 * c + r < limit;
+        ok[t][r] = !kMasked || b * kKvBlock + 16 * t + 4 * c + r < limit;
         s[t][r] = ok[t][r] ? v[r] * sc2 : -INFINITY;
         mx = fmaxf(mx, s[t][r]);
       }
     }
     mx = fmaxf(m, row_pair_max32(row_pair_max16(mx)));
     if (__any(mx > m)) {
-      const float f = m == -INFINITY ? 0.f : exp2f(m - mx);  // what the sums so far are worth
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);  // what the sums so far are worth
       den *= f;
 #pragma unroll
       for (int t = 0; t < 8; ++t)
@@ -167,7 +176,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        p[t][r] = ok[t][r] ? exp2f(s[t][r] - base) : 0.f;
+        p[t][r] = ok[t][r] ? fast_exp2(s[t][r] - base) : 0.f;
         den += p[t][r];
       }
     bf16x8_t va[8];
@@ -197,6 +206,25 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
       for (int t = 2 * g; t < 2 * g + 2; ++t)
         acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[t], bp, acc[t], 0, 0, 0);
       bias[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, bp, bias[g], 0, 0, 0);
+    }
+  };
+  // two blocks in turn, the next one's loads in flight behind this one's work
+  // (clamped, so that none is behind a branch and waited for with the others)
+  if (b0 < b1) {
+    const int full = min(b1, max(b0, sure / kKvBlock));  // blocks before it need no mask
+    Raw x, y;
+    load(x, b0);
+    int b = b0;
+    for (; b + 2 <= full; b += 2) {
+      load(y, b + 1);
+      block(x, b, std::false_type{});
+      load(x, min(b + 2, b1 - 1));
+      block(y, b + 1, std::false_type{});
+    }
+    for (; b < b1; ++b) {
+      load(y, min(b + 1, b1 - 1));
+      block(x, b, std::true_type{});
+      x = y;
     }
   }
 
@@ -228,7 +256,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
     for (int w = 0; w < W; ++w) {
       // a wave without rows has m = -inf and sums 0; one whose scores are all NaN
       // has m = -inf and NaN sums, which must count
-      const float f = wm[w][cl] == -INFINITY ? 1.f : exp2f(wm[w][cl] - mx);
+      const float f = wm[w][cl] == -INFINITY ? 1.f : fast_exp2(wm[w][cl] - mx);
       sum = fmaf(f, wl[w][cl], sum);
       o0 = fmaf(f, wacc[w][cl][d], o0);
       o1 = fmaf(f, wacc[w][cl][d + 1], o1);
@@ -251,32 +279,67 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
   }
 }
 
-// The splits of one column added up, in their order: one workgroup per (kv
-// head, column).
-__global__ __launch_bounds__(kKvHeadDim) void kv4_combine_kernel(Kv4AttnArgs a, int waves) {
+// The splits of one column added up, in a fixed order: one workgroup per (kv
+// head, column), kCombine groups of 128 threads, each of which takes every
+// kCombine-th split's value sums; its first loads are in flight while the splits'
+// weights are worked out.
+constexpr int kCombine = 8, kAhead = 8;
+
+__global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4AttnArgs a,
+                                                                            int waves) {
   __shared__ float wgt[kMaxSplits];
-  const int kvh = blockIdx.x % a.nkv, cc = blockIdx.x / a.nkv;
-  const int tile = cc / kCols, cl = cc % kCols, d = threadIdx.x;
+  __shared__ float red[kCombine * kKvHeadDim / 64][2];
+  __shared__ float so[kCombine][kKvHeadDim];
+  const int kvh = blockIdx.x % a.nkv, cc = blockIdx.x / a.nkv, tid = threadIdx.x;
+  const int tile = cc / kCols, cl = cc % kCols, d = tid % kKvHeadDim, p = tid / kKvHeadDim;
   const int64_t first = a.pos ? *a.pos : a.start;
   const int rows = tile_rows(a, first, tile);
   const int per = waves * blocks_per_wave(rows, a.splits * waves);  // blocks of a split
   const int ns = ((rows + kKvBlock - 1) / kKvBlock + per - 1) / per;
+  const size_t o = ((size_t)(cc / a.group) * a.nkv * a.group + kvh * a.group + cc % a.group) *
+                   kKvHeadDim;
+  if (ns == 0) {  // no rows
+    if (tid < kKvHeadDim) a.out[o + tid] = 0;
+    return;
+  }
   const float* base = a.part + ((size_t)(tile * a.nkv + kvh) * a.splits * kCols + cl) * kPart;
   const size_t stride = (size_t)kCols * kPart;
-  float mx = -INFINITY;
-  for (int s = 0; s < ns; ++s) mx = fmaxf(mx, base[s * stride]);
-  for (int s = d; s < ns; s += kKvHeadDim) {
-    const float ms = base[s * stride];
-    wgt[s] = ms == -INFINITY ? 1.f : exp2f(ms - mx);
-  }
+  const float ms = tid < ns ? base[tid * stride] : -INFINITY;
+  const float ls = tid < ns ? base[tid * stride + 1] : 0.f;
+  float v[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) v[u] = base[min(p + kCombine * u, ns - 1) * stride + 2 + d];
+  float mx = group_max<64>(ms);
+  if ((tid & 63) == 0) red[tid >> 6][0] = mx;
   __syncthreads();
-  float sum = 0.f, o = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    sum = fmaf(wgt[s], base[s * stride + 1], sum);
-    o = fmaf(wgt[s], base[s * stride + 2 + d], o);
+#pragma unroll
+  for (int w = 0; w < kCombine * kKvHeadDim / 64; ++w) mx = fmaxf(mx, red[w][0]);
+  // (a split without a score above -inf has sums of 0, or NaN, which must count)
+  const float f = tid >= ns ? 0.f : ms == -INFINITY ? 1.f : fast_exp2(ms - mx);
+  if (tid < kMaxSplits) wgt[tid] = f;
+  const float part = group_sum<64>(f * ls);
+  if ((tid & 63) == 0) red[tid >> 6][1] = part;
+  __syncthreads();
+  float acc = 0.f;
+  for (int s0 = p; s0 < ns; s0 += kCombine * kAhead) {
+    if (s0 != p) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) v[u] = base[min(s0 + kCombine * u, ns - 1) * stride + 2 + d];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (s0 + kCombine * u < ns) acc = fmaf(wgt[s0 + kCombine * u], v[u], acc);
   }
-  a.out[((size_t)(cc / a.group) * a.nkv * a.group + kvh * a.group + cc % a.group) * kKvHeadDim +
-        d] = (uint16_t)f32_to_bf16(sum == 0.f ? 0.f : o / sum);
+  so[p][d] = acc;
+  __syncthreads();
+  if (tid < kKvHeadDim) {
+    float sum = 0.f, r = 0.f;
+#pragma unroll
+    for (int w = 0; w < kCombine * kKvHeadDim / 64; ++w) sum += red[w][1];
+#pragma unroll
+    for (int w = 0; w < kCombine; ++w) r += so[w][tid];
+    a.out[o + tid] = (uint16_t)f32_to_bf16(sum == 0.f ? 0.f : r / sum);
+  }
 }
 
 constexpr int kWaves = 4;
@@ -317,7 +380,7 @@ int launch_attn(Kv4AttnArgs a, int64_t tiles, hipStream_t stream) {
                      a);
   if (a.splits > 1)
     hipLaunchKernelGGL(kv4_combine_kernel, dim3((unsigned)(a.tokens * a.group * a.nkv)),
-                       dim3(kKvHeadDim), 0, stream, a, kWaves);
+                       dim3(kCombine * kKvHeadDim), 0, stream, a, kWaves);
   return hip_status(hipGetLastError());
 }
 
