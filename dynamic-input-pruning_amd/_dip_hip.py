@@ -19,7 +19,6 @@ import math
 import os
 import threading
 from pathlib import Path
-from typing import NamedTuple
 
 import torch
 
@@ -872,19 +871,41 @@ KV4_GROUP = 32   # dimensions of a row that share a scale
 KV4_BLOCK = 32   # rows of a block: max_len is a multiple
 
 
-class KV4Cache(NamedTuple):
-    """A 4-bit key/value cache (kv4_cache makes one): one layer's arrays, or
-    with a leading dimension every layer's (``layer(i)`` is one of them)."""
-    k: torch.Tensor       # int8 [n_kv_heads, max_len, 64]
-    v: torch.Tensor       # int8 [n_kv_heads, max_len / 32, 2048]
-    scales: torch.Tensor  # bf16 [n_kv_heads, max_len, 2, 4]
+class KV4Cache:
+    """A 4-bit key/value cache (kv4_cache makes one): one layer's arrays, or with
+    a leading dimension every layer's, of which ``layer(i)`` is one.
+
+      k       int8 [n_kv_heads, max_len, 64]
+      v       int8 [n_kv_heads, max_len / 32, 2048]
+      scales  bf16 [n_kv_heads, max_len, 2, 4]
+
+    The arrays are checked here, once, so that a call need not."""
+
+    __slots__ = ("k", "v", "scales", "device", "n_kv_heads", "max_len", "one_layer")
+
+    def __init__(self, k, v, scales):
+        dev = _dev(k, v, scales)
+        if k.dim() not in (3, 4) or k.shape[-2] % KV4_BLOCK or k.shape[-1] != 64 or not k.numel():
+            raise RuntimeError("cache arrays must be as kv4_cache makes them")
+        *lead, nkv, max_len, _ = k.shape
+        for t, dt, shape in ((k, torch.int8, (max_len, 64)),
+                             (v, torch.int8, (max_len // KV4_BLOCK, 2048)),
+                             (scales, torch.bfloat16, (max_len, 2, 4))):
+            if t.dtype != dt or tuple(t.shape) != (*lead, nkv, *shape) or not t.is_contiguous() \
+                    or t.data_ptr() % 16:
+                raise RuntimeError("cache arrays must be as kv4_cache makes them")
+        self.k, self.v, self.scales = k, v, scales
+        self.device, self.n_kv_heads, self.max_len = dev, nkv, max_len
+        self.one_layer = not lead
 
     def layer(self, i: int) -> "KV4Cache":
         return KV4Cache(self.k[i], self.v[i], self.scales[i])
 
-    @property
-    def max_len(self) -> int:
-        return self.k.shape[-2]
+    def __iter__(self):
+        return iter((self.k, self.v, self.scales))
+
+    def _replace(self, **arrays) -> "KV4Cache":
+        return KV4Cache(**{"k": self.k, "v": self.v, "scales": self.scales, **arrays})
 
 
 def kv4_cache(n_kv_heads: int, max_len: int, device="cuda", layers=None) -> KV4Cache:
@@ -900,24 +921,23 @@ def kv4_cache(n_kv_heads: int, max_len: int, device="cuda", layers=None) -> KV4C
 
 
 def _kv4(cache: KV4Cache, *ts):
-    """(device, n_kv_heads, max_len) of one layer's cache, all on one device."""
-    k, v, sc = cache
-    dev = _dev(k, v, sc, *ts)
-    if k.dim() != 3 or k.shape[1] % KV4_BLOCK or k.shape[2] != 64:
-        raise RuntimeError("cache must be one layer's arrays, as kv4_cache makes them")
-    nkv, max_len, _ = k.shape
-    for t, dt, shape in ((k, torch.int8, (nkv, max_len, 64)),
-                         (v, torch.int8, (nkv, max_len // KV4_BLOCK, 2048)),
-                         (sc, torch.bfloat16, (nkv, max_len, 2, 4))):
-        if t.dtype != dt or t.shape != shape or not t.is_contiguous() or t.data_ptr() % 16:
-            raise RuntimeError("cache must be one layer's arrays, as kv4_cache makes them")
-    return dev, nkv, max_len
+    """The device of one layer's cache, which the tensors must share."""
+    if not isinstance(cache, KV4Cache) or not cache.one_layer:
+        raise RuntimeError("cache must be one layer's KV4Cache")
+    dev = cache.device
+    for t in ts:
+        if t.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
+    return dev
+
+
+_same_device = contextlib.nullcontext()
 
 
 def _on(dev: torch.device):
     """The device the library launches on, where it is not the current one."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if dev.index is None or dev.index == torch._C._cuda_getDevice():
+        return _same_device
     return torch.cuda.device(dev)
 
 
@@ -931,7 +951,7 @@ def _rows_in(start: int, n: int, max_len: int):
 def kv4_write(k, v, cache: KV4Cache, start: int = 0) -> None:
     """Quantise k and v (bf16 [tokens, n_kv_heads, 128], any strides of the first
     two dimensions) into rows start .. of one layer's cache."""
-    dev, nkv, max_len = _kv4(cache, k, v)
+    dev, nkv, max_len = _kv4(cache, k, v), cache.n_kv_heads, cache.max_len
     if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (nkv, 128) \
             or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise RuntimeError(f"k and v must be bf16 [tokens, {nkv}, 128]")
@@ -943,37 +963,46 @@ def kv4_write(k, v, cache: KV4Cache, start: int = 0) -> None:
             and not t.data_ptr() & 3 else t.clone(memory_format=torch.contiguous_format)
             for t in (k, v))
     with _on(dev):
-        _check(lib.dip_kv4_write(_ptr(k), _ptr(v), k.stride(0), k.stride(1), v.stride(0),
-                                 v.stride(1), _ptr(cache.k), _ptr(cache.v), _ptr(cache.scales),
-                                 start, n, nkv, 128, max_len, _stream(dev)), "dip_kv4_write")
+        _check(lib.dip_kv4_write(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
+                                 v.stride(0), v.stride(1), cache.k.data_ptr(),
+                                 cache.v.data_ptr(), cache.scales.data_ptr(), start, n, nkv, 128,
+                                 max_len, _stream(dev)), "dip_kv4_write")
 
 
 def kv4_read(cache: KV4Cache, start: int = 0, rows=None):
     """(k, v) bf16 [rows, n_kv_heads, 128]: what rows start .. (to the end of the
     cache by default) of one layer's cache stand for, exactly."""
-    dev, nkv, max_len = _kv4(cache)
+    dev, nkv, max_len = _kv4(cache), cache.n_kv_heads, cache.max_len
     start, n = _rows_in(start, max_len - int(start) if rows is None else rows, max_len)
-    k, v = torch.empty(2, n, nkv, 128, dtype=torch.bfloat16, device=dev)
+    k, v = torch.empty(2, n, nkv, 128, dtype=torch.bfloat16, device=dev).unbind(0)
     with _on(dev):
-        _check(lib.dip_kv4_read(_ptr(cache.k), _ptr(cache.v), _ptr(cache.scales), _ptr(k), _ptr(v),
-                                start, n, nkv, 128, max_len, _stream(dev)), "dip_kv4_read")
+        _check(lib.dip_kv4_read(cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
+                                k.data_ptr(), v.data_ptr(), start, n, nkv, 128, max_len,
+                                _stream(dev)), "dip_kv4_read")
     return k, v
 
 
-def _qk_kv4_check(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads, n_kv_heads, tokens):
-    dev, nkv, max_len = _kv4(cache, qkv, q_norm_w, k_norm_w, cos, sin, q_out)
+def _dense(t: torch.Tensor, n: int, name: str) -> int:
+    """The pointer of a contiguous, 16-byte aligned bf16 tensor of n values."""
+    p = t.data_ptr()
+    if t.dtype is not torch.bfloat16 or t.numel() != n or not t.is_contiguous() or p & 15:
+        raise RuntimeError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor of {n} "
+                           "values")
+    return p
+
+
+def _qk_kv4_ptrs(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads, n_kv_heads, tokens):
+    """(device, rows of the tables, pointers of the first five and of q_out)."""
+    dev, nkv = _kv4(cache, qkv, q_norm_w, k_norm_w, cos, sin, q_out), cache.n_kv_heads
     if n_kv_heads != nkv or n_heads < 1:
         raise RuntimeError(f"the cache has {nkv} kv heads, the call {n_kv_heads}")
-    _bf16_vec(qkv, tokens * (n_heads + 2 * nkv) * 128, "qkv")
-    _bf16_vec(q_norm_w, 128, "q_norm_w")
-    _bf16_vec(k_norm_w, 128, "k_norm_w")
-    _bf16_vec(q_out, tokens * n_heads * 128, "q_out")
-    for name, t in (("cos", cos), ("sin", sin)):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.shape[-1] != 128:
-            raise RuntimeError(f"{name} must be a contiguous bf16 [rows, 128] table")
-    if cos.shape != sin.shape:
-        raise RuntimeError("cos and sin must have as many rows")
-    return dev, max_len, cos.numel() // 128
+    table = cos.numel() // 128
+    if cos.shape != sin.shape or cos.shape[-1] != 128:
+        raise RuntimeError("cos and sin must be tables of as many rows of 128 values")
+    return (dev, table, _dense(qkv, tokens * (n_heads + 2 * nkv) * 128, "qkv"),
+            _dense(q_norm_w, 128, "q_norm_w"), _dense(k_norm_w, 128, "k_norm_w"),
+            _dense(cos, table * 128, "cos"), _dense(sin, table * 128, "sin"),
+            _dense(q_out, tokens * n_heads * 128, "q_out"))
 
 
 def qk_norm_rope_kv4(qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out, cache: KV4Cache,
@@ -981,16 +1010,16 @@ def qk_norm_rope_kv4(qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out, cache: KV4Ca
     """qk_norm_rope_cache into one layer's 4-bit cache: one token's q|k|v at the
     position in `pos` (int64, on the device); the tables must have the cache's
     rows."""
-    dev, max_len, table = _qk_kv4_check(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads,
-                                        n_kv_heads, 1)
-    if table < max_len:
-        raise RuntimeError(f"cos and sin have {table} rows, the cache {max_len}")
+    dev, table, qkv_p, qw, kw, cos_p, sin_p, q_p = _qk_kv4_ptrs(
+        qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads, n_kv_heads, 1)
+    if table < cache.max_len:
+        raise RuntimeError(f"cos and sin have {table} rows, the cache {cache.max_len}")
     _pos_tensor(pos, dev)
     with _on(dev):
-        _check(lib.dip_qk_norm_rope_kv4(_ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos),
-                                        _ptr(sin), _ptr(pos), _ptr(q_out), _ptr(cache.k),
-                                        _ptr(cache.v), _ptr(cache.scales), n_heads, n_kv_heads,
-                                        128, max_len, float(eps), _stream(dev)),
+        _check(lib.dip_qk_norm_rope_kv4(qkv_p, qw, kw, cos_p, sin_p, pos.data_ptr(), q_p,
+                                        cache.k.data_ptr(), cache.v.data_ptr(),
+                                        cache.scales.data_ptr(), n_heads, n_kv_heads, 128,
+                                        cache.max_len, eps, _stream(dev)),
                "dip_qk_norm_rope_kv4")
     return q_out
 
@@ -1000,40 +1029,29 @@ def qk_norm_rope_kv4_rows(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache: KV4Ca
     """qk_norm_rope_kv4 for a prompt's tokens: row t of qkv [tokens, ..] at
     position start + t, q to row t of q_out."""
     tokens = qkv.shape[0]
-    dev, max_len, table = _qk_kv4_check(qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads,
-                                        n_kv_heads, tokens)
-    start, tokens = _rows_in(start, tokens, min(max_len, table))
+    dev, table, qkv_p, qw, kw, cos_p, sin_p, q_p = _qk_kv4_ptrs(
+        qkv, q_norm_w, k_norm_w, cos, sin, q_out, cache, n_heads, n_kv_heads, tokens)
+    start, tokens = _rows_in(start, tokens, min(cache.max_len, table))
     with _on(dev):
-        _check(lib.dip_qk_norm_rope_kv4_rows(_ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(cos),
-                                             _ptr(sin), start, _ptr(q_out), _ptr(cache.k),
-                                             _ptr(cache.v), _ptr(cache.scales), tokens, n_heads,
-                                             n_kv_heads, 128, max_len, float(eps), _stream(dev)),
+        _check(lib.dip_qk_norm_rope_kv4_rows(qkv_p, qw, kw, cos_p, sin_p, start, q_p,
+                                             cache.k.data_ptr(), cache.v.data_ptr(),
+                                             cache.scales.data_ptr(), tokens, n_heads, n_kv_heads,
+                                             128, cache.max_len, eps, _stream(dev)),
                "dip_qk_norm_rope_kv4_rows")
     return q_out
 
 
-def _attn_out(q, out, n: int, dev):
-    if q.dtype != torch.bfloat16 or not q.is_contiguous() or q.data_ptr() % 16:
-        raise RuntimeError("q must be a contiguous, 16-byte aligned bf16 tensor")
-    if out is None:
-        return torch.empty_like(q)
-    if out.device != dev:
-        raise RuntimeError("out must be on q's device")
-    return _bf16_vec(out, n, "out")
-
-
 def _scratch(nbytes: int, ws, dev, name: str):
-    """The caller's workspace, or the caching allocator's, so that calls on several
-    streams and captured graphs each have their own (nothing has to be cleared)."""
+    """(pointer, bytes, tensor) of the caller's workspace, or the caching
+    allocator's, so that calls on several streams and captured graphs each have
+    their own (nothing has to be cleared)."""
     if ws is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    if ws.device != dev or not ws.is_contiguous() or ws.numel() * ws.element_size() < nbytes:
+        if not nbytes:
+            return None, 0, None
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    elif ws.device != dev or not ws.is_contiguous() or ws.numel() * ws.element_size() < nbytes:
         raise RuntimeError(f"{name} workspace too small")
-    return ws
-
-
-def _nbytes(ws) -> int:
-    return 0 if ws is None else ws.numel() * ws.element_size()
+    return ws.data_ptr(), ws.numel() * ws.element_size(), ws
 
 
 def kv4_decode_attention_workspace_bytes(n_heads: int, n_kv_heads: int, max_len: int) -> int:
@@ -1043,19 +1061,25 @@ def kv4_decode_attention_workspace_bytes(n_heads: int, n_kv_heads: int, max_len:
 def kv4_decode_attention(q, cache: KV4Cache, pos, out, scale: float, ws=None):
     """Grouped-query attention of one token (q, n_heads * 128 values) over rows
     0 .. pos of one layer's 4-bit cache -> out (new if None)."""
-    dev, nkv, max_len = _kv4(cache, q)
-    nh = q.numel() // 128
-    if q.numel() != nh * 128 or nh < 1 or nh % nkv:
+    dev, nkv, max_len, n = _kv4(cache, q), cache.n_kv_heads, cache.max_len, q.numel()
+    nh = n // 128
+    if n != nh * 128 or nh < 1 or nh % nkv:
         raise RuntimeError(f"q must hold a multiple of {nkv} heads of 128 values")
+    q_p = _dense(q, n, "q")
     _pos_tensor(pos, dev)
-    out = _attn_out(q, out, nh * 128, dev)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.device != dev:
+        raise RuntimeError("out must be on q's device")
     with _on(dev):
-        ws = _scratch(kv4_decode_attention_workspace_bytes(nh, nkv, max_len), ws, dev,
-                      "attention")
-        _check(lib.dip_kv4_decode_attention(_ptr(q), _ptr(cache.k), _ptr(cache.v),
-                                            _ptr(cache.scales), _ptr(pos), _ptr(out), nh, nkv,
-                                            128, max_len, float(scale), _ptr(ws), _nbytes(ws),
-                                            _stream(dev)), "dip_kv4_decode_attention")
+        ws_p, nbytes, ws = _scratch(
+            lib.dip_kv4_decode_attention_workspace_size(nh, nkv, 128, max_len), ws, dev,
+            "attention")
+        _check(lib.dip_kv4_decode_attention(q_p, cache.k.data_ptr(), cache.v.data_ptr(),
+                                            cache.scales.data_ptr(), pos.data_ptr(),
+                                            _dense(out, n, "out"), nh, nkv, 128, max_len, scale,
+                                            ws_p, nbytes, _stream(dev)),
+               "dip_kv4_decode_attention")
     return out
 
 
@@ -1063,21 +1087,25 @@ def kv4_prompt_attention(q, cache: KV4Cache, start: int, out, scale: float, ws=N
     """Grouped-query attention of a prompt's tokens (q [tokens, n_heads * 128] at
     positions start ..), token t over rows 0 .. start + t of one layer's 4-bit
     cache -> out (new if None)."""
-    dev, nkv, max_len = _kv4(cache, q)
+    dev, nkv, max_len, n = _kv4(cache, q), cache.n_kv_heads, cache.max_len, q.numel()
     if q.dim() != 2 or q.shape[1] % (128 * nkv) or not q.shape[1]:
         raise RuntimeError(f"q must be [tokens, a multiple of {nkv} heads of 128 values]")
-    tokens, nh = q.shape[0], q.shape[1] // 128
-    start, tokens = _rows_in(start, tokens, max_len)
-    out = _attn_out(q, out, q.numel(), dev)
+    nh = q.shape[1] // 128
+    start, tokens = _rows_in(start, q.shape[0], max_len)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.device != dev:
+        raise RuntimeError("out must be on q's device")
+    q_p, out_p = _dense(q, n, "q"), _dense(out, n, "out")
     if tokens == 0:
         return out
     with _on(dev):
-        ws = _scratch(lib.dip_kv4_prompt_attention_workspace_size(tokens, start, nh, nkv, 128), ws,
-                      dev, "attention")
-        _check(lib.dip_kv4_prompt_attention(_ptr(q), _ptr(cache.k), _ptr(cache.v),
-                                            _ptr(cache.scales), start, _ptr(out), tokens, nh,
-                                            nkv, 128, max_len, float(scale), _ptr(ws),
-                                            _nbytes(ws), _stream(dev)),
+        ws_p, nbytes, ws = _scratch(
+            lib.dip_kv4_prompt_attention_workspace_size(tokens, start, nh, nkv, 128), ws, dev,
+            "attention")
+        _check(lib.dip_kv4_prompt_attention(q_p, cache.k.data_ptr(), cache.v.data_ptr(),
+                                            cache.scales.data_ptr(), start, out_p, tokens, nh,
+                                            nkv, 128, max_len, scale, ws_p, nbytes, _stream(dev)),
                "dip_kv4_prompt_attention")
     return out
 
@@ -1111,26 +1139,30 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     NaN counts as -inf; a row of nothing else gives token 0, probability 0."""
     check_sampling(temperature, top_k, top_p, min_p)
     dev = _dev(logits, u)
-    if logits.dtype not in _LOGIT_TYPES or logits.dim() != 2 or logits.shape[1] < 1:
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    if kind is None or logits.dim() != 2 or logits.shape[1] < 1:
         raise RuntimeError("logits must be bf16, fp16 or fp32 [rows, vocab]")
     rows, vocab = logits.shape
     if vocab > 1 and logits.stride(1) != 1 or logits.stride(0) < 0:
         logits = logits.contiguous()
-    u = _want(u.reshape(-1), torch.float32, "u", (rows,))
+    if u.dtype is not torch.float32 or u.numel() != rows:
+        raise RuntimeError(f"u must be a float32 tensor of {rows} values")
+    u = u.contiguous()
     token = torch.empty(rows, dtype=torch.int64, device=dev) if out is None else out
     prob = torch.empty(rows, dtype=torch.float32, device=dev) if prob is None else prob
     for name, t, dt in (("out", token, torch.int64), ("prob", prob, torch.float32)):
-        if t.dtype != dt or t.numel() != rows or not t.is_contiguous() or t.device != dev:
+        if t.dtype is not dt or t.numel() != rows or not t.is_contiguous() or t.device != dev:
             raise RuntimeError(f"{name} must be a contiguous {dt} tensor of {rows} values on the "
                                "logits' device")
     if rows == 0:
         return token, prob
     with _on(dev):
-        ws = _scratch(lib.dip_sample_workspace_size(rows, vocab), ws, dev, "sampling")
-        _check(lib.dip_sample(_ptr(logits), _LOGIT_TYPES[logits.dtype], rows, vocab,
-                              logits.stride(0), _ptr(u), float(temperature), int(top_k),
-                              float(top_p), float(min_p), _ptr(token), _ptr(prob), _ptr(ws),
-                              _nbytes(ws), _stream(dev)), "dip_sample")
+        ws_p, nbytes, ws = _scratch(lib.dip_sample_workspace_size(rows, vocab), ws, dev,
+                                    "sampling")
+        _check(lib.dip_sample(logits.data_ptr(), kind, rows, vocab, logits.stride(0),
+                              u.data_ptr(), temperature, int(top_k), top_p, min_p,
+                              token.data_ptr(), prob.data_ptr(), ws_p, nbytes, _stream(dev)),
+               "dip_sample")
     return token, prob
 
 

@@ -342,14 +342,21 @@ __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4A
   }
 }
 
-constexpr int kWaves = 4;
+// How many waves a workgroup has and how many workgroups share a tile's rows.
+struct Split {
+  int waves, splits;
+};
 
-// Splits of the cache's rows for `tiles` tiles of columns: enough workgroups to
-// fill the chip about twice over, a block of rows per wave at least.
-inline int splits_for(int64_t tiles, int64_t nkv, int64_t max_rows) {
+// Up to kShort rows one workgroup of 8 waves takes a tile's and writes the result
+// itself; longer caches are spread over enough workgroups to fill the chip about
+// twice over, a block of rows per wave at least, and added up in a second launch.
+constexpr int64_t kShort = 1024;
+
+inline Split split_for(int64_t tiles, int64_t nkv, int64_t max_rows) {
+  if (max_rows <= kShort) return {8, 1};
   const int64_t want = (2 * device_cus() + tiles * nkv - 1) / (tiles * nkv);
-  const int64_t most = (max_rows + kKvBlock * kWaves - 1) / (kKvBlock * kWaves);
-  return (int)max((int64_t)1, min(min(want, most), (int64_t)kMaxSplits));
+  const int64_t most = (max_rows + kKvBlock * 4 - 1) / (kKvBlock * 4);
+  return {4, (int)max((int64_t)1, min(min(want, most), (int64_t)kMaxSplits))};
 }
 
 inline int64_t col_tiles(int64_t tokens, int64_t group) {
@@ -373,14 +380,17 @@ int check_attn(const void* q, const void* kc, const void* vc, const void* sc, co
   return DIP_OK;
 }
 
-int launch_attn(Kv4AttnArgs a, int64_t tiles, hipStream_t stream) {
+int launch_attn(Kv4AttnArgs a, int64_t tiles, Split sp, hipStream_t stream) {
+  a.splits = sp.splits;
   const int64_t grid = tiles * a.nkv * a.splits;
   if (grid > INT32_MAX || (int64_t)a.tokens * a.group * a.nkv > INT32_MAX) return DIP_ERR_SHAPE;
-  hipLaunchKernelGGL((kv4_attn_kernel<kWaves>), dim3((unsigned)grid), dim3(kWaves * 64), 0, stream,
-                     a);
+  if (sp.waves == 8)
+    hipLaunchKernelGGL((kv4_attn_kernel<8>), dim3((unsigned)grid), dim3(512), 0, stream, a);
+  else
+    hipLaunchKernelGGL((kv4_attn_kernel<4>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (a.splits > 1)
     hipLaunchKernelGGL(kv4_combine_kernel, dim3((unsigned)(a.tokens * a.group * a.nkv)),
-                       dim3(kCombine * kKvHeadDim), 0, stream, a, kWaves);
+                       dim3(kCombine * kKvHeadDim), 0, stream, a, sp.waves);
   return hip_status(hipGetLastError());
 }
 
@@ -395,7 +405,7 @@ extern "C" size_t dip_kv4_decode_attention_workspace_size(int64_t n_heads, int64
       max_len <= 0)
     return 0;
   const int64_t tiles = col_tiles(1, n_heads / n_kv_heads);
-  return part_bytes(tiles, n_kv_heads, splits_for(tiles, n_kv_heads, max_len));
+  return part_bytes(tiles, n_kv_heads, split_for(tiles, n_kv_heads, max_len).splits);
 }
 
 extern "C" int dip_kv4_decode_attention(const uint16_t* q, const int8_t* k_cache,
@@ -412,11 +422,12 @@ extern "C" int dip_kv4_decode_attention(const uint16_t* q, const int8_t* k_cache
   Kv4AttnArgs a{q, reinterpret_cast<const uint32_t*>(k_cache),
                 reinterpret_cast<const uint32_t*>(v_cache), kv_scales, pos,
                 static_cast<float*>(workspace), out, 0, 1, (int)n_kv_heads, (int)group,
-                (int)max_len, splits_for(tiles, n_kv_heads, max_len), scale};
-  const size_t need = part_bytes(tiles, n_kv_heads, a.splits);
+                (int)max_len, 0, scale};
+  const Split sp = split_for(tiles, n_kv_heads, max_len);
+  const size_t need = part_bytes(tiles, n_kv_heads, sp.splits);
   if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return DIP_ERR_ALIGN;
-  return launch_attn(a, tiles, (hipStream_t)stream);
+  return launch_attn(a, tiles, sp, (hipStream_t)stream);
 }
 
 extern "C" size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_t start,
@@ -426,7 +437,7 @@ extern "C" size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_
       tokens <= 0 || start < 0)
     return 0;
   const int64_t tiles = col_tiles(tokens, n_heads / n_kv_heads);
-  return part_bytes(tiles, n_kv_heads, splits_for(tiles, n_kv_heads, start + tokens));
+  return part_bytes(tiles, n_kv_heads, split_for(tiles, n_kv_heads, start + tokens).splits);
 }
 
 extern "C" int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache,
@@ -444,9 +455,10 @@ extern "C" int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache
   Kv4AttnArgs a{q, reinterpret_cast<const uint32_t*>(k_cache),
                 reinterpret_cast<const uint32_t*>(v_cache), kv_scales, nullptr,
                 static_cast<float*>(workspace), out, start, (int)tokens, (int)n_kv_heads,
-                (int)group, (int)max_len, splits_for(tiles, n_kv_heads, start + tokens), scale};
-  const size_t need = part_bytes(tiles, n_kv_heads, a.splits);
+                (int)group, (int)max_len, 0, scale};
+  const Split sp = split_for(tiles, n_kv_heads, start + tokens);
+  const size_t need = part_bytes(tiles, n_kv_heads, sp.splits);
   if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return DIP_ERR_ALIGN;
-  return launch_attn(a, tiles, (hipStream_t)stream);
+  return launch_attn(a, tiles, sp, (hipStream_t)stream);
 }
