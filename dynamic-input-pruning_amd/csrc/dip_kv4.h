@@ -70,35 +70,34 @@ DIP_DEV int kv4_nibble(uint32_t w, int shift) {
   return (int)kv4_rotl(w, (28 - shift) & 31) >> 28;
 }
 
-// Max over aligned groups of 16 lanes of whole numbers.
-DIP_DEV uint32_t group_umax16(uint32_t v) {
+// Max over aligned groups of W lanes (4 or 16) of whole numbers.
+template <int W>
+DIP_DEV uint32_t group_umax(uint32_t v) {
+  static_assert(W == 4 || W == 16, "W");
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true));
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true));
+  if (W == 4) return v;
   v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xF, 0xF, true));
   return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xF, 0xF, true));
 }
 
-// A pair of bf16 values per lane, 16 lanes to a group: the group's scale (bf16
-// bits) and the pair's numbers as nibbles.
-struct Kv4Pair {
-  uint32_t scale, q0, q1;
-};
+// The larger magnitude of a bf16 pair, as the fp32 bits that order like it.
+DIP_DEV uint32_t kv4_abs_max(uint32_t pair) {
+  return max((pair << 16) & 0x7FFFFFFFu, pair & 0x7FFF0000u);
+}
 
-DIP_DEV Kv4Pair kv4_quantize(uint32_t pair) {
-  const float x0 = bf16_to_f32(pair & 0xFFFFu), x1 = __uint_as_float(pair & 0xFFFF0000u);
-  const uint32_t a =
-      group_umax16(max((pair << 16) & 0x7FFFFFFFu, pair & 0x7FFF0000u));  // |x| orders as its bits
-  uint32_t sb = __float_as_uint(__uint_as_float(a) / 7.0f) & 0xFFF80000u;
-  if (sb < 0x0D800000u) sb = 0u;         // below 2^-100
-  if (a >= 0x7F800000u) sb = 0x7FC00000u;  // an infinity or a NaN in the group
-  const float s = __uint_as_float(sb);
-  Kv4Pair r;
-  r.scale = sb >> 16;
-  const bool some = s > 0.f;
-  const float q0 = some ? rintf(x0 / s) : 0.f, q1 = some ? rintf(x1 / s) : 0.f;
-  r.q0 = (uint32_t)(int)fminf(fmaxf(q0, -7.f), 7.f) & 15u;
-  r.q1 = (uint32_t)(int)fminf(fmaxf(q1, -7.f), 7.f) & 15u;
-  return r;
+// A group's scale, as fp32 bits (the low 16 are 0), from its largest magnitude.
+DIP_DEV uint32_t kv4_scale_bits(uint32_t a) {
+  const uint32_t s = __float_as_uint(__uint_as_float(a) / 7.0f) & 0xFFF80000u;
+  if (a >= 0x7F800000u) return 0x7FC00000u;  // an infinity or a NaN in the group
+  return s < 0x0D800000u ? 0u : s;           // below 2^-100
+}
+
+// x's number in a group of that scale, as a nibble.
+DIP_DEV uint32_t kv4_number(float x, uint32_t scale_bits) {
+  const float s = __uint_as_float(scale_bits);
+  const float q = s > 0.f ? rintf(x / s) : 0.f;
+  return (uint32_t)(int)fminf(fmaxf(q, -7.f), 7.f) & 15u;
 }
 
 }  // namespace dip

@@ -9,11 +9,28 @@ namespace {
 
 constexpr int kWriteWaves = 4;  // waves of a workgroup, each with a task of its own
 
-// A sum over the wave in 64 bits.
-DIP_DEV double wave_sum64(double v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-  return v;
+// A sum over 16 lanes in 64 bits.
+template <int CTRL>
+DIP_DEV double dpp_mov64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+  const uint32_t hi =
+      (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+DIP_DEV double sum16_64(double v) {
+  v += dpp_mov64<0xB1>(v);   // the lanes of group_sum<16>
+  v += dpp_mov64<0x4E>(v);
+  v += dpp_mov64<0x141>(v);
+  return v + dpp_mov64<0x140>(v);
+}
+
+// 1 / sqrt(x) in 64 bits, x > 0 and normal: two Newton steps on the hardware's
+// estimate (2^-26 or better).
+DIP_DEV double rsqrt64(double x) {
+  double r = __builtin_amdgcn_rsq(x);
+  r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
+  return fma(r * 0.5, fma(-x * r, r, 1.0), r);
 }
 
 struct Kv4WriteArgs {
@@ -31,19 +48,27 @@ struct Kv4WriteArgs {
   uint16_t* sc;
   int64_t start;
   int tokens, nh, nkv, max_len, vblocks;
+  int k_vec;  // not kNorm: every head of k starts at a multiple of 16 bytes
   float eps;
 };
 
 // One wave per task: first the values, a task per (block of 32 rows, lane
 // quarter, kv head), which is the 8 rows that share words, so no two waves write
-// one word; then the q and k heads, a task per (token, head).  Lane l holds
-// dimensions 2 l and 2 l + 1 and a scale group is 16 lanes.  Words whose rows
-// lie partly outside the written ones keep those rows' nibbles.
+// one word; then the q and k heads, a task per four heads of a token.  Words whose
+// rows lie partly outside the written ones keep those rows' nibbles.
 //
-// The norm's mean and root are taken in 64 bits: a key next to a border
-// between two of the cache's numbers falls to the same side whatever the order
-// of the sum, so a cache row is a function of its token alone.  The other
-// roundings are those of qk_rope_cache_kernel (dip_decode.hip).
+// A values' task: lane l holds dimensions 2 l and 2 l + 1 of each row, a scale
+// group is 16 lanes.  A heads' task: 16 lanes per head, lane i the dimensions
+// 8 i .. 8 i + 7 (one 16-byte load), which are one word of a key; a scale group is
+// four lanes, and rotate_half's partner dimension is in lane i ^ 8.  (A wave per
+// head, two dimensions per lane and the sum by lane shuffles: 4099 tokens of
+// 64 / 8 heads 133 us.)
+//
+// The norm's mean and root are taken in 64 bits, and x * r is the 64-bit
+// product's fp32 rounding (r in two parts): a key next to a border between two of
+// the cache's numbers falls to the same side whatever the order of the sum, so a
+// cache row is a function of its token alone.  The other roundings are those of
+// qk_rope_cache_kernel (dip_decode.hip).
 template <bool kNorm>
 __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArgs a) {
   const int l = threadIdx.x & 63;
@@ -70,13 +95,15 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
     for (int j = 0; j < 8; ++j) {
       if (!in[j]) continue;
       const int64_t row = block * kKvBlock + 16 * (j >> 2) + 4 * c + (j & 3);
-      const Kv4Pair p = kv4_quantize(pair[j]);
-      word[0] |= kv4_rotl(p.q0, kv4_shift(j));
-      word[1] |= kv4_rotl(p.q1, kv4_shift(j));
+      const float x0 = bf16_to_f32(pair[j] & 0xFFFFu);
+      const float x1 = __uint_as_float(pair[j] & 0xFFFF0000u);
+      const uint32_t sb = kv4_scale_bits(group_umax<16>(kv4_abs_max(pair[j])));
+      word[0] |= kv4_rotl(kv4_number(x0, sb), kv4_shift(j));
+      word[1] |= kv4_rotl(kv4_number(x1, sb), kv4_shift(j));
       mask |= kv4_rotl(15u, kv4_shift(j));
       if ((l & 15) == 0)
         a.sc[((size_t)head * a.max_len + row) * kKvScaleVals + kKvGroups + (l >> 4)] =
-            (uint16_t)p.scale;
+            (uint16_t)(sb >> 16);
     }
     if (mask == 0u) return;
     uint32_t* blk = a.vc + ((size_t)head * (a.max_len / kKvBlock) + block) * kKvBlockWords;
@@ -87,53 +114,78 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
     }
     return;
   }
-  const int heads = kNorm ? a.nh + a.nkv : a.nkv;
-  const int64_t t = (task - vtasks) / heads;
-  const int head = (int)((task - vtasks) % heads);
+  const int heads = kNorm ? a.nh + a.nkv : a.nkv, quads = (heads + 3) / 4;
+  const int64_t t = (task - vtasks) / quads;
+  const int head = (int)((task - vtasks) % quads) * 4 + (l >> 4), i = l & 15;
   if (t >= a.tokens) return;
+  const bool on = head < heads;
   const int64_t row = ok ? first + t : 0;
-  uint32_t pair =
-      *reinterpret_cast<const uint32_t*>(a.k + t * a.k_tok + (int64_t)head * a.k_head + 2 * l);
+  uint32_t x[4] = {0u, 0u, 0u, 0u};
+  if (on) {
+    const uint16_t* p = a.k + t * a.k_tok + (int64_t)head * a.k_head + 8 * i;
+    if (kNorm || a.k_vec) {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = reinterpret_cast<const uint32_t*>(p)[e];
+    }
+  }
   const bool is_q = kNorm && head < a.nh;
   if (kNorm) {
-    const uint32_t wp = reinterpret_cast<const uint32_t*>(is_q ? a.q_w : a.k_w)[l];
-    const double x0 = bf16_to_f32(pair & 0xFFFFu), x1 = bf16_to_f32(pair >> 16);
-    const double ss = wave_sum64(x0 * x0 + x1 * x1);
-    const double r = 1.0 / sqrt(ss * (1.0 / kKvHeadDim) + (double)a.eps);
-    const uint32_t y0 = f32_to_bf16(bf16_to_f32(wp & 0xFFFFu) *
-                                    bf16_to_f32(f32_to_bf16((float)(x0 * r))));
-    const uint32_t y1 =
-        f32_to_bf16(bf16_to_f32(wp >> 16) * bf16_to_f32(f32_to_bf16((float)(x1 * r))));
-    // rotate_half: dims [0, 64) take -y[d + 64], dims [64, 128) take y[d - 64]
-    float r0 = bf16_to_f32(__shfl_xor(y0, 32, 64)), r1 = bf16_to_f32(__shfl_xor(y1, 32, 64));
-    if (l < 32) {
-      r0 = -r0;
-      r1 = -r1;
+    const uint4 wv = reinterpret_cast<const uint4*>(is_q ? a.q_w : a.k_w)[i];
+    const uint4 cv = reinterpret_cast<const uint4*>(a.cos_t)[row * 16 + i];
+    const uint4 sv = reinterpret_cast<const uint4*>(a.sin_t)[row * 16 + i];
+    const uint32_t w[4] = {wv.x, wv.y, wv.z, wv.w}, cs[4] = {cv.x, cv.y, cv.z, cv.w};
+    const uint32_t sn[4] = {sv.x, sv.y, sv.z, sv.w};
+    auto lo = [](uint32_t v) { return __uint_as_float(v << 16); };
+    auto hi = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };
+    auto pack = [](float u, float v) { return f32x2_to_bf16x2_nan(u, v); };
+    double ss = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const double u = lo(x[e]), v = hi(x[e]);
+      ss = fma(u, u, ss);
+      ss = fma(v, v, ss);
     }
-    const uint32_t cs = reinterpret_cast<const uint32_t*>(a.cos_t)[row * 64 + l];
-    const uint32_t sn = reinterpret_cast<const uint32_t*>(a.sin_t)[row * 64 + l];
-    auto rounded = [](float v) { return bf16_to_f32(f32_to_bf16(v)); };
-    pair = f32_to_bf16(rounded(bf16_to_f32(y0) * bf16_to_f32(cs & 0xFFFFu)) +
-                       rounded(r0 * bf16_to_f32(sn & 0xFFFFu))) |
-           (f32_to_bf16(rounded(bf16_to_f32(y1) * bf16_to_f32(cs >> 16)) +
-                        rounded(r1 * bf16_to_f32(sn >> 16)))
-            << 16);
+    const double r = rsqrt64(fma(sum16_64(ss), 1.0 / kKvHeadDim, (double)a.eps));
+    const float r0 = (float)r, r1 = (float)(r - (double)r0);
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t n = pack(fmaf(lo(x[e]), r0, lo(x[e]) * r1), fmaf(hi(x[e]), r0, hi(x[e]) * r1));
+      y[e] = pack(lo(w[e]) * lo(n), hi(w[e]) * hi(n));
+    }
+    // rotate_half: dims [0, 64) take -y[d + 64], dims [64, 128) take y[d - 64]
+    const uint32_t flip = i < 8 ? 0x80008000u : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t h = (uint32_t)__builtin_amdgcn_mov_dpp((int)y[e], 0x128, 0xF, 0xF, true);
+      const uint32_t s = sn[e] ^ flip;
+      const uint32_t u = pack(lo(y[e]) * lo(cs[e]), hi(y[e]) * hi(cs[e]));
+      const uint32_t v = pack(lo(h) * lo(s), hi(h) * hi(s));
+      x[e] = pack(lo(u) + lo(v), hi(u) + hi(v));
+    }
     if (is_q) {
-      reinterpret_cast<uint32_t*>(a.q_out)[(t * a.nh + head) * 64 + l] = pair;
+      reinterpret_cast<uint4*>(a.q_out)[(t * a.nh + head) * 16 + i] =
+          make_uint4(x[0], x[1], x[2], x[3]);
       return;
     }
   }
-  if (!ok) return;
+  if (!ok || !on) return;
   const int kvh = kNorm ? head - a.nh : head;
-  const Kv4Pair p = kv4_quantize(pair);
-  // dimensions 8 (l / 4) .. + 7 are four lanes' pairs
-  uint32_t w = kv4_rotl(p.q0 | (p.q1 << 16), kv4_shift(2 * (l & 3)));
-  w |= (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0xB1, 0xF, 0xF, true);
-  w |= (uint32_t)__builtin_amdgcn_mov_dpp((int)w, 0x4E, 0xF, 0xF, true);
+  uint32_t m = 0u, word = 0u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m = max(m, kv4_abs_max(x[e]));
+  const uint32_t sb = kv4_scale_bits(group_umax<4>(m));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    word |= kv4_rotl(kv4_number(__uint_as_float(x[e] << 16), sb), kv4_shift(2 * e));
+    word |= kv4_rotl(kv4_number(__uint_as_float(x[e] & 0xFFFF0000u), sb), kv4_shift(2 * e + 1));
+  }
   const size_t at = (size_t)kvh * a.max_len + row;
-  if ((l & 3) == 0)
-    a.kc[at * (kKvKeyBytes / 4) + 4 * ((l >> 2) & 3) + (l >> 4)] = w;
-  if ((l & 15) == 0) a.sc[at * kKvScaleVals + (l >> 4)] = (uint16_t)p.scale;
+  a.kc[at * (kKvKeyBytes / 4) + 4 * (i & 3) + (i >> 2)] = word;
+  if ((i & 3) == 0) a.sc[at * kKvScaleVals + (i >> 2)] = (uint16_t)(sb >> 16);
 }
 
 // Rows start .. start + rows - 1 as bf16 [rows, nkv, 128]: a wave per (block,
@@ -184,7 +236,7 @@ int launch_write(Kv4WriteArgs a, hipStream_t stream) {
   // a token at a position on the device is in one block, whichever it is
   a.vblocks = a.pos ? 1 : (int)touched(a.start, a.tokens);
   const int64_t tasks = (int64_t)a.vblocks * 4 * a.nkv +
-                        (int64_t)a.tokens * (kNorm ? a.nh + a.nkv : a.nkv);
+                        (int64_t)a.tokens * (((kNorm ? a.nh + a.nkv : a.nkv) + 3) / 4);
   const int64_t grid = (tasks + kWriteWaves - 1) / kWriteWaves;
   if (grid > INT32_MAX) return DIP_ERR_SHAPE;
   hipLaunchKernelGGL((kv4_write_kernel<kNorm>), dim3((unsigned)grid), dim3(64 * kWriteWaves), 0,
@@ -260,6 +312,7 @@ extern "C" int dip_kv4_write(const uint16_t* k, const uint16_t* v, int64_t k_tok
   a.k_head = k_head_stride;
   a.v_tok = v_tok_stride;
   a.v_head = v_head_stride;
+  a.k_vec = aligned16(k) && (k_tok_stride | k_head_stride) % 8 == 0;
   a.start = start;
   a.kc = reinterpret_cast<uint32_t*>(k_cache);
   a.vc = reinterpret_cast<uint32_t*>(v_cache);
