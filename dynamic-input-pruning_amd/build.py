@@ -42,7 +42,8 @@ COMMON = [
 # Flags of one source: its MFMA sums stay in the registers that the other
 # instructions use (by default they move through the accumulator half of the
 # register file, 130 of a cache block's 630 instructions).
-EXTRA = {"dip_kv4_attn": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+_VGPR_SUMS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+EXTRA = {"dip_kv4_attn": _VGPR_SUMS, "dip_kv4_prompt": _VGPR_SUMS}
 
 
 def _run(cmd):

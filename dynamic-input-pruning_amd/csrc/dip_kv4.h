@@ -100,4 +100,33 @@ DIP_DEV uint32_t kv4_number(float x, uint32_t scale_bits) {
   return (uint32_t)(int)fminf(fmaxf(q, -7.f), 7.f) & 15u;
 }
 
+// The attention kernels' arguments (dip_kv4_attn.hip, dip_kv4_prompt.hip).
+struct Kv4AttnArgs {
+  const uint16_t* q;  // [tokens, nkv * group, 128]
+  const uint32_t* kc;
+  const uint32_t* vc;
+  const uint16_t* sc;
+  const int64_t* pos;  // the first token's position, or null: `start`
+  float* part;         // [tiles, nkv, splits, columns of a tile, kKvPart]
+  uint16_t* out;       // [tokens, nkv * group, 128]
+  int64_t start;
+  int tokens, nkv, group, max_len, splits;
+  float scale;
+};
+
+constexpr int kKvPart = 2 + kKvHeadDim;  // max, sum, value sum of one column
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// 2^x; results below the normal range are 0.
+DIP_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Cache rows that the token at position pos attends: 0 .. pos.
+DIP_DEV int rows_at(int64_t pos, int max_len) {
+  return pos < 0 ? 0 : (pos < (int64_t)max_len ? (int)pos + 1 : max_len);
+}
+
+// A prompt's attention over the cache expanded to bf16 (dip_kv4_prompt.hip).
+size_t prompt_tiles_workspace(int64_t tokens, int64_t start, int64_t nkv, int64_t group);
+int launch_prompt_tiles(Kv4AttnArgs a, void* workspace, hipStream_t stream);
+
 }  // namespace dip

@@ -9,27 +9,8 @@ namespace dip {
 namespace {
 
 constexpr int kCols = 16;                  // (token, query head) pairs of a tile: MFMA columns
-constexpr int kPart = 2 + kKvHeadDim;      // max, sum, value sum of one column
+constexpr int kPart = kKvPart;
 constexpr int kMaxSplits = 256;
-constexpr float kLog2e = 1.44269504088896340736f;
-
-// Cache rows that the token at position pos attends: 0 .. pos.
-DIP_DEV int rows_at(int64_t pos, int max_len) {
-  return pos < 0 ? 0 : (pos < (int64_t)max_len ? (int)pos + 1 : max_len);
-}
-
-struct Kv4AttnArgs {
-  const uint16_t* q;  // [tokens, nkv * group, 128]
-  const uint32_t* kc;
-  const uint32_t* vc;
-  const uint16_t* sc;
-  const int64_t* pos;  // the first token's position, or null: `start`
-  float* part;         // [tiles, nkv, splits, kCols, kPart]
-  uint16_t* out;       // [tokens, nkv * group, 128]
-  int64_t start;
-  int tokens, nkv, group, max_len, splits;
-  float scale;
-};
 
 // The tile's last token's rows, and the blocks of 32 rows that a wave of `waves`
 // takes of them.
@@ -42,8 +23,6 @@ DIP_DEV int blocks_per_wave(int rows, int waves) {
   return max(1, (blocks + waves - 1) / waves);
 }
 
-// 2^x; results below the normal range are 0.
-DIP_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 DIP_DEV float scale_lo(uint32_t w) { return __uint_as_float(w << 16); }
 DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
@@ -351,6 +330,7 @@ struct Split {
 // itself; longer caches are spread over enough workgroups to fill the chip about
 // twice over, a block of rows per wave at least, and added up in a second launch.
 constexpr int64_t kShort = 1024;
+constexpr int64_t kManyColumns = 64;
 
 inline Split split_for(int64_t tiles, int64_t nkv, int64_t max_rows) {
   if (max_rows <= kShort) return {8, 1};
@@ -430,13 +410,21 @@ extern "C" int dip_kv4_decode_attention(const uint16_t* q, const int8_t* k_cache
   return launch_attn(a, tiles, sp, (hipStream_t)stream);
 }
 
+namespace {
+// Prompts of many columns go over the cache expanded to bf16, in tiles of 128
+// columns; few are served by the token's kernel, 16 columns to a tile.
+inline bool by_tiles(int64_t tokens, int64_t group) { return tokens * group > kManyColumns; }
+}  // namespace
+
 extern "C" size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_t start,
                                                           int64_t n_heads, int64_t n_kv_heads,
                                                           int64_t head_dim) {
   if (head_dim != kKvHeadDim || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
-      tokens <= 0 || start < 0)
+      tokens <= 0 || start < 0 || start > (1 << 30) || tokens > (1 << 30))
     return 0;
-  const int64_t tiles = col_tiles(tokens, n_heads / n_kv_heads);
+  const int64_t group = n_heads / n_kv_heads;
+  if (by_tiles(tokens, group)) return prompt_tiles_workspace(tokens, start, n_kv_heads, group);
+  const int64_t tiles = col_tiles(tokens, group);
   return part_bytes(tiles, n_kv_heads, split_for(tiles, n_kv_heads, start + tokens).splits);
 }
 
@@ -456,9 +444,10 @@ extern "C" int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache
                 reinterpret_cast<const uint32_t*>(v_cache), kv_scales, nullptr,
                 static_cast<float*>(workspace), out, start, (int)tokens, (int)n_kv_heads,
                 (int)group, (int)max_len, 0, scale};
-  const Split sp = split_for(tiles, n_kv_heads, start + tokens);
-  const size_t need = part_bytes(tiles, n_kv_heads, sp.splits);
+  const size_t need =
+      dip_kv4_prompt_attention_workspace_size(tokens, start, n_heads, n_kv_heads, head_dim);
   if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return DIP_ERR_ALIGN;
-  return launch_attn(a, tiles, sp, (hipStream_t)stream);
+  if (by_tiles(tokens, group)) return launch_prompt_tiles(a, workspace, (hipStream_t)stream);
+  return launch_attn(a, tiles, split_for(tiles, n_kv_heads, start + tokens), (hipStream_t)stream);
 }
