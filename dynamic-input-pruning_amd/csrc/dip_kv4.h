@@ -127,6 +127,7 @@ DIP_DEV int rows_at(int64_t pos, int max_len) {
 
 // A prompt's attention over the cache expanded to bf16 (dip_kv4_prompt.hip).
 size_t prompt_tiles_workspace(int64_t tokens, int64_t start, int64_t nkv, int64_t group);
+int64_t prompt_tiles_us100(int64_t tokens, int64_t start, int64_t nkv, int64_t group);
 int launch_prompt_tiles(Kv4AttnArgs a, void* workspace, hipStream_t stream);
 
 }  // namespace dip

@@ -321,22 +321,31 @@ __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4A
   }
 }
 
-// How many waves a workgroup has and how many workgroups share a tile's rows.
-struct Split {
-  int waves, splits;
+// How a launch cuts its tiles' rows.  Alone, a workgroup of 8 waves takes a tile's
+// and writes the result itself; otherwise twice `pairs` workgroups of 4 waves (two
+// to a CU) do, whose sums a second launch adds up.  `us` is about what it takes,
+// from measured times: 3 us, 5 us and 1.35 us per block of a wave for each round of
+// the workgroups, 6.5 us for the second launch (64 columns of 8 kv heads over 20000
+// rows: 26 us, by this 28; 512 columns over 8000 rows: 51, 51; 1024 over 1000: 26,
+// 26; 8 over 1000 in one launch 11, in two 13).  (Split tiles with 8 waves: 20011 rows of 64 / 8 heads 15.2 us for 11.6.)
+struct Cut {
+  int pairs;
+  int64_t us100;
+  int waves() const { return pairs == 1 ? 8 : 4; }
+  int splits() const { return pairs == 1 ? 1 : 2 * pairs; }
 };
 
-// Up to kShort rows one workgroup of 8 waves takes a tile's and writes the result
-// itself; longer caches are spread over enough workgroups to fill the chip about
-// twice over, a block of rows per wave at least, and added up in a second launch.
-constexpr int64_t kShort = 1024;
-constexpr int64_t kManyColumns = 64;
-
-inline Split split_for(int64_t tiles, int64_t nkv, int64_t max_rows) {
-  if (max_rows <= kShort) return {8, 1};
-  const int64_t want = (2 * device_cus() + tiles * nkv - 1) / (tiles * nkv);
-  const int64_t most = (max_rows + kKvBlock * 4 - 1) / (kKvBlock * 4);
-  return {4, (int)max((int64_t)1, min(min(want, most), (int64_t)kMaxSplits))};
+inline Cut cut_for(int64_t tiles, int64_t nkv, int64_t max_rows) {
+  const int64_t blocks = (max_rows + kKvBlock - 1) / kKvBlock, cus = device_cus();
+  const int64_t most = min((blocks + 7) / 8, (int64_t)kMaxSplits / 2);
+  Cut best{1, INT64_MAX};
+  for (int64_t s = 1; s <= most; s = s < 8 ? s + 1 : s + s / 8) {
+    const int64_t rounds = (tiles * nkv * s + cus - 1) / cus;
+    const int64_t per = (blocks + 8 * s - 1) / (8 * s);
+    const int64_t us = 300 + rounds * (500 + 135 * per) + (s > 1 ? 650 : 0);
+    if (us < best.us100) best = Cut{(int)s, us};
+  }
+  return best;
 }
 
 inline int64_t col_tiles(int64_t tokens, int64_t group) {
@@ -360,17 +369,17 @@ int check_attn(const void* q, const void* kc, const void* vc, const void* sc, co
   return DIP_OK;
 }
 
-int launch_attn(Kv4AttnArgs a, int64_t tiles, Split sp, hipStream_t stream) {
-  a.splits = sp.splits;
+int launch_attn(Kv4AttnArgs a, int64_t tiles, Cut cut, hipStream_t stream) {
+  a.splits = cut.splits();
   const int64_t grid = tiles * a.nkv * a.splits;
   if (grid > INT32_MAX || (int64_t)a.tokens * a.group * a.nkv > INT32_MAX) return DIP_ERR_SHAPE;
-  if (sp.waves == 8)
+  if (cut.waves() == 8)
     hipLaunchKernelGGL((kv4_attn_kernel<8>), dim3((unsigned)grid), dim3(512), 0, stream, a);
   else
     hipLaunchKernelGGL((kv4_attn_kernel<4>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (a.splits > 1)
     hipLaunchKernelGGL(kv4_combine_kernel, dim3((unsigned)(a.tokens * a.group * a.nkv)),
-                       dim3(kCombine * kKvHeadDim), 0, stream, a, sp.waves);
+                       dim3(kCombine * kKvHeadDim), 0, stream, a, cut.waves());
   return hip_status(hipGetLastError());
 }
 
@@ -385,7 +394,7 @@ extern "C" size_t dip_kv4_decode_attention_workspace_size(int64_t n_heads, int64
       max_len <= 0)
     return 0;
   const int64_t tiles = col_tiles(1, n_heads / n_kv_heads);
-  return part_bytes(tiles, n_kv_heads, split_for(tiles, n_kv_heads, max_len).splits);
+  return part_bytes(tiles, n_kv_heads, cut_for(tiles, n_kv_heads, max_len).splits());
 }
 
 extern "C" int dip_kv4_decode_attention(const uint16_t* q, const int8_t* k_cache,
@@ -403,17 +412,22 @@ extern "C" int dip_kv4_decode_attention(const uint16_t* q, const int8_t* k_cache
                 reinterpret_cast<const uint32_t*>(v_cache), kv_scales, pos,
                 static_cast<float*>(workspace), out, 0, 1, (int)n_kv_heads, (int)group,
                 (int)max_len, 0, scale};
-  const Split sp = split_for(tiles, n_kv_heads, max_len);
-  const size_t need = part_bytes(tiles, n_kv_heads, sp.splits);
+  const Cut cut = cut_for(tiles, n_kv_heads, max_len);
+  const size_t need = part_bytes(tiles, n_kv_heads, cut.splits());
   if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return DIP_ERR_ALIGN;
-  return launch_attn(a, tiles, sp, (hipStream_t)stream);
+  return launch_attn(a, tiles, cut, (hipStream_t)stream);
 }
 
 namespace {
-// Prompts of many columns go over the cache expanded to bf16, in tiles of 128
-// columns; few are served by the token's kernel, 16 columns to a tile.
-inline bool by_tiles(int64_t tokens, int64_t group) { return tokens * group > kManyColumns; }
+// Whether a prompt goes over the cache expanded to bf16, in tiles of 128 columns,
+// or through the token's kernel, 16 columns to a tile: the one that takes less by
+// the two estimates (8 kv heads: from 2000 columns on over 300 rows, 800 over 3000,
+// 200 over 20000).
+inline bool by_tiles(int64_t tokens, int64_t start, int64_t nkv, int64_t group) {
+  return prompt_tiles_us100(tokens, start, nkv, group) <
+         cut_for(col_tiles(tokens, group), nkv, start + tokens).us100;
+}
 }  // namespace
 
 extern "C" size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_t start,
@@ -423,9 +437,10 @@ extern "C" size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_
       tokens <= 0 || start < 0 || start > (1 << 30) || tokens > (1 << 30))
     return 0;
   const int64_t group = n_heads / n_kv_heads;
-  if (by_tiles(tokens, group)) return prompt_tiles_workspace(tokens, start, n_kv_heads, group);
+  if (by_tiles(tokens, start, n_kv_heads, group))
+    return prompt_tiles_workspace(tokens, start, n_kv_heads, group);
   const int64_t tiles = col_tiles(tokens, group);
-  return part_bytes(tiles, n_kv_heads, split_for(tiles, n_kv_heads, start + tokens).splits);
+  return part_bytes(tiles, n_kv_heads, cut_for(tiles, n_kv_heads, start + tokens).splits());
 }
 
 extern "C" int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache,
@@ -448,6 +463,7 @@ extern "C" int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache
       dip_kv4_prompt_attention_workspace_size(tokens, start, n_heads, n_kv_heads, head_dim);
   if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return DIP_ERR_ALIGN;
-  if (by_tiles(tokens, group)) return launch_prompt_tiles(a, workspace, (hipStream_t)stream);
-  return launch_attn(a, tiles, split_for(tiles, n_kv_heads, start + tokens), (hipStream_t)stream);
+  if (by_tiles(tokens, start, n_kv_heads, group))
+    return launch_prompt_tiles(a, workspace, (hipStream_t)stream);
+  return launch_attn(a, tiles, cut_for(tiles, n_kv_heads, start + tokens), (hipStream_t)stream);
 }
