@@ -11,24 +11,23 @@
 // (logit, index), so ties are cut by index and the row is never sorted.
 //
 // A weight is a whole number, w * 2^shift rounded (shift such that a row's sum
-// stays below 2^63; w in 64 bits): sums are exact, in any order and by any
-// atomics, so the token does not depend on how a row is split.  In 32 bits a sum
+// stays below 2^63, 51 at most; w in 64 bits): sums are exact, in any order and by
+// any atomics, so the token does not depend on how a row is split.  In 32 bits a sum
 // over 150000 tokens is off by more than an unlikely token's weight.  Weights
 // below 2^-shift / 2 (2^-45 at 150000 tokens) are 0 and never drawn.
 //
 // Each row is cut into slices, one workgroup each, in up to four launches:
 //   max     the largest logit of each slice (with its index), and the smallest;
-//   hist    tokens and their weights counted in kBins bins of even width in the
-//           logit, per slice in LDS, then added to the row's;
-//   gather  from the histogram every slice finds the bins that can hold a border;
-//           it adds up the weights of the bins before them and lists the tokens in
-//           them;
-//   draw    one workgroup per row sorts the list (a few to a few hundred tokens),
+//   hist    the weights of the tokens, and their number, added up in kBins bins of
+//           even width in the logit: in LDS, kept per slice, and added to the row's;
+//   gather  from the row's histogram every slice finds the bins that can hold a
+//           border; it adds up its own bins before them and lists its tokens in them;
+//   draw    one workgroup per row orders the list (a few to a few hundred tokens),
 //           finds the border, the slice that the draw falls in, and the token in
 //           it.  Rows whose list overflows (thousands of equal logits) are
 //           searched by the bits of the logit instead.
-// Without top-k and top-p there is no histogram, greedy draws need the first
-// launch and a choice among its results.
+// Without top-k and top-p there is no histogram; greedy draws need the first launch
+// and a choice among its results.
 #include "dip_common.h"
 #include "dip_internal.h"
 
@@ -37,10 +36,10 @@
 namespace dip {
 namespace {
 
-constexpr int kThreads = 1024;      // draw
-constexpr int kSliceThreads = 256;  // the other launches
+constexpr int kThreads = 256;
 constexpr int kBins = 1024;
 constexpr int kListMax = 4096;
+constexpr int kRankMax = 512;  // longer lists are sorted, not ranked by comparing all pairs
 constexpr int kMaxSlices = 256;
 constexpr int kRadixBins = 256;
 constexpr uint32_t kKeyMinusInf = 0x007FFFFFu;  // order_key of -inf, and of NaN
@@ -63,17 +62,27 @@ DIP_DEV float load_logit(const void* row, int64_t i) {
   return bf16_to_f32(static_cast<const uint16_t*>(row)[i]);
 }
 
-// A row's workspace.
-struct RowState {
-  uint64_t best[kMaxSlices];         // per slice: order_key << 32 | ~index of its largest
-  uint32_t least[kMaxSlices];        // smallest order_key above -inf
-  unsigned long long sure[kMaxSlices];  // weights before the bins of the list
-  unsigned long long hw[kBins];      // histogram: weights, tokens
-  uint32_t hn[kBins];
-  uint32_t listed;
-  uint32_t pad;
-  uint64_t list[kListMax];           // order_key << 32 | ~index
+// Where the histogram says that the borders lie, and the row's ends.
+struct Plan {
+  uint32_t top, least;        // order_keys of the largest logit and the smallest above -inf
+  int lo, hi;                 // the bins to list; lo = kBins: none
+  int by_k, ranked;           // top-k cuts tokens; its or top-p's border is in the list
+  uint64_t above_n, above_w;  // tokens and weights of the bins before lo
+  uint64_t total;             // weights of all bins
 };
+
+// A row's workspace, followed by the slices' histograms (kBins weights each).
+struct RowState {
+  Plan plan;
+  uint64_t best[kMaxSlices];            // per slice: order_key << 32 | ~index of its largest
+  uint32_t least[kMaxSlices];           // smallest order_key above -inf
+  unsigned long long sure[kMaxSlices];  // weights before the bins of the list
+  unsigned long long hw[kBins];         // histogram: weights, tokens
+  uint32_t hn[kBins];
+  uint32_t listed, pad[3];
+  uint64_t list[kListMax];              // order_key << 32 | ~index
+};
+static_assert(sizeof(RowState) % 16 == 0, "rows of the workspace stay aligned");
 
 struct SampleArgs {
   const void* logits;
@@ -84,24 +93,31 @@ struct SampleArgs {
   int shift;
   int slices;
   int64_t slice_vecs;  // 16-byte pieces of a row that a slice takes
-  RowState* rows;
+  char* rows;  // row_state(a, r) of each
+  int64_t row_ws;
   int64_t* token;
   float* prob;
 };
 
+DIP_DEV RowState& row_state(const SampleArgs& a, int r) {
+  return *reinterpret_cast<RowState*>(a.rows + r * a.row_ws);
+}
+DIP_DEV unsigned long long* slice_hist(const SampleArgs& a, int r, int s) {
+  return reinterpret_cast<unsigned long long*>(a.rows + r * a.row_ws + sizeof(RowState)) +
+         (size_t)s * kBins;
+}
 DIP_DEV const char* row_of(const SampleArgs& a, int r) {
   return static_cast<const char*>(a.logits) + (int64_t)r * a.row_bytes;
 }
 
-// f(index, order_key) of every token in the 16-byte pieces [v0, v1) of a row, by
-// `threads` threads.  Pieces lie where memory has them; one that reaches over an
+// f(index, order_key) of every token in the 16-byte pieces [v0, v1) of a row, by the
+// workgroup's threads.  Pieces lie where memory has them; one that reaches over an
 // end of the row is loaded token by token.
 template <int kType, typename F>
-DIP_DEV void each_token(const char* row, int64_t vocab, int64_t v0, int64_t v1, int tid,
-                        int threads, F f) {
+DIP_DEV void each_token(const char* row, int64_t vocab, int64_t v0, int64_t v1, F f) {
   constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
   const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
-  for (int64_t v = v0 + tid; v < v1; v += threads) {
+  for (int64_t v = v0 + threadIdx.x; v < v1; v += kThreads) {
     const int64_t e0 = v * kVec - off;
     if (e0 >= 0 && e0 + kVec <= vocab) {
       const uint4 w = *reinterpret_cast<const uint4*>(row + e0 * kSize);
@@ -128,33 +144,46 @@ DIP_DEV int64_t row_vecs(const char* row, int64_t vocab) {
   return ((reinterpret_cast<uintptr_t>(row) & 15) + vocab * kSize + 15) / 16;
 }
 
-// What a row's largest logit makes of the others.
+// What a row's largest logit makes of the others.  Weights are 2^-(k / 64) 2^-(f / 64)
+// with k + f = 64 (max - logit) / (temperature ln 2): a table of 64 roots and the
+// series of exp to z^5 (z < 0.011, so the rest is below 2e-15).
 struct Weigher {
   uint32_t top;
-  double most, per_log2;  // logits per factor of 2
+  double most, per_64th, least;  // 64ths of an octave per logit; min-p, scaled
   float bins_per_logit;
-  double scale, min_p;
+  const double* roots;  // 2^(shift - j / 64), in LDS
 
-  DIP_DEV Weigher(const SampleArgs& a, uint32_t top_key, uint32_t least_key) : top(top_key) {
+  // The workgroup's `lds` gets the roots; a barrier must follow before their use.
+  DIP_DEV Weigher(const SampleArgs& a, uint32_t top_key, uint32_t least_key, double* lds)
+      : top(top_key), roots(lds) {
+    if (threadIdx.x < 64) lds[threadIdx.x] = exp2(a.shift - threadIdx.x * (1.0 / 64));
     most = key_value(top);
-    per_log2 = 1.4426950408889634074 / a.temperature;
-    scale = (double)(1ull << a.shift);
-    min_p = a.min_p;
+    per_64th = 64 * 1.4426950408889634074 / a.temperature;
+    least = a.min_p * (double)(1ull << a.shift);
     // bins reach down to the smallest logit, or to the weight that counts as 0
-    const double range = min(most - (double)key_value(least_key), (a.shift + 1) / per_log2);
+    const double range = min(most - (double)key_value(least_key), 64 * (a.shift + 1) / per_64th);
     bins_per_logit = range > 0 ? (float)(kBins / range) : 0.f;
   }
-  DIP_DEV double weight(uint32_t k) const {
-    if (k == top) return 1.0;
+  // w * 2^shift
+  DIP_DEV double scaled(uint32_t k) const {
+    if (k == top) return roots[0];
     if (k <= kKeyMinusInf) return 0.0;
-    return exp2(((double)key_value(k) - most) * per_log2);
+    const double d = fmin((most - (double)key_value(k)) * per_64th, 64 * 64.0);
+    const int n = (int)d;
+    const double z = (d - n) * (-0.69314718055994530942 / 64);
+    const double p = fma(z, fma(z, fma(z, fma(z, fma(z, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0),
+                         1.0);
+    return ldexp(roots[n & 63] * p, -(n >> 6));
   }
-  DIP_DEV unsigned long long whole(double w) const { return (unsigned long long)(w * scale + 0.5); }
-  DIP_DEV unsigned long long whole_of(uint32_t k) const { return whole(weight(k)); }
+  // Rounded to a whole number: below 2^52, so the sum's low bits are it.
+  DIP_DEV static unsigned long long whole(double w) {
+    return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+  }
+  DIP_DEV unsigned long long whole_of(uint32_t k) const { return whole(scaled(k)); }
   // The weight if min-p keeps it, else 0.
   DIP_DEV unsigned long long kept_whole(uint32_t k) const {
-    const double w = weight(k);
-    return w >= min_p ? whole(w) : 0ull;
+    const double w = scaled(k);
+    return w >= least ? whole(w) : 0ull;
   }
   // Never lower for a smaller logit.
   DIP_DEV int bin(uint32_t k) const {
@@ -168,7 +197,7 @@ struct Cut {  // the last kept token of the order
   int64_t index;
 };
 
-template <int kN, typename T, typename F>
+template <typename T, typename F>
 DIP_DEV T block_reduce(T v, F f, T* lds) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v = f(v, (T)__shfl_xor(v, m, 64));
@@ -176,73 +205,82 @@ DIP_DEV T block_reduce(T v, F f, T* lds) {
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
   v = lds[0];
-  for (int i = 1; i < kN / 64; ++i) v = f(v, lds[i]);
+#pragma unroll
+  for (int i = 1; i < kThreads / 64; ++i) v = f(v, lds[i]);
   return v;
 }
 
 // The sum of the threads before this one; `total`: of all.
-template <int kN, typename T>
-DIP_DEV T block_exclusive(T v, T* lds, T& total) {
-  T run = v;
+DIP_DEV uint64_t block_exclusive(uint64_t v, uint64_t* lds, uint64_t& total) {
+  uint64_t run = v;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
-    const T o = __shfl_up(run, m, 64);
+    const uint64_t o = __shfl_up(run, m, 64);
     if ((int)(threadIdx.x & 63) >= m) run += o;
   }
   __syncthreads();
   if ((threadIdx.x & 63) == 63) lds[threadIdx.x >> 6] = run;
   __syncthreads();
-  T before = 0;
+  uint64_t before = 0;
   total = 0;
-  for (int i = 0; i < kN / 64; ++i) {
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
     if (i == (int)(threadIdx.x >> 6)) before = total;
     total += lds[i];
   }
   return before + run - v;
 }
 
-// The row's largest and smallest logits from the slices' (one workgroup-wide
-// call; every thread gets them).
-template <int kN>
+constexpr int kLdsWords = 2 * (kThreads / 64) + 4;  // of the calls above and below
+
+// The row's largest (order_key << 32 | ~index) and smallest logits, from the slices'.
 DIP_DEV void row_ends(const SampleArgs& a, const RowState& st, uint64_t* lds, uint64_t& best,
                       uint32_t& least) {
   uint64_t b = 0;
   uint32_t l = 0xFFFFFFFFu;
-  for (int s = threadIdx.x; s < a.slices; s += kN) {
+  for (int s = threadIdx.x; s < a.slices; s += kThreads) {
     b = max(b, st.best[s]);
     l = min(l, st.least[s]);
   }
-  best = block_reduce<kN>(b, [](uint64_t x, uint64_t y) { return max(x, y); }, lds);
-  least = block_reduce<kN>(l, [](uint32_t x, uint32_t y) { return min(x, y); },
-                           reinterpret_cast<uint32_t*>(lds));
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    b = max(b, (uint64_t)__shfl_xor(b, m, 64));
+    l = min(l, (uint32_t)__shfl_xor(l, m, 64));
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    lds[2 * (threadIdx.x >> 6)] = b;
+    lds[2 * (threadIdx.x >> 6) + 1] = l;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    b = max(b, lds[2 * i]);
+    l = min(l, (uint32_t)lds[2 * i + 1]);
+  }
+  best = b;
+  least = l;
 }
 
-// Where the histogram says that the border lies.
-struct Plan {
-  int lo, hi;              // the bins to list; lo = kBins: none
-  uint64_t above_n, above_w;  // tokens and weights of the bins before lo
-  uint64_t tokens, total;  // of all bins
-};
-
-// One workgroup-wide call.  lds: 4 kN / 64 + 4 words of 64 bits.
-template <int kN>
-DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& wt, uint64_t* lds) {
-  constexpr int kPer = (kBins + kN - 1) / kN;
-  uint64_t* sh = lds + 2 * (kN / 64);
+DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& wt, Plan p,
+                       uint64_t* lds) {
+  constexpr int kPer = kBins / kThreads;
+  uint64_t* sh = lds + 2 * (kThreads / 64);
   const int b0 = threadIdx.x * kPer;
   uint64_t n[kPer], w[kPer], sn = 0, sw = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    n[i] = b0 + i < kBins ? st.hn[b0 + i] : 0;
-    w[i] = b0 + i < kBins ? st.hw[b0 + i] : 0;
+    n[i] = st.hn[b0 + i];
+    w[i] = st.hw[b0 + i];
     sn += n[i];
     sw += w[i];
   }
-  Plan p;
-  const uint64_t bn = block_exclusive<kN>(sn, lds, p.tokens);
-  const uint64_t bw = block_exclusive<kN>(sw, lds, p.total);
-  // the first bin at which `test(tokens, weights up to and with it)` holds: its
-  // number, and tokens and weights before it
+  uint64_t tokens = 0;
+  const bool some_k = a.top_k > 0 && a.top_k < a.vocab;  // else nobody counted the tokens
+  const uint64_t bn = some_k ? block_exclusive(sn, lds, tokens) : 0;
+  const uint64_t bw = block_exclusive(sw, lds, p.total);
+  // the first bin at which `test(tokens, weights up to and with it)` holds, and
+  // what lies before it, in sh[0 .. 2]
   auto first = [&](auto test) {
     __syncthreads();
     if (threadIdx.x == 0) sh[0] = kBins;
@@ -250,8 +288,7 @@ DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& w
     uint64_t cn = bn, cw = bw;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const bool before = test(cn, cw);
-      if (b0 + i < kBins && !before && test(cn + n[i], cw + w[i])) {
+      if (!test(cn, cw) && test(cn + n[i], cw + w[i])) {
         sh[0] = (uint64_t)(b0 + i);
         sh[1] = cn;
         sh[2] = cw;
@@ -261,16 +298,15 @@ DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& w
     }
     __syncthreads();
   };
-  const bool by_k = a.top_k > 0 && (uint64_t)a.top_k < p.tokens;
+  p.by_k = some_k && (uint64_t)a.top_k < tokens;
   p.lo = p.hi = kBins;
   p.above_n = p.above_w = 0;
   uint64_t base = p.total;  // what top-p takes its share of, at least
-  if (by_k) {
+  if (p.by_k) {
     first([&](uint64_t cn, uint64_t) { return cn >= (uint64_t)a.top_k; });
     p.lo = p.hi = (int)sh[0];
     p.above_n = sh[1];
-    p.above_w = sh[2];
-    base = sh[2];
+    base = p.above_w = sh[2];
   }
   if (a.top_p < 1) {
     const double mass = a.top_p * (double)base;
@@ -279,114 +315,161 @@ DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& w
       p.lo = (int)sh[0];
       p.above_n = sh[1];
       p.above_w = sh[2];
+      if (!p.by_k) p.hi = p.lo;
     }
-    if (!by_k) p.hi = p.lo;
   }
-  // min-p alone cuts before the first bin to list: nothing to look for
-  if (p.lo < kBins && a.min_p > 0) {
-    const double least = wt.most + log2(a.min_p) / wt.per_log2;
-    const double bin = (wt.most - least) * wt.bins_per_logit;
-    if (p.lo > bin + 2) p.lo = p.hi = kBins;
+  p.ranked = p.lo < kBins;
+  // min-p's border: surely in the bins m .. m + 2.  If nothing is to be looked for
+  // before their end, they alone are listed; if they begin before lo, from there on.
+  if (a.min_p > 0) {
+    const double bin = -log2(a.min_p) * 64 / wt.per_64th * wt.bins_per_logit;
+    const int m = max(0, (bin < kBins ? (int)bin : kBins) - 1);
+    if (m < p.lo && m < kBins) {
+      if (m + 2 < p.lo) {
+        p.ranked = 0;
+        p.hi = m + 2;
+      }
+      p.lo = m;
+      __syncthreads();
+      if (b0 <= m && m < b0 + kPer) {
+        uint64_t cn = bn, cw = bw;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (b0 + i < m) cn += n[i], cw += w[i];
+        sh[1] = cn;
+        sh[2] = cw;
+      }
+      __syncthreads();
+      p.above_n = sh[1];
+      p.above_w = sh[2];
+    }
   }
   __syncthreads();
   return p;
 }
 
 template <int kType>
-__global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(SampleArgs a) {
-  __shared__ uint64_t lds[kSliceThreads / 64];
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
   const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
   const char* row = row_of(a, r);
-  RowState& st = a.rows[r];
+  RowState& st = row_state(a, r);
   uint64_t best = 0;
   uint32_t least = 0xFFFFFFFFu;
   each_token<kType>(row, a.vocab, s * a.slice_vecs,
-                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)), threadIdx.x,
-                    kSliceThreads, [&](int64_t i, uint32_t k) {
+                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)),
+                    [&](int64_t i, uint32_t k) {
                       best = max(best, (uint64_t)k << 32 | (uint32_t)~(uint32_t)i);
                       if (k > kKeyMinusInf) least = min(least, k);
                     });
-  best = block_reduce<kSliceThreads>(best, [](uint64_t x, uint64_t y) { return max(x, y); }, lds);
-  least = block_reduce<kSliceThreads>(least, [](uint32_t x, uint32_t y) { return min(x, y); },
-                                      reinterpret_cast<uint32_t*>(lds));
+  best = block_reduce(best, [](uint64_t x, uint64_t y) { return max(x, y); }, lds);
+  least = block_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); },
+                       reinterpret_cast<uint32_t*>(lds));
   if (threadIdx.x == 0) {
     st.best[s] = best;
     st.least[s] = least;
     if (s == 0) st.listed = 0;
   }
-  for (int b = s * kSliceThreads + threadIdx.x; b < kBins; b += a.slices * kSliceThreads) {
+  for (int b = s * kThreads + threadIdx.x; b < kBins; b += a.slices * kThreads) {
     st.hn[b] = 0;
     st.hw[b] = 0;
   }
 }
 
-template <int kType>
-__global__ __launch_bounds__(kSliceThreads) void sample_hist_kernel(SampleArgs a) {
-  __shared__ uint64_t lds[kSliceThreads / 64];
-  __shared__ uint32_t hn[kBins];
+// kCount: top-k needs the number of tokens in the bins too.
+template <int kType, bool kCount>
+__global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
+  __shared__ double roots[64];
+  __shared__ uint32_t hn[kCount ? kBins : 1];
   __shared__ unsigned long long hw[kBins];
   const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
   const char* row = row_of(a, r);
-  RowState& st = a.rows[r];
-  for (int b = threadIdx.x; b < kBins; b += kSliceThreads) hn[b] = 0, hw[b] = 0;
+  RowState& st = row_state(a, r);
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    if (kCount) hn[b] = 0;
+    hw[b] = 0;
+  }
   uint64_t best;
   uint32_t least;
-  row_ends<kSliceThreads>(a, st, lds, best, least);
+  row_ends(a, st, lds, best, least);
   const uint32_t top = (uint32_t)(best >> 32);
   if (top <= kKeyMinusInf) return;
-  const Weigher wt(a, top, least);
+  const Weigher wt(a, top, least, roots);
   __syncthreads();
   each_token<kType>(row, a.vocab, s * a.slice_vecs,
-                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)), threadIdx.x,
-                    kSliceThreads, [&](int64_t, uint32_t k) {
+                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)),
+                    [&](int64_t, uint32_t k) {
                       const unsigned long long w = wt.whole_of(k);
                       if (w == 0) return;
                       const int b = wt.bin(k);
-                      atomicAdd(&hn[b], 1u);
+                      if (kCount) atomicAdd(&hn[b], 1u);
                       atomicAdd(&hw[b], w);
                     });
   __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kSliceThreads)
-    if (hn[b]) {
-      atomicAdd(&st.hn[b], hn[b]);
-      atomicAdd(&st.hw[b], hw[b]);
-    }
+  unsigned long long* own = slice_hist(a, r, s);
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    own[b] = hw[b];
+    if (!hw[b]) continue;
+    if (kCount) atomicAdd(&st.hn[b], hn[b]);
+    atomicAdd(&st.hw[b], hw[b]);
+  }
 }
 
 // kHist: the histogram has been made.
 template <int kType, bool kHist>
-__global__ __launch_bounds__(kSliceThreads) void sample_gather_kernel(SampleArgs a) {
-  __shared__ uint64_t lds[4 * (kSliceThreads / 64) + 4];
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
+  __shared__ double roots[64];
   const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
   const char* row = row_of(a, r);
-  RowState& st = a.rows[r];
+  RowState& st = row_state(a, r);
   uint64_t best;
   uint32_t least;
-  row_ends<kSliceThreads>(a, st, lds, best, least);
+  row_ends(a, st, lds, best, least);
   const uint32_t top = (uint32_t)(best >> 32);
-  if (top <= kKeyMinusInf) return;
-  const Weigher wt(a, top, least);
-  int lo = kBins, hi = kBins;
-  if (kHist) {
-    const Plan p = make_plan<kSliceThreads>(a, st, wt, lds);
-    lo = p.lo;
-    hi = p.hi;
+  Plan p{top, least, kBins, kBins, 0, 0, 0, 0, 0};
+  if (top <= kKeyMinusInf) {
+    if (s == 0 && threadIdx.x == 0) st.plan = p;
+    return;
   }
+  const Weigher wt(a, top, least, roots);
+  __syncthreads();
+  const int64_t v0 = s * a.slice_vecs;
+  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
   uint64_t sure = 0;
-  each_token<kType>(row, a.vocab, s * a.slice_vecs,
-                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)), threadIdx.x,
-                    kSliceThreads, [&](int64_t i, uint32_t k) {
-                      if (k <= kKeyMinusInf) return;
-                      const int b = kHist ? wt.bin(k) : 0;
-                      if (b < lo) {
-                        sure += wt.kept_whole(k);
-                      } else if (b <= hi && wt.whole_of(k) > 0) {
-                        const uint32_t at = atomicAdd(&st.listed, 1u);
-                        if (at < kListMax) st.list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)i;
-                      }
-                    });
-  sure = block_reduce<kSliceThreads>(sure, [](uint64_t x, uint64_t y) { return x + y; }, lds);
-  if (threadIdx.x == 0) st.sure[s] = sure;
+  if (kHist) {
+    p = make_plan(a, st, wt, p, lds);
+    const unsigned long long* own = slice_hist(a, r, s);
+    for (int b = threadIdx.x; b < p.lo; b += kThreads) sure += own[b];
+    if (p.lo < kBins)
+      each_token<kType>(row, a.vocab, v0, v1, [&](int64_t i, uint32_t k) {
+        if (k <= kKeyMinusInf) return;
+        const int b = wt.bin(k);
+        if (b < p.lo || b > p.hi || wt.whole_of(k) == 0) return;
+        const uint32_t at = atomicAdd(&st.listed, 1u);
+        if (at < kListMax) st.list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)i;
+      });
+  } else {
+    each_token<kType>(row, a.vocab, v0, v1,
+                      [&](int64_t, uint32_t k) { sure += wt.kept_whole(k); });
+  }
+  sure = block_reduce(sure, [](uint64_t x, uint64_t y) { return x + y; }, lds);
+  if (threadIdx.x == 0) {
+    st.sure[s] = sure;
+    if (s == 0) st.plan = p;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void sample_greedy_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
+  uint64_t best;
+  uint32_t least;
+  row_ends(a, row_state(a, blockIdx.x), lds, best, least);
+  if (threadIdx.x != 0) return;
+  const bool some = (uint32_t)(best >> 32) > kKeyMinusInf;
+  a.token[blockIdx.x] = some ? (int64_t)(uint32_t)~(uint32_t)best : 0;
+  if (a.prob) a.prob[blockIdx.x] = some ? 1.f : 0.f;
 }
 
 // The border of the first `count` tokens (mass < 0), or of the fewest whose
@@ -406,7 +489,7 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
   for (int level = 24; level >= 0; level -= 8) {
     for (int b = tid; b < kRadixBins; b += kThreads) hn[b] = 0, hw[b] = 0;
     __syncthreads();
-    each_token<kType>(row, a.vocab, 0, vecs, tid, kThreads, [&](int64_t i, uint32_t k) {
+    each_token<kType>(row, a.vocab, 0, vecs, [&](int64_t i, uint32_t k) {
       if (!kept(k, i) || (level < 24 && (k >> (level + 8)) != (prefix >> (level + 8)))) return;
       const unsigned long long w = wt.whole_of(k);
       if (w == 0) return;
@@ -452,7 +535,7 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
   const int64_t lo = min(tid * per, a.vocab), end = min(lo + per, a.vocab);
   uint64_t mine = 0, all;
   for (int64_t i = lo; i < end; ++i) mine += order_key(load_logit<kType>(row, i)) == prefix;
-  const uint64_t before = block_exclusive<kThreads>(mine, lds, all);
+  const uint64_t before = block_exclusive(mine, lds, all);
   if (before < need && need <= before + mine) {
     uint64_t left = need - before;
     for (int64_t i = lo; i < end; ++i)
@@ -467,13 +550,29 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
   return c;
 }
 
-// Descending, n a power of two.
-DIP_DEV void sort_list(uint64_t* v, int n) {
-  for (int size = 2; size <= n; size *= 2)
-    for (int step = size / 2; step > 0; step /= 2) {
-      for (int t = threadIdx.x; t < n / 2; t += kThreads) {
+// v[0 .. n) in descending order (its values differ), `out` of as many words.
+DIP_DEV void order_list(uint64_t* v, uint64_t* out, int n) {
+  if (n <= kRankMax) {  // each one's place is the number of larger ones
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const uint64_t x = v[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += v[j] > x;
+      out[rank] = x;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) v[i] = out[i];
+    __syncthreads();
+    return;
+  }
+  int size = 2 * kRankMax;
+  while (size < n) size *= 2;
+  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) v[i] = 0;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2)
+    for (int step = run / 2; step > 0; step /= 2) {
+      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
         const int i = 2 * t - (t & (step - 1)), j = i + step;
-        const bool down = (i & size) == 0;
+        const bool down = (i & run) == 0;
         const uint64_t x = v[i], y = v[j];
         if (down ? x < y : x > y) {
           v[i] = y;
@@ -486,172 +585,159 @@ DIP_DEV void sort_list(uint64_t* v, int n) {
 
 template <int kType, bool kHist>
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
-  __shared__ uint64_t lds[4 * (kThreads / 64) + 4];
-  __shared__ uint64_t list[kListMax];
+  __shared__ uint64_t lds[kLdsWords];
+  __shared__ double roots[64];
+  __shared__ uint64_t list[kHist ? kListMax : 1], spare[kHist ? kRankMax : 1];
   __shared__ unsigned long long sums[kMaxSlices];
-  __shared__ uint32_t hn[kRadixBins];
-  __shared__ unsigned long long hw[kRadixBins];
+  __shared__ uint32_t hn[kHist ? kRadixBins : 1];
+  __shared__ unsigned long long hw[kHist ? kRadixBins : 1];
   const int r = blockIdx.x, tid = threadIdx.x;
   const char* row = row_of(a, r);
-  RowState& st = a.rows[r];
+  const RowState& st = row_state(a, r);
   uint64_t* sh = lds + 2 * (kThreads / 64);
-  uint64_t best;
-  uint32_t least;
-  row_ends<kThreads>(a, st, lds, best, least);
-  const uint32_t top = (uint32_t)(best >> 32);
-  if (top <= kKeyMinusInf || a.temperature == 0) {  // nothing to choose from, or greedy
+  const Plan p = st.plan;
+  if (p.top <= kKeyMinusInf) {  // nothing to choose from
     if (tid == 0) {
-      const bool some = top > kKeyMinusInf;
-      a.token[r] = some ? (int64_t)(uint32_t)~(uint32_t)best : 0;
-      if (a.prob) a.prob[r] = some ? 1.f : 0.f;
+      a.token[r] = 0;
+      if (a.prob) a.prob[r] = 0.f;
     }
     return;
   }
-  const Weigher wt(a, top, least);
+  const int n = kHist && p.lo < kBins ? (int)min(st.listed, (uint32_t)kListMax + 1) : 0;
+  if (tid < a.slices) sums[tid] = st.sure[tid];
+  if (kHist && n <= kListMax)
+    for (int i = tid; i < n; i += kThreads) list[i] = st.list[i];
+  const double u = a.u[r];
+  const Weigher wt(a, p.top, p.least, roots);
+  __syncthreads();
   constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
   const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
   auto slice_of = [&](int64_t i) { return (int)((i + off) / kVec / a.slice_vecs); };
-  for (int s = tid; s < a.slices; s += kThreads) sums[s] = st.sure[s];
   Cut cut{0u, a.vocab};
   auto kept = [&](uint32_t k, int64_t i) { return k > cut.key || (k == cut.key && i <= cut.index); };
-  if (kHist) {
-    const Plan p = make_plan<kThreads>(a, st, wt, lds);
-    const bool by_k = a.top_k > 0 && (uint64_t)a.top_k < p.tokens;
-    const uint32_t n = p.lo < kBins ? st.listed : 0u;
-    if (n > kListMax) {
-      if (by_k)
-        cut = search_bits<kType>(a, row, wt, kept, (uint64_t)a.top_k, -1.0, hn, hw, lds);
-      if (a.top_p < 1) {
-        uint64_t w = 0;
-        each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), tid, kThreads,
-                          [&](int64_t i, uint32_t k) {
-                            if (kept(k, i)) w += wt.whole_of(k);
-                          });
-        w = block_reduce<kThreads>(w, [](uint64_t x, uint64_t y) { return x + y; }, lds);
-        cut = search_bits<kType>(a, row, wt, kept, 0, a.top_p * (double)w, hn, hw, lds);
-      }
-      for (int s = tid; s < a.slices; s += kThreads) sums[s] = 0;
-      __syncthreads();
-      each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), tid, kThreads,
+  if (kHist && n > kListMax) {
+    if (p.by_k) cut = search_bits<kType>(a, row, wt, kept, (uint64_t)a.top_k, -1.0, hn, hw, lds);
+    if (a.top_p < 1) {
+      uint64_t w = 0;
+      each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab),
                         [&](int64_t i, uint32_t k) {
-                          if (!kept(k, i)) return;
-                          const unsigned long long w = wt.kept_whole(k);
-                          if (w) atomicAdd(&sums[slice_of(i)], w);
+                          if (kept(k, i)) w += wt.whole_of(k);
                         });
-    } else if (n > 0) {
-      int size = 64;
-      while (size < (int)n) size *= 2;
-      for (int i = tid; i < size; i += kThreads) list[i] = i < (int)n ? st.list[i] : 0;
-      __syncthreads();
-      sort_list(list, size);
-      // kPer neighbours per thread, and the weights before them
-      constexpr int kPer = kListMax / kThreads;
-      unsigned long long w[kPer];
+      w = block_reduce(w, [](uint64_t x, uint64_t y) { return x + y; }, lds);
+      cut = search_bits<kType>(a, row, wt, kept, 0, a.top_p * (double)w, hn, hw, lds);
+    }
+    if (tid < a.slices) sums[tid] = 0;
+    __syncthreads();
+    each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, uint32_t k) {
+      if (!kept(k, i)) return;
+      const unsigned long long w = wt.kept_whole(k);
+      if (w) atomicAdd(&sums[slice_of(i)], w);
+    });
+  } else if (kHist && n > 0) {
+    order_list(list, spare, n);
+    // a run of `per` neighbours per thread, and the weights before it
+    const int per = (n + kThreads - 1) / kThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    int last = n - 1;  // of the list, kept by top-k and top-p
+    if (p.ranked) {
       uint64_t mine = 0, all;
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int i = tid * kPer + e;
-        w[e] = i < (int)n ? wt.whole_of((uint32_t)(list[i] >> 32)) : 0;
-        mine += w[e];
-      }
-      const uint64_t before = block_exclusive<kThreads>(mine, lds, all);
-      const int nk = by_k ? (int)min((uint64_t)n, (uint64_t)a.top_k - p.above_n) : (int)n;
-      int last = nk - 1;  // of the list, kept
+      for (int i = i0; i < i1; ++i) mine += wt.whole_of((uint32_t)(list[i] >> 32));
+      const uint64_t before = p.above_w + block_exclusive(mine, lds, all);
+      if (p.by_k) last = (int)min((uint64_t)n, (uint64_t)a.top_k - p.above_n) - 1;
       if (a.top_p < 1) {
-        // the sum that top-p takes its share of
-        if (tid == 0) sh[1] = (uint64_t)nk;
-        if (by_k) {
-          uint64_t run = before;
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            run += w[e];
-            if (tid * kPer + e == nk - 1) sh[0] = p.above_w + run;
+        if (tid == 0) sh[1] = (uint64_t)last;
+        uint64_t run = before;
+        if (p.by_k) {  // the sum that top-p takes its share of
+          for (int i = i0; i < i1; ++i) {
+            run += wt.whole_of((uint32_t)(list[i] >> 32));
+            if (i == last) sh[0] = run;
           }
         } else if (tid == 0) {
           sh[0] = p.total;
         }
         __syncthreads();
         const double mass = a.top_p * (double)sh[0];
-        uint64_t run = p.above_w + before;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
+        run = before;
+        for (int i = i0; i < i1; ++i) {
           const bool was = (double)run >= mass;
-          run += w[e];
-          if (tid * kPer + e < nk && !was && (double)run >= mass) sh[1] = (uint64_t)(tid * kPer + e);
+          run += wt.whole_of((uint32_t)(list[i] >> 32));
+          if (i <= last && !was && (double)run >= mass) sh[1] = (uint64_t)i;
         }
         __syncthreads();
-        last = min(last, (int)sh[1]);
+        last = (int)sh[1];
       }
-      cut.key = (uint32_t)(list[last] >> 32);
-      cut.index = (int64_t)(uint32_t)~(uint32_t)list[last];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int i = tid * kPer + e;
-        if (i > last) continue;
-        const unsigned long long x = wt.kept_whole((uint32_t)(list[i] >> 32));
-        if (x) atomicAdd(&sums[slice_of((int64_t)(uint32_t)~(uint32_t)list[i])], x);
-      }
+    }
+    cut.key = (uint32_t)(list[last] >> 32);
+    cut.index = (int64_t)(uint32_t)~(uint32_t)list[last];
+    for (int i = i0; i < i1 && i <= last; ++i) {
+      const unsigned long long x = wt.kept_whole((uint32_t)(list[i] >> 32));
+      if (x) atomicAdd(&sums[slice_of((int64_t)(uint32_t)~(uint32_t)list[i])], x);
     }
   }
   __syncthreads();
   // the slice, then the token in it: running sums by index
   uint64_t total;
   const uint64_t mine = tid < a.slices ? sums[tid] : 0;
-  const uint64_t before = block_exclusive<kThreads>(mine, lds, total);
+  const uint64_t before = block_exclusive(mine, lds, total);
   // u beyond 1 or NaN: the last kept token
-  double t = (double)a.u[r] * (double)total;
-  uint64_t goal = t >= 0 ? (t < (double)total ? (uint64_t)t : total - 1) : (t < 0 ? 0 : total - 1);
+  const double t = u * (double)total;
+  uint64_t goal = t < 0 ? 0 : t < (double)total ? (uint64_t)t : total - 1;
   goal = min(goal, total - 1);
   if (goal >= before && goal - before < mine) {
     sh[0] = (uint64_t)tid;
     sh[1] = before;
   }
   __syncthreads();
-  const int s = (int)sh[0];
+  const int64_t v0 = (int64_t)sh[0] * a.slice_vecs;
+  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
   goal -= sh[1];  // within the slice
-  const int64_t lo = max((int64_t)0, s * a.slice_vecs * kVec - off);
-  const int64_t end = min((s + 1) * a.slice_vecs * kVec - off, a.vocab);
-  const int64_t per = (end - lo + kThreads - 1) / kThreads;
-  const int64_t i0 = min(lo + tid * per, end), i1 = min(i0 + per, end);
+  // a run of neighbouring pieces per thread
+  const int64_t per = (v1 - v0 + kThreads - 1) / kThreads;
+  const int64_t e0 = max((int64_t)0, (v0 + tid * per) * kVec - off);
+  const int64_t e1 = min(min((v0 + (tid + 1) * per) * kVec, v1 * kVec) - off, a.vocab);
+  auto weight = [&](int64_t i, uint32_t& k) {
+    k = order_key(load_logit<kType>(row, i));
+    return k > kKeyMinusInf && kept(k, i) ? wt.kept_whole(k) : 0ull;
+  };
   uint64_t here = 0, in_slice;
-  for (int64_t i = i0; i < i1; ++i) {
-    const uint32_t k = order_key(load_logit<kType>(row, i));
-    if (k > kKeyMinusInf && kept(k, i)) here += wt.kept_whole(k);
-  }
-  uint64_t run = block_exclusive<kThreads>(here, lds, in_slice);
-  if (goal >= run && goal - run < here) {
-    for (int64_t i = i0; i < i1; ++i) {
-      const uint32_t k = order_key(load_logit<kType>(row, i));
-      if (k <= kKeyMinusInf || !kept(k, i)) continue;
-      run += wt.kept_whole(k);
-      if (run > goal) {
-        a.token[r] = i;
-        if (a.prob) a.prob[r] = (float)(wt.weight(k) * wt.scale / (double)total);
-        break;
-      }
+  uint32_t k;
+#pragma unroll 8
+  for (int64_t i = e0; i < e1; ++i) here += weight(i, k);
+  uint64_t run = block_exclusive(here, lds, in_slice);
+  if (goal < run || goal - run >= here) return;
+  for (int64_t i = e0; i < e1; ++i) {
+    run += weight(i, k);
+    if (run > goal) {
+      a.token[r] = i;
+      if (a.prob) a.prob[r] = (float)(wt.scaled(k) / (double)total);
+      break;
     }
   }
 }
 
-// Slices of a row: about a thousand workgroups in all, of 512 pieces at least.
+// Slices of a row: about a thousand workgroups in all, of 256 pieces at least.
 inline int slices_for(int64_t rows, int64_t vecs) {
-  const int64_t want = max((int64_t)1, 1024 / rows), most = (vecs + 511) / 512;
+  const int64_t want = max((int64_t)1, 1024 / rows), most = (vecs + 255) / 256;
   return (int)max((int64_t)1, min(min(want, most), (int64_t)kMaxSlices));
 }
+inline int64_t max_vecs(int64_t vocab, int size) { return (vocab * size + 15) / 16 + 1; }
 
 template <int kType>
 int launch_sample(const SampleArgs& a, int rows, hipStream_t s) {
-  const dim3 grid((unsigned)rows * a.slices), slice(kSliceThreads);
-  hipLaunchKernelGGL((sample_max_kernel<kType>), grid, slice, 0, s, a);
-  const bool hist = a.temperature > 0 && ((a.top_k > 0 && a.top_k < a.vocab) || a.top_p < 1);
-  if (hist) {
-    hipLaunchKernelGGL((sample_hist_kernel<kType>), grid, slice, 0, s, a);
-    hipLaunchKernelGGL((sample_gather_kernel<kType, true>), grid, slice, 0, s, a);
-    hipLaunchKernelGGL((sample_draw_kernel<kType, true>), dim3(rows), dim3(kThreads), 0, s, a);
+  const dim3 slices((unsigned)rows * a.slices), each(rows), block(kThreads);
+  hipLaunchKernelGGL((sample_max_kernel<kType>), slices, block, 0, s, a);
+  const bool count = a.top_k > 0 && a.top_k < a.vocab;
+  if (a.temperature == 0) {
+    hipLaunchKernelGGL(sample_greedy_kernel, each, block, 0, s, a);
+  } else if (count || a.top_p < 1) {
+    if (count)
+      hipLaunchKernelGGL((sample_hist_kernel<kType, true>), slices, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((sample_hist_kernel<kType, false>), slices, block, 0, s, a);
+    hipLaunchKernelGGL((sample_gather_kernel<kType, true>), slices, block, 0, s, a);
+    hipLaunchKernelGGL((sample_draw_kernel<kType, true>), each, block, 0, s, a);
   } else {
-    if (a.temperature > 0)
-      hipLaunchKernelGGL((sample_gather_kernel<kType, false>), grid, slice, 0, s, a);
-    hipLaunchKernelGGL((sample_draw_kernel<kType, false>), dim3(rows), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((sample_gather_kernel<kType, false>), slices, block, 0, s, a);
+    hipLaunchKernelGGL((sample_draw_kernel<kType, false>), each, block, 0, s, a);
   }
   return hip_status(hipGetLastError());
 }
@@ -661,9 +747,11 @@ int launch_sample(const SampleArgs& a, int rows, hipStream_t s) {
 
 using namespace dip;
 
+// For fp32 logits, which take the most slices.
 extern "C" size_t dip_sample_workspace_size(int64_t rows, int64_t vocab) {
   if (rows <= 0 || vocab <= 0) return 0;
-  return (size_t)rows * sizeof(RowState);
+  return (size_t)rows * (sizeof(RowState) +
+                         (size_t)slices_for(rows, max_vecs(vocab, 4)) * kBins * sizeof(uint64_t));
 }
 
 extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t vocab,
@@ -683,10 +771,13 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
   if (reinterpret_cast<uintptr_t>(logits) % size || !aligned16(workspace)) return DIP_ERR_ALIGN;
   int shift = 62;
   for (int64_t n = 1; n < vocab; n *= 2) --shift;
-  const int64_t vecs = (vocab * size + 15) / 16 + 1;
+  shift = min(shift, 51);
+  const int64_t vecs = max_vecs(vocab, size);
   const int slices = slices_for(rows, vecs);
   SampleArgs a{logits, vocab, row_stride * size, u, temperature, top_p, min_p, top_k, shift, slices,
-               (vecs + slices - 1) / slices, static_cast<RowState*>(workspace), token, prob};
+               (vecs + slices - 1) / slices, static_cast<char*>(workspace),
+               (int64_t)(sizeof(RowState) + (size_t)slices * kBins * sizeof(uint64_t)), token,
+               prob};
   hipStream_t s = (hipStream_t)stream;
   if (dtype == DIP_F32) return launch_sample<DIP_F32>(a, (int)rows, s);
   if (dtype == DIP_F16) return launch_sample<DIP_F16>(a, (int)rows, s);
