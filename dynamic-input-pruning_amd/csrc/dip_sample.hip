@@ -110,32 +110,33 @@ DIP_DEV const char* row_of(const SampleArgs& a, int r) {
   return static_cast<const char*>(a.logits) + (int64_t)r * a.row_bytes;
 }
 
-// f(index, order_key) of every token in the 16-byte pieces [v0, v1) of a row, by the
-// workgroup's threads.  Pieces lie where memory has them; one that reaches over an
-// end of the row is loaded token by token.
+// f(index, order_key) of the tokens in 16-byte piece v of a row.  Pieces lie where
+// memory has them; one that reaches over an end of the row is loaded token by token.
+template <int kType, typename F>
+DIP_DEV void piece_tokens(const char* row, int64_t vocab, int64_t v, F f) {
+  constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
+  const int64_t e0 = v * kVec - (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
+  if (e0 >= 0 && e0 + kVec <= vocab) {
+    const uint4 w = *reinterpret_cast<const uint4*>(row + e0 * kSize);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      const uint32_t b = kSize == 4 ? x[i] : (x[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+      const float l = kType == DIP_F32   ? __uint_as_float(b)
+                      : kType == DIP_F16 ? __half2float(__ushort_as_half((unsigned short)b))
+                                         : bf16_to_f32(b);
+      f(e0 + i, order_key(l));
+    }
+  } else {
+    for (int i = 0; i < kVec; ++i)
+      if (e0 + i >= 0 && e0 + i < vocab) f(e0 + i, order_key(load_logit<kType>(row, e0 + i)));
+  }
+}
+
+// The same of the pieces [v0, v1), by the workgroup's threads.
 template <int kType, typename F>
 DIP_DEV void each_token(const char* row, int64_t vocab, int64_t v0, int64_t v1, F f) {
-  constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
-  const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += kThreads) {
-    const int64_t e0 = v * kVec - off;
-    if (e0 >= 0 && e0 + kVec <= vocab) {
-      const uint4 w = *reinterpret_cast<const uint4*>(row + e0 * kSize);
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const uint32_t b = kSize == 4 ? x[i] : (x[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
-        const float l = kType == DIP_F32   ? __uint_as_float(b)
-                        : kType == DIP_F16 ? __half2float(__ushort_as_half((unsigned short)b))
-                                           : bf16_to_f32(b);
-        f(e0 + i, order_key(l));
-      }
-    } else {
-      for (int i = 0; i < kVec; ++i)
-        if (e0 + i >= 0 && e0 + i < vocab)
-          f(e0 + i, order_key(load_logit<kType>(row, e0 + i)));
-    }
-  }
+  for (int64_t v = v0 + threadIdx.x; v < v1; v += kThreads) piece_tokens<kType>(row, vocab, v, f);
 }
 
 template <int kType>
@@ -690,27 +691,36 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   const int64_t v0 = (int64_t)sh[0] * a.slice_vecs;
   const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
   goal -= sh[1];  // within the slice
-  // a run of neighbouring pieces per thread
+  // a run of neighbouring pieces per thread; then the run that the draw falls in,
+  // a token per thread
   const int64_t per = (v1 - v0 + kThreads - 1) / kThreads;
-  const int64_t e0 = max((int64_t)0, (v0 + tid * per) * kVec - off);
-  const int64_t e1 = min(min((v0 + (tid + 1) * per) * kVec, v1 * kVec) - off, a.vocab);
-  auto weight = [&](int64_t i, uint32_t& k) {
-    k = order_key(load_logit<kType>(row, i));
-    return k > kKeyMinusInf && kept(k, i) ? wt.kept_whole(k) : 0ull;
-  };
+  const int64_t w0 = min(v0 + tid * per, v1), w1 = min(w0 + per, v1);
   uint64_t here = 0, in_slice;
-  uint32_t k;
-#pragma unroll 8
-  for (int64_t i = e0; i < e1; ++i) here += weight(i, k);
-  uint64_t run = block_exclusive(here, lds, in_slice);
-  if (goal < run || goal - run >= here) return;
-  for (int64_t i = e0; i < e1; ++i) {
-    run += weight(i, k);
-    if (run > goal) {
+  for (int64_t v = w0; v < w1; ++v)
+    piece_tokens<kType>(row, a.vocab, v, [&](int64_t i, uint32_t k) {
+      if (kept(k, i)) here += wt.kept_whole(k);
+    });
+  const uint64_t run = block_exclusive(here, lds, in_slice);
+  if (goal >= run && goal - run < here) {
+    sh[0] = (uint64_t)w0;
+    sh[1] = goal - run;
+  }
+  __syncthreads();
+  const int64_t first = (int64_t)sh[0] * kVec - off;
+  const int64_t end = min(first + per * kVec, a.vocab);
+  goal = sh[1];
+  for (int64_t i0 = max(first, (int64_t)0); i0 < end; i0 += kThreads) {
+    const int64_t i = i0 + tid;
+    const uint32_t k = i < end ? order_key(load_logit<kType>(row, i)) : 0u;
+    const uint64_t w = i < end && kept(k, i) ? wt.kept_whole(k) : 0ull;
+    uint64_t all;
+    const uint64_t sum = block_exclusive(w, lds, all);
+    if (goal >= sum && goal - sum < w) {
       a.token[r] = i;
       if (a.prob) a.prob[r] = (float)(wt.scaled(k) / (double)total);
-      break;
     }
+    if (goal < all) break;
+    goal -= all;
   }
 }
 
