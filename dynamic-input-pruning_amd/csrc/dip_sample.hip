@@ -32,6 +32,7 @@
 #include "dip_internal.h"
 
 #include <hip/hip_fp16.h>
+#include <math.h>
 
 namespace dip {
 namespace {
@@ -42,24 +43,25 @@ constexpr int kListMax = 4096;
 constexpr int kRankMax = 512;  // longer lists are sorted, not ranked by comparing all pairs
 constexpr int kMaxSlices = 256;
 constexpr int kRadixBins = 256;
-constexpr uint32_t kKeyMinusInf = 0x007FFFFFu;  // order_key of -inf, and of NaN
+constexpr uint32_t kKeyMinusInf = 0x007FFFFFu;  // order_key of -inf
 
-// fp32 as a whole number that orders like it, -0 as 0 and NaN as -inf.
+// fp32 (no NaN) as a whole number that orders like it, -0 as 0.
 DIP_DEV uint32_t order_key(float x) {
-  x += 0.f;
-  if (x != x) return kKeyMinusInf;
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 DIP_DEV float key_value(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// NaN as -inf.
+DIP_DEV float no_nan(float x) { return fmaxf(x, -INFINITY); }
+
 template <int kType>
 DIP_DEV float load_logit(const void* row, int64_t i) {
-  if (kType == DIP_F32) return static_cast<const float*>(row)[i];
-  if (kType == DIP_F16) return __half2float(static_cast<const __half*>(row)[i]);
-  return bf16_to_f32(static_cast<const uint16_t*>(row)[i]);
+  if (kType == DIP_F32) return no_nan(static_cast<const float*>(row)[i]);
+  if (kType == DIP_F16) return no_nan(__half2float(static_cast<const __half*>(row)[i]));
+  return no_nan(bf16_to_f32(static_cast<const uint16_t*>(row)[i]));
 }
 
 // Where the histogram says that the borders lie, and the row's ends.
@@ -88,8 +90,9 @@ struct SampleArgs {
   const void* logits;
   int64_t vocab, row_bytes;
   const float* u;
-  double temperature, top_p, min_p;
+  double top_p, per_64th, least, least_64ths;  // see Weigher; min-p in 64ths of an octave
   int64_t top_k;
+  float per_hi, per_lo;
   int shift;
   int slices;
   int64_t slice_vecs;  // 16-byte pieces of a row that a slice takes
@@ -110,33 +113,74 @@ DIP_DEV const char* row_of(const SampleArgs& a, int r) {
   return static_cast<const char*>(a.logits) + (int64_t)r * a.row_bytes;
 }
 
-// f(index, order_key) of the tokens in 16-byte piece v of a row.  Pieces lie where
-// memory has them; one that reaches over an end of the row is loaded token by token.
-template <int kType, typename F>
-DIP_DEV void piece_tokens(const char* row, int64_t vocab, int64_t v, F f) {
-  constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
-  const int64_t e0 = v * kVec - (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
-  if (e0 >= 0 && e0 + kVec <= vocab) {
-    const uint4 w = *reinterpret_cast<const uint4*>(row + e0 * kSize);
-    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+// The 16-byte piece v of a row.  Pieces lie where memory has them; one that reaches
+// over an end of the row is not loaded here, but token by token by its visitor.
+template <int kType>
+struct Piece {
+  static constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
+  int64_t first;  // its first token
+  bool inside;
+  uint4 w;
+
+  DIP_DEV Piece() {}
+  DIP_DEV Piece(const char* row, int64_t vocab, int64_t v) {
+    first = v * kVec - (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
+    inside = first >= 0 && first + kVec <= vocab;
+    w = make_uint4(0, 0, 0, 0);
+    if (inside) w = *reinterpret_cast<const uint4*>(row + first * kSize);
+  }
+  // f(index, logit) of its tokens, NaN as -inf.
+  template <typename F>
+  DIP_DEV void tokens(const char* row, int64_t vocab, F f) const {
+    if (inside) {
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const uint32_t b = kSize == 4 ? x[i] : (x[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
-      const float l = kType == DIP_F32   ? __uint_as_float(b)
-                      : kType == DIP_F16 ? __half2float(__ushort_as_half((unsigned short)b))
-                                         : bf16_to_f32(b);
-      f(e0 + i, order_key(l));
+      for (int i = 0; i < kVec; ++i) {
+        const uint32_t b = kSize == 4 ? x[i] : (x[i / 2] >> (16 * (i & 1))) & 0xFFFFu;
+        const float l = kType == DIP_F32   ? __uint_as_float(b)
+                        : kType == DIP_F16 ? __half2float(__ushort_as_half((unsigned short)b))
+                                           : bf16_to_f32(b);
+        f(first + i, no_nan(l));
+      }
+    } else {
+      for (int i = 0; i < kVec; ++i)
+        if (first + i >= 0 && first + i < vocab)
+          f(first + i, load_logit<kType>(row, first + i));
     }
-  } else {
-    for (int i = 0; i < kVec; ++i)
-      if (e0 + i >= 0 && e0 + i < vocab) f(e0 + i, order_key(load_logit<kType>(row, e0 + i)));
+  }
+};
+
+// kAhead pieces of a thread, kThreads apart, loaded together: a row's pass is a
+// few waits for memory, not one per piece (250 rows of 32003, four pieces one after
+// the other: 15.6 us).
+constexpr int kAhead = 4;
+
+template <int kType>
+struct Batch {
+  Piece<kType> p[kAhead];
+
+  DIP_DEV Batch(const char* row, int64_t vocab, int64_t v) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) p[j] = Piece<kType>(row, vocab, v + j * kThreads);
+  }
+};
+
+// f(index, logit) of the tokens in the pieces [v0, v1) by the workgroup's threads,
+// `head` being this thread's first ones (loaded before what the caller waits for).
+template <int kType, typename F>
+DIP_DEV void each_token(Batch<kType> head, const char* row, int64_t vocab, int64_t v0,
+                        int64_t v1, F f) {
+  for (int64_t v = v0 + threadIdx.x; v < v1;) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v + j * kThreads < v1) head.p[j].tokens(row, vocab, f);
+    v += kAhead * kThreads;
+    if (v < v1) head = Batch<kType>(row, vocab, v);
   }
 }
-
-// The same of the pieces [v0, v1), by the workgroup's threads.
 template <int kType, typename F>
 DIP_DEV void each_token(const char* row, int64_t vocab, int64_t v0, int64_t v1, F f) {
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += kThreads) piece_tokens<kType>(row, vocab, v, f);
+  each_token<kType>(Batch<kType>(row, vocab, v0 + threadIdx.x), row, vocab, v0, v1, f);
 }
 
 template <int kType>
@@ -145,51 +189,98 @@ DIP_DEV int64_t row_vecs(const char* row, int64_t vocab) {
   return ((reinterpret_cast<uintptr_t>(row) & 15) + vocab * kSize + 15) / 16;
 }
 
-// What a row's largest logit makes of the others.  Weights are 2^-(k / 64) 2^-(f / 64)
-// with k + f = 64 (max - logit) / (temperature ln 2): a table of 64 roots and the
-// series of exp to z^5 (z < 0.011, so the rest is below 2e-15).
+// 2^-(j / 64), j = 0 .. 63, from the series of exp.
+struct Roots {
+  double v[64];
+  constexpr Roots() : v() {
+    for (int j = 0; j < 64; ++j) {
+      const double x = -0.69314718055994530942 * j / 64;
+      double term = 1.0, sum = 1.0;
+      for (int i = 1; i < 24; ++i) {
+        term *= x / i;
+        sum += term;
+      }
+      v[j] = sum;
+    }
+  }
+};
+__device__ const Roots kRoots = Roots();
+
+// What a row's largest logit makes of the others.  A weight is 2^-(n / 64) exp(z)
+// with n - 64 z / ln 2 = 64 (max - logit) / (temperature ln 2), |z| < 0.0055: a table
+// of 64 roots in 64 bits, and z and exp(z) - 1 = z + z^2 / 2 + z^3 / 6 in 32, with the
+// roundings of the difference and of its product carried along.  That is off by
+// 4e-10 of the weight, at random; a running sum over n tokens by 4e-10 / sqrt(n) of
+// itself.  (All in 64 bits, whose conversions run at a quarter of the rate: 250
+// rows of 32003 15.7 us in the launch that adds the weights up.)
 struct Weigher {
-  uint32_t top;
-  double most, per_64th, least;  // 64ths of an octave per logit; min-p, scaled
+  float most, per_hi, per_lo;  // 64ths of an octave per logit, in two parts
+  bool inf;                    // the largest is +inf, and only its equals count
+  double least;                // min-p * 2^shift
   float bins_per_logit;
-  const double* roots;  // 2^(shift - j / 64), in LDS
+  const double* roots;         // 2^(shift - j / 64), in LDS
 
   // The workgroup's `lds` gets the roots; a barrier must follow before their use.
   DIP_DEV Weigher(const SampleArgs& a, uint32_t top_key, uint32_t least_key, double* lds)
-      : top(top_key), roots(lds) {
-    if (threadIdx.x < 64) lds[threadIdx.x] = exp2(a.shift - threadIdx.x * (1.0 / 64));
-    most = key_value(top);
-    per_64th = 64 * 1.4426950408889634074 / a.temperature;
-    least = a.min_p * (double)(1ull << a.shift);
+      : per_hi(a.per_hi), per_lo(a.per_lo), least(a.least), roots(lds) {
+    if (threadIdx.x < 64)
+      lds[threadIdx.x] = __builtin_amdgcn_ldexp(kRoots.v[threadIdx.x], a.shift);
+    most = key_value(top_key);
+    inf = most == INFINITY;
+    if (inf) most = 0.f;
     // bins reach down to the smallest logit, or to the weight that counts as 0
-    const double range = min(most - (double)key_value(least_key), 64 * (a.shift + 1) / per_64th);
-    bins_per_logit = range > 0 ? (float)(kBins / range) : 0.f;
+    const float range = fminf(most - key_value(least_key), 64.f * (a.shift + 1) / per_hi);
+    bins_per_logit = range > 0.f && !inf ? fminf(kBins / range, 3e38f) : 0.f;
   }
-  // w * 2^shift
-  DIP_DEV double scaled(uint32_t k) const {
-    if (k == top) return roots[0];
-    if (k <= kKeyMinusInf) return 0.0;
-    const double d = fmin((most - (double)key_value(k)) * per_64th, 64 * 64.0);
-    const int n = (int)d;
-    const double z = (d - n) * (-0.69314718055994530942 / 64);
-    const double p = fma(z, fma(z, fma(z, fma(z, fma(z, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0),
-                         1.0);
-    return ldexp(roots[n & 63] * p, -(n >> 6));
+  // The logits that the other functions take.
+  DIP_DEV float value(float x) const {
+    return !inf ? x : x == INFINITY ? 0.f : -INFINITY;
+  }
+  // w * 2^shift; 0 for -inf.  kExact: the difference's rounding counts (of bf16 and
+  // fp16 numbers it is rounded only where the smaller is below 2^-13 of the larger).
+  template <bool kExact>
+  DIP_DEV double scaled(float x) const {
+    const float hi = most - x, n = rintf(hi * per_hi);
+    float low = hi * per_lo;
+    if (kExact) {
+      const float part = hi - most;  // most - x = hi + lo exactly
+      const float lo = (most - (hi - part)) - (x + part);
+      low = fmaf(lo, per_hi, low);
+    }
+    const float f = fmaf(-hi, per_hi, n) - low;
+    constexpr float c = 0.69314718055994530942f / 64;
+    const float q = f * fmaf(f, fmaf(f, c * c * c / 6, c * c / 2), c);
+    const int i = (int)fminf(n, 4096.f);
+    const double r = roots[i & 63];
+    // the octaves off the exponent (a root's is 2^shift or less, 2^-14 at the least)
+    const uint64_t w = __builtin_bit_cast(uint64_t, fma(r, (double)q, r)) -
+                       ((uint64_t)((uint32_t)(i & ~63) << 14) << 32);
+    return n <= 64.f * 60 ? __builtin_bit_cast(double, w) : 0.0;  // (not for -inf)
   }
   // Rounded to a whole number: below 2^52, so the sum's low bits are it.
   DIP_DEV static unsigned long long whole(double w) {
     return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
   }
-  DIP_DEV unsigned long long whole_of(uint32_t k) const { return whole(scaled(k)); }
+  template <bool kExact>
+  DIP_DEV unsigned long long whole_of(float x) const {
+    return whole(scaled<kExact>(x));
+  }
   // The weight if min-p keeps it, else 0.
-  DIP_DEV unsigned long long kept_whole(uint32_t k) const {
-    const double w = scaled(k);
+  template <bool kExact>
+  DIP_DEV unsigned long long kept_whole(float x) const {
+    const double w = scaled<kExact>(x);
     return w >= least ? whole(w) : 0ull;
   }
   // Never lower for a smaller logit.
-  DIP_DEV int bin(uint32_t k) const {
-    if (k == top) return 0;
-    return (int)fminf(((float)most - key_value(k)) * bins_per_logit, (float)(kBins - 1));
+  DIP_DEV int bin(float x) const {
+    return (int)fminf((most - x) * bins_per_logit, (float)(kBins - 1));
+  }
+  // The same of logits as they are, given by their keys.
+  DIP_DEV double key_scaled(uint32_t k) const { return scaled<true>(value(key_value(k))); }
+  DIP_DEV unsigned long long key_whole(uint32_t k) const { return whole(key_scaled(k)); }
+  DIP_DEV unsigned long long key_kept(uint32_t k) const {
+    const double w = key_scaled(k);
+    return w >= least ? whole(w) : 0ull;
   }
 };
 
@@ -322,8 +413,8 @@ DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& w
   p.ranked = p.lo < kBins;
   // min-p's border: surely in the bins m .. m + 2.  If nothing is to be looked for
   // before their end, they alone are listed; if they begin before lo, from there on.
-  if (a.min_p > 0) {
-    const double bin = -log2(a.min_p) * 64 / wt.per_64th * wt.bins_per_logit;
+  if (a.least > 0) {
+    const double bin = a.least_64ths / a.per_64th * wt.bins_per_logit;
     const int m = max(0, (bin < kBins ? (int)bin : kBins) - 1);
     if (m < p.lo && m < kBins) {
       if (m + 2 < p.lo) {
@@ -349,28 +440,32 @@ DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& w
   return p;
 }
 
-template <int kType>
+// kIndex: of equal ones the first, for greedy draws.
+template <int kType, bool kIndex>
 __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
   __shared__ uint64_t lds[kLdsWords];
   const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
   const char* row = row_of(a, r);
   RowState& st = row_state(a, r);
-  uint64_t best = 0;
-  uint32_t least = 0xFFFFFFFFu;
+  float most = -INFINITY, low = INFINITY;
+  int64_t at = 0;  // a thread's tokens come in ascending order
   each_token<kType>(row, a.vocab, s * a.slice_vecs,
                     min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)),
-                    [&](int64_t i, uint32_t k) {
-                      best = max(best, (uint64_t)k << 32 | (uint32_t)~(uint32_t)i);
-                      if (k > kKeyMinusInf) least = min(least, k);
+                    [&](int64_t i, float x) {
+                      if (kIndex) at = x > most ? i : at;
+                      most = fmaxf(most, x);
+                      if (!kIndex) low = fminf(low, x == -INFINITY ? INFINITY : x);
                     });
+  uint64_t best = (uint64_t)order_key(most) << 32 | (uint32_t)~(uint32_t)at;
   best = block_reduce(best, [](uint64_t x, uint64_t y) { return max(x, y); }, lds);
-  least = block_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); },
-                       reinterpret_cast<uint32_t*>(lds));
+  const uint32_t least = block_reduce(order_key(low), [](uint32_t x, uint32_t y) { return min(x, y); },
+                                      reinterpret_cast<uint32_t*>(lds));
   if (threadIdx.x == 0) {
     st.best[s] = best;
     st.least[s] = least;
     if (s == 0) st.listed = 0;
   }
+  if (kIndex) return;
   for (int b = s * kThreads + threadIdx.x; b < kBins; b += a.slices * kThreads) {
     st.hn[b] = 0;
     st.hw[b] = 0;
@@ -387,6 +482,9 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
   const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
   const char* row = row_of(a, r);
   RowState& st = row_state(a, r);
+  const int64_t v0 = s * a.slice_vecs;
+  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
+  const Batch<kType> head(row, a.vocab, v0 + threadIdx.x);
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
     if (kCount) hn[b] = 0;
     hw[b] = 0;
@@ -398,15 +496,17 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
   if (top <= kKeyMinusInf) return;
   const Weigher wt(a, top, least, roots);
   __syncthreads();
-  each_token<kType>(row, a.vocab, s * a.slice_vecs,
-                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)),
-                    [&](int64_t, uint32_t k) {
-                      const unsigned long long w = wt.whole_of(k);
-                      if (w == 0) return;
-                      const int b = wt.bin(k);
-                      if (kCount) atomicAdd(&hn[b], 1u);
-                      atomicAdd(&hw[b], w);
-                    });
+  const auto add = [&](int64_t, float x) {
+    const unsigned long long w = wt.whole_of<kType == DIP_F32>(x);
+    if (w == 0) return;
+    const int b = wt.bin(x);
+    if (kCount) atomicAdd(&hn[b], 1u);
+    atomicAdd(&hw[b], w);
+  };
+  if (wt.inf)
+    each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) { add(i, wt.value(x)); });
+  else
+    each_token<kType>(head, row, a.vocab, v0, v1, add);
   __syncthreads();
   unsigned long long* own = slice_hist(a, r, s);
   for (int b = threadIdx.x; b < kBins; b += kThreads) {
@@ -425,6 +525,9 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
   const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
   const char* row = row_of(a, r);
   RowState& st = row_state(a, r);
+  const int64_t v0 = s * a.slice_vecs;
+  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
+  const Batch<kType> head(row, a.vocab, v0 + threadIdx.x);
   uint64_t best;
   uint32_t least;
   row_ends(a, st, lds, best, least);
@@ -436,24 +539,25 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
   }
   const Weigher wt(a, top, least, roots);
   __syncthreads();
-  const int64_t v0 = s * a.slice_vecs;
-  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
   uint64_t sure = 0;
   if (kHist) {
     p = make_plan(a, st, wt, p, lds);
     const unsigned long long* own = slice_hist(a, r, s);
     for (int b = threadIdx.x; b < p.lo; b += kThreads) sure += own[b];
     if (p.lo < kBins)
-      each_token<kType>(row, a.vocab, v0, v1, [&](int64_t i, uint32_t k) {
-        if (k <= kKeyMinusInf) return;
-        const int b = wt.bin(k);
-        if (b < p.lo || b > p.hi || wt.whole_of(k) == 0) return;
+      each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) {
+        const float y = wt.value(x);
+        const int b = wt.bin(y);
+        if (b < p.lo || b > p.hi || wt.whole_of<kType == DIP_F32>(y) == 0) return;
         const uint32_t at = atomicAdd(&st.listed, 1u);
-        if (at < kListMax) st.list[at] = (uint64_t)k << 32 | (uint32_t)~(uint32_t)i;
+        if (at < kListMax) st.list[at] = (uint64_t)order_key(x) << 32 | (uint32_t)~(uint32_t)i;
       });
   } else {
-    each_token<kType>(row, a.vocab, v0, v1,
-                      [&](int64_t, uint32_t k) { sure += wt.kept_whole(k); });
+    const auto add = [&](int64_t, float x) { sure += wt.kept_whole<kType == DIP_F32>(x); };
+    if (wt.inf)
+      each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) { add(i, wt.value(x)); });
+    else
+      each_token<kType>(head, row, a.vocab, v0, v1, add);
   }
   sure = block_reduce(sure, [](uint64_t x, uint64_t y) { return x + y; }, lds);
   if (threadIdx.x == 0) {
@@ -490,9 +594,10 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
   for (int level = 24; level >= 0; level -= 8) {
     for (int b = tid; b < kRadixBins; b += kThreads) hn[b] = 0, hw[b] = 0;
     __syncthreads();
-    each_token<kType>(row, a.vocab, 0, vecs, [&](int64_t i, uint32_t k) {
+    each_token<kType>(row, a.vocab, 0, vecs, [&](int64_t i, float x) {
+      const uint32_t k = order_key(x);
       if (!kept(k, i) || (level < 24 && (k >> (level + 8)) != (prefix >> (level + 8)))) return;
-      const unsigned long long w = wt.whole_of(k);
+      const unsigned long long w = wt.key_whole(k);
       if (w == 0) return;
       atomicAdd(&hn[(k >> level) & 255], 1u);
       atomicAdd(&hw[(k >> level) & 255], w);
@@ -528,7 +633,7 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
   }
   uint64_t need = count - above_n;
   if (by_mass) {
-    const double n = ceil((mass - (double)above_w) / (double)wt.whole_of(prefix));
+    const double n = ceil((mass - (double)above_w) / (double)wt.key_whole(prefix));
     need = n < 1.0 ? 1 : (n < (double)ties ? (uint64_t)n : ties);
   }
   // the index of the need-th token of that key
@@ -621,17 +726,19 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     if (a.top_p < 1) {
       uint64_t w = 0;
       each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab),
-                        [&](int64_t i, uint32_t k) {
-                          if (kept(k, i)) w += wt.whole_of(k);
+                        [&](int64_t i, float x) {
+                          const uint32_t k = order_key(x);
+                          if (kept(k, i)) w += wt.key_whole(k);
                         });
       w = block_reduce(w, [](uint64_t x, uint64_t y) { return x + y; }, lds);
       cut = search_bits<kType>(a, row, wt, kept, 0, a.top_p * (double)w, hn, hw, lds);
     }
     if (tid < a.slices) sums[tid] = 0;
     __syncthreads();
-    each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, uint32_t k) {
+    each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, float x) {
+      const uint32_t k = order_key(x);
       if (!kept(k, i)) return;
-      const unsigned long long w = wt.kept_whole(k);
+      const unsigned long long w = wt.key_kept(k);
       if (w) atomicAdd(&sums[slice_of(i)], w);
     });
   } else if (kHist && n > 0) {
@@ -641,7 +748,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     int last = n - 1;  // of the list, kept by top-k and top-p
     if (p.ranked) {
       uint64_t mine = 0, all;
-      for (int i = i0; i < i1; ++i) mine += wt.whole_of((uint32_t)(list[i] >> 32));
+      for (int i = i0; i < i1; ++i) mine += wt.key_whole((uint32_t)(list[i] >> 32));
       const uint64_t before = p.above_w + block_exclusive(mine, lds, all);
       if (p.by_k) last = (int)min((uint64_t)n, (uint64_t)a.top_k - p.above_n) - 1;
       if (a.top_p < 1) {
@@ -649,7 +756,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         uint64_t run = before;
         if (p.by_k) {  // the sum that top-p takes its share of
           for (int i = i0; i < i1; ++i) {
-            run += wt.whole_of((uint32_t)(list[i] >> 32));
+            run += wt.key_whole((uint32_t)(list[i] >> 32));
             if (i == last) sh[0] = run;
           }
         } else if (tid == 0) {
@@ -660,7 +767,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
         run = before;
         for (int i = i0; i < i1; ++i) {
           const bool was = (double)run >= mass;
-          run += wt.whole_of((uint32_t)(list[i] >> 32));
+          run += wt.key_whole((uint32_t)(list[i] >> 32));
           if (i <= last && !was && (double)run >= mass) sh[1] = (uint64_t)i;
         }
         __syncthreads();
@@ -670,7 +777,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     cut.key = (uint32_t)(list[last] >> 32);
     cut.index = (int64_t)(uint32_t)~(uint32_t)list[last];
     for (int i = i0; i < i1 && i <= last; ++i) {
-      const unsigned long long x = wt.kept_whole((uint32_t)(list[i] >> 32));
+      const unsigned long long x = wt.key_kept((uint32_t)(list[i] >> 32));
       if (x) atomicAdd(&sums[slice_of((int64_t)(uint32_t)~(uint32_t)list[i])], x);
     }
   }
@@ -696,10 +803,18 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   const int64_t per = (v1 - v0 + kThreads - 1) / kThreads;
   const int64_t w0 = min(v0 + tid * per, v1), w1 = min(w0 + per, v1);
   uint64_t here = 0, in_slice;
-  for (int64_t v = w0; v < w1; ++v)
-    piece_tokens<kType>(row, a.vocab, v, [&](int64_t i, uint32_t k) {
-      if (kept(k, i)) here += wt.kept_whole(k);
-    });
+  for (int64_t v = w0; v < w1; v += kAhead) {
+    Piece<kType> p[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) p[j] = Piece<kType>(row, a.vocab, v + j);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (v + j < w1)
+        p[j].tokens(row, a.vocab, [&](int64_t i, float x) {
+          const uint32_t k = order_key(x);
+          if (kept(k, i)) here += wt.key_kept(k);
+        });
+  }
   const uint64_t run = block_exclusive(here, lds, in_slice);
   if (goal >= run && goal - run < here) {
     sh[0] = (uint64_t)w0;
@@ -712,12 +827,12 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   for (int64_t i0 = max(first, (int64_t)0); i0 < end; i0 += kThreads) {
     const int64_t i = i0 + tid;
     const uint32_t k = i < end ? order_key(load_logit<kType>(row, i)) : 0u;
-    const uint64_t w = i < end && kept(k, i) ? wt.kept_whole(k) : 0ull;
+    const uint64_t w = i < end && kept(k, i) ? wt.key_kept(k) : 0ull;
     uint64_t all;
     const uint64_t sum = block_exclusive(w, lds, all);
     if (goal >= sum && goal - sum < w) {
       a.token[r] = i;
-      if (a.prob) a.prob[r] = (float)(wt.scaled(k) / (double)total);
+      if (a.prob) a.prob[r] = (float)(wt.key_scaled(k) / (double)total);
     }
     if (goal < all) break;
     goal -= all;
@@ -734,9 +849,12 @@ inline int64_t max_vecs(int64_t vocab, int size) { return (vocab * size + 15) / 
 template <int kType>
 int launch_sample(const SampleArgs& a, int rows, hipStream_t s) {
   const dim3 slices((unsigned)rows * a.slices), each(rows), block(kThreads);
-  hipLaunchKernelGGL((sample_max_kernel<kType>), slices, block, 0, s, a);
+  if (a.per_64th == 0)
+    hipLaunchKernelGGL((sample_max_kernel<kType, true>), slices, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((sample_max_kernel<kType, false>), slices, block, 0, s, a);
   const bool count = a.top_k > 0 && a.top_k < a.vocab;
-  if (a.temperature == 0) {
+  if (a.per_64th == 0) {
     hipLaunchKernelGGL(sample_greedy_kernel, each, block, 0, s, a);
   } else if (count || a.top_p < 1) {
     if (count)
@@ -784,10 +902,26 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
   shift = min(shift, 51);
   const int64_t vecs = max_vecs(vocab, size);
   const int slices = slices_for(rows, vecs);
-  SampleArgs a{logits, vocab, row_stride * size, u, temperature, top_p, min_p, top_k, shift, slices,
-               (vecs + slices - 1) / slices, static_cast<char*>(workspace),
-               (int64_t)(sizeof(RowState) + (size_t)slices * kBins * sizeof(uint64_t)), token,
-               prob};
+  SampleArgs a{};
+  a.logits = logits;
+  a.vocab = vocab;
+  a.row_bytes = row_stride * size;
+  a.u = u;
+  a.top_p = top_p;
+  // (0: greedy; a temperature below 1e-30 counts as that)
+  a.per_64th = temperature > 0 ? 64 * 1.4426950408889634074 / fmax(temperature, 1e-30) : 0;
+  a.per_hi = (float)a.per_64th;
+  a.per_lo = (float)(a.per_64th - a.per_hi);
+  a.least = min_p * (double)(1ull << shift);
+  a.least_64ths = min_p > 0 ? -log2(min_p) * 64 : 0;
+  a.top_k = top_k;
+  a.shift = shift;
+  a.slices = slices;
+  a.slice_vecs = (vecs + slices - 1) / slices;
+  a.rows = static_cast<char*>(workspace);
+  a.row_ws = (int64_t)(sizeof(RowState) + (size_t)slices * kBins * sizeof(uint64_t));
+  a.token = token;
+  a.prob = prob;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == DIP_F32) return launch_sample<DIP_F32>(a, (int)rows, s);
   if (dtype == DIP_F16) return launch_sample<DIP_F16>(a, (int)rows, s);
