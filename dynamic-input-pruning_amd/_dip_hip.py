@@ -1148,12 +1148,13 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     if u.dtype is not torch.float32 or u.numel() != rows:
         raise RuntimeError(f"u must be a float32 tensor of {rows} values")
     u = u.contiguous()
-    token = torch.empty(rows, dtype=torch.int64, device=dev) if out is None else out
-    prob = torch.empty(rows, dtype=torch.float32, device=dev) if prob is None else prob
-    for name, t, dt in (("out", token, torch.int64), ("prob", prob, torch.float32)):
-        if t.dtype is not dt or t.numel() != rows or not t.is_contiguous() or t.device != dev:
+    for name, t, dt in (("out", out, torch.int64), ("prob", prob, torch.float32)):
+        if t is not None and (t.dtype is not dt or t.numel() != rows or not t.is_contiguous()
+                              or t.device != dev):
             raise RuntimeError(f"{name} must be a contiguous {dt} tensor of {rows} values on the "
                                "logits' device")
+    token = torch.empty(rows, dtype=torch.int64, device=dev) if out is None else out
+    prob = torch.empty(rows, dtype=torch.float32, device=dev) if prob is None else prob
     if rows == 0:
         return token, prob
     with _on(dev):

@@ -27,7 +27,7 @@
 //           it.  Rows whose list overflows (thousands of equal logits) are
 //           searched by the bits of the logit instead.
 // Without top-k and top-p there is no histogram; greedy draws need the first launch
-// and a choice among its results.
+// and a choice among its results.  Short rows go through all of it in one launch.
 #include "dip_common.h"
 #include "dip_internal.h"
 
@@ -37,7 +37,7 @@
 namespace dip {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;  // of a slice's workgroup, and what kN stands at below
 constexpr int kBins = 1024;
 constexpr int kListMax = 4096;
 constexpr int kRankMax = 512;  // longer lists are sorted, not ranked by comparing all pairs
@@ -150,37 +150,37 @@ struct Piece {
   }
 };
 
-// kAhead pieces of a thread, kThreads apart, loaded together: a row's pass is a
+// kAhead pieces of a thread, kN apart, loaded together: a row's pass is a
 // few waits for memory, not one per piece (250 rows of 32003, four pieces one after
 // the other: 15.6 us).
 constexpr int kAhead = 4;
 
-template <int kType>
+template <int kType, int kN = kThreads>
 struct Batch {
   Piece<kType> p[kAhead];
 
   DIP_DEV Batch(const char* row, int64_t vocab, int64_t v) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) p[j] = Piece<kType>(row, vocab, v + j * kThreads);
+    for (int j = 0; j < kAhead; ++j) p[j] = Piece<kType>(row, vocab, v + j * kN);
   }
 };
 
 // f(index, logit) of the tokens in the pieces [v0, v1) by the workgroup's threads,
 // `head` being this thread's first ones (loaded before what the caller waits for).
-template <int kType, typename F>
-DIP_DEV void each_token(Batch<kType> head, const char* row, int64_t vocab, int64_t v0,
+template <int kType, int kN = kThreads, typename F>
+DIP_DEV void each_token(Batch<kType, kN> head, const char* row, int64_t vocab, int64_t v0,
                         int64_t v1, F f) {
   for (int64_t v = v0 + threadIdx.x; v < v1;) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
-      if (v + j * kThreads < v1) head.p[j].tokens(row, vocab, f);
-    v += kAhead * kThreads;
-    if (v < v1) head = Batch<kType>(row, vocab, v);
+      if (v + j * kN < v1) head.p[j].tokens(row, vocab, f);
+    v += kAhead * kN;
+    if (v < v1) head = Batch<kType, kN>(row, vocab, v);
   }
 }
-template <int kType, typename F>
+template <int kType, int kN = kThreads, typename F>
 DIP_DEV void each_token(const char* row, int64_t vocab, int64_t v0, int64_t v1, F f) {
-  each_token<kType>(Batch<kType>(row, vocab, v0 + threadIdx.x), row, vocab, v0, v1, f);
+  each_token<kType, kN>(Batch<kType, kN>(row, vocab, v0 + threadIdx.x), row, vocab, v0, v1, f);
 }
 
 template <int kType>
@@ -213,6 +213,9 @@ __device__ const Roots kRoots = Roots();
 // 4e-10 of the weight, at random; a running sum over n tokens by 4e-10 / sqrt(n) of
 // itself.  (All in 64 bits, whose conversions run at a quarter of the rate: 250
 // rows of 32003 15.7 us in the launch that adds the weights up.)
+// kExact: the rounding of the difference counts (of bf16 and fp16 numbers it is
+// rounded only where the smaller is below 2^-13 of the larger).
+template <bool kExact>
 struct Weigher {
   float most, per_hi, per_lo;  // 64ths of an octave per logit, in two parts
   bool inf;                    // the largest is +inf, and only its equals count
@@ -236,9 +239,7 @@ struct Weigher {
   DIP_DEV float value(float x) const {
     return !inf ? x : x == INFINITY ? 0.f : -INFINITY;
   }
-  // w * 2^shift; 0 for -inf.  kExact: the difference's rounding counts (of bf16 and
-  // fp16 numbers it is rounded only where the smaller is below 2^-13 of the larger).
-  template <bool kExact>
+  // w * 2^shift; 0 for -inf.
   DIP_DEV double scaled(float x) const {
     const float hi = most - x, n = rintf(hi * per_hi);
     float low = hi * per_lo;
@@ -261,14 +262,12 @@ struct Weigher {
   DIP_DEV static unsigned long long whole(double w) {
     return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
   }
-  template <bool kExact>
   DIP_DEV unsigned long long whole_of(float x) const {
-    return whole(scaled<kExact>(x));
+    return whole(scaled(x));
   }
   // The weight if min-p keeps it, else 0.
-  template <bool kExact>
   DIP_DEV unsigned long long kept_whole(float x) const {
-    const double w = scaled<kExact>(x);
+    const double w = scaled(x);
     return w >= least ? whole(w) : 0ull;
   }
   // Never lower for a smaller logit.
@@ -276,7 +275,7 @@ struct Weigher {
     return (int)fminf((most - x) * bins_per_logit, (float)(kBins - 1));
   }
   // The same of logits as they are, given by their keys.
-  DIP_DEV double key_scaled(uint32_t k) const { return scaled<true>(value(key_value(k))); }
+  DIP_DEV double key_scaled(uint32_t k) const { return scaled(value(key_value(k))); }
   DIP_DEV unsigned long long key_whole(uint32_t k) const { return whole(key_scaled(k)); }
   DIP_DEV unsigned long long key_kept(uint32_t k) const {
     const double w = key_scaled(k);
@@ -289,7 +288,7 @@ struct Cut {  // the last kept token of the order
   int64_t index;
 };
 
-template <typename T, typename F>
+template <int kN = kThreads, typename T, typename F>
 DIP_DEV T block_reduce(T v, F f, T* lds) {
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) v = f(v, (T)__shfl_xor(v, m, 64));
@@ -298,11 +297,12 @@ DIP_DEV T block_reduce(T v, F f, T* lds) {
   __syncthreads();
   v = lds[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 64; ++i) v = f(v, lds[i]);
+  for (int i = 1; i < kN / 64; ++i) v = f(v, lds[i]);
   return v;
 }
 
 // The sum of the threads before this one; `total`: of all.
+template <int kN = kThreads>
 DIP_DEV uint64_t block_exclusive(uint64_t v, uint64_t* lds, uint64_t& total) {
   uint64_t run = v;
 #pragma unroll
@@ -316,14 +316,16 @@ DIP_DEV uint64_t block_exclusive(uint64_t v, uint64_t* lds, uint64_t& total) {
   uint64_t before = 0;
   total = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) {
+  for (int i = 0; i < kN / 64; ++i) {
     if (i == (int)(threadIdx.x >> 6)) before = total;
     total += lds[i];
   }
   return before + run - v;
 }
 
-constexpr int kLdsWords = 2 * (kThreads / 64) + 4;  // of the calls above and below
+template <int kN>
+constexpr int lds_words = 2 * (kN / 64) + 4;  // of the calls above and below
+constexpr int kLdsWords = lds_words<kThreads>;
 
 // The row's largest (order_key << 32 | ~index) and smallest logits, from the slices'.
 DIP_DEV void row_ends(const SampleArgs& a, const RowState& st, uint64_t* lds, uint64_t& best,
@@ -354,23 +356,24 @@ DIP_DEV void row_ends(const SampleArgs& a, const RowState& st, uint64_t* lds, ui
   least = l;
 }
 
-DIP_DEV Plan make_plan(const SampleArgs& a, const RowState& st, const Weigher& wt, Plan p,
-                       uint64_t* lds) {
-  constexpr int kPer = kBins / kThreads;
-  uint64_t* sh = lds + 2 * (kThreads / 64);
+template <int kN = kThreads, typename W>
+DIP_DEV Plan make_plan(const SampleArgs& a, const uint32_t* hn, const unsigned long long* hw,
+                       const W& wt, Plan p, uint64_t* lds) {
+  constexpr int kPer = kBins / kN;
+  uint64_t* sh = lds + 2 * (kN / 64);
   const int b0 = threadIdx.x * kPer;
+  const bool some_k = a.top_k > 0 && a.top_k < a.vocab;  // else nobody counted the tokens
   uint64_t n[kPer], w[kPer], sn = 0, sw = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    n[i] = st.hn[b0 + i];
-    w[i] = st.hw[b0 + i];
+    n[i] = some_k ? hn[b0 + i] : 0;
+    w[i] = hw[b0 + i];
     sn += n[i];
     sw += w[i];
   }
   uint64_t tokens = 0;
-  const bool some_k = a.top_k > 0 && a.top_k < a.vocab;  // else nobody counted the tokens
-  const uint64_t bn = some_k ? block_exclusive(sn, lds, tokens) : 0;
-  const uint64_t bw = block_exclusive(sw, lds, p.total);
+  const uint64_t bn = some_k ? block_exclusive<kN>(sn, lds, tokens) : 0;
+  const uint64_t bw = block_exclusive<kN>(sw, lds, p.total);
   // the first bin at which `test(tokens, weights up to and with it)` holds, and
   // what lies before it, in sh[0 .. 2]
   auto first = [&](auto test) {
@@ -494,10 +497,10 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
   row_ends(a, st, lds, best, least);
   const uint32_t top = (uint32_t)(best >> 32);
   if (top <= kKeyMinusInf) return;
-  const Weigher wt(a, top, least, roots);
+  const Weigher<kType == DIP_F32> wt(a, top, least, roots);
   __syncthreads();
   const auto add = [&](int64_t, float x) {
-    const unsigned long long w = wt.whole_of<kType == DIP_F32>(x);
+    const unsigned long long w = wt.whole_of(x);
     if (w == 0) return;
     const int b = wt.bin(x);
     if (kCount) atomicAdd(&hn[b], 1u);
@@ -537,23 +540,23 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
     if (s == 0 && threadIdx.x == 0) st.plan = p;
     return;
   }
-  const Weigher wt(a, top, least, roots);
+  const Weigher<kType == DIP_F32> wt(a, top, least, roots);
   __syncthreads();
   uint64_t sure = 0;
   if (kHist) {
-    p = make_plan(a, st, wt, p, lds);
+    p = make_plan(a, st.hn, st.hw, wt, p, lds);
     const unsigned long long* own = slice_hist(a, r, s);
     for (int b = threadIdx.x; b < p.lo; b += kThreads) sure += own[b];
     if (p.lo < kBins)
       each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) {
         const float y = wt.value(x);
         const int b = wt.bin(y);
-        if (b < p.lo || b > p.hi || wt.whole_of<kType == DIP_F32>(y) == 0) return;
+        if (b < p.lo || b > p.hi || wt.whole_of(y) == 0) return;
         const uint32_t at = atomicAdd(&st.listed, 1u);
         if (at < kListMax) st.list[at] = (uint64_t)order_key(x) << 32 | (uint32_t)~(uint32_t)i;
       });
   } else {
-    const auto add = [&](int64_t, float x) { sure += wt.kept_whole<kType == DIP_F32>(x); };
+    const auto add = [&](int64_t, float x) { sure += wt.kept_whole(x); };
     if (wt.inf)
       each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) { add(i, wt.value(x)); });
     else
@@ -581,20 +584,20 @@ __global__ __launch_bounds__(kThreads) void sample_greedy_kernel(SampleArgs a) {
 // weights reach `mass`, among those that `kept` keeps: the key from its highest
 // byte down, then the index among the tokens of that key.  A workgroup-wide call,
 // for rows that the list cannot hold.
-template <int kType, typename K>
-DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt, K kept,
+template <int kType, int kN = kThreads, typename W, typename K>
+DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const W& wt, K kept,
                         uint64_t count, double mass, uint32_t* hn, unsigned long long* hw,
                         uint64_t* lds) {
-  uint64_t* sh = lds + 2 * (kThreads / 64);
+  uint64_t* sh = lds + 2 * (kN / 64);
   const int tid = threadIdx.x;
   const bool by_mass = mass >= 0;
   const int64_t vecs = row_vecs<kType>(row, a.vocab);
   uint32_t prefix = 0;
   uint64_t above_n = 0, above_w = 0, ties = 0;
   for (int level = 24; level >= 0; level -= 8) {
-    for (int b = tid; b < kRadixBins; b += kThreads) hn[b] = 0, hw[b] = 0;
+    for (int b = tid; b < kRadixBins; b += kN) hn[b] = 0, hw[b] = 0;
     __syncthreads();
-    each_token<kType>(row, a.vocab, 0, vecs, [&](int64_t i, float x) {
+    each_token<kType, kN>(row, a.vocab, 0, vecs, [&](int64_t i, float x) {
       const uint32_t k = order_key(x);
       if (!kept(k, i) || (level < 24 && (k >> (level + 8)) != (prefix >> (level + 8)))) return;
       const unsigned long long w = wt.key_whole(k);
@@ -637,11 +640,11 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
     need = n < 1.0 ? 1 : (n < (double)ties ? (uint64_t)n : ties);
   }
   // the index of the need-th token of that key
-  const int64_t per = (a.vocab + kThreads - 1) / kThreads;
+  const int64_t per = (a.vocab + kN - 1) / kN;
   const int64_t lo = min(tid * per, a.vocab), end = min(lo + per, a.vocab);
   uint64_t mine = 0, all;
   for (int64_t i = lo; i < end; ++i) mine += order_key(load_logit<kType>(row, i)) == prefix;
-  const uint64_t before = block_exclusive(mine, lds, all);
+  const uint64_t before = block_exclusive<kN>(mine, lds, all);
   if (before < need && need <= before + mine) {
     uint64_t left = need - before;
     for (int64_t i = lo; i < end; ++i)
@@ -657,26 +660,27 @@ DIP_DEV Cut search_bits(const SampleArgs& a, const char* row, const Weigher& wt,
 }
 
 // v[0 .. n) in descending order (its values differ), `out` of as many words.
+template <int kN = kThreads>
 DIP_DEV void order_list(uint64_t* v, uint64_t* out, int n) {
   if (n <= kRankMax) {  // each one's place is the number of larger ones
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += kN) {
       const uint64_t x = v[i];
       int rank = 0;
       for (int j = 0; j < n; ++j) rank += v[j] > x;
       out[rank] = x;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) v[i] = out[i];
+    for (int i = threadIdx.x; i < n; i += kN) v[i] = out[i];
     __syncthreads();
     return;
   }
   int size = 2 * kRankMax;
   while (size < n) size *= 2;
-  for (int i = n + (int)threadIdx.x; i < size; i += kThreads) v[i] = 0;
+  for (int i = n + (int)threadIdx.x; i < size; i += kN) v[i] = 0;
   __syncthreads();
   for (int run = 2; run <= size; run *= 2)
     for (int step = run / 2; step > 0; step /= 2) {
-      for (int t = threadIdx.x; t < size / 2; t += kThreads) {
+      for (int t = threadIdx.x; t < size / 2; t += kN) {
         const int i = 2 * t - (t & (step - 1)), j = i + step;
         const bool down = (i & run) == 0;
         const uint64_t x = v[i], y = v[j];
@@ -687,6 +691,70 @@ DIP_DEV void order_list(uint64_t* v, uint64_t* out, int n) {
       }
       __syncthreads();
     }
+}
+
+// The last of the ordered list that top-k and top-p keep.
+template <int kN, typename W>
+DIP_DEV int last_kept(const SampleArgs& a, const Plan& p, const W& wt, const uint64_t* list,
+                      int n, uint64_t* lds) {
+  uint64_t* sh = lds + 2 * (kN / 64);
+  int last = n - 1;
+  if (!p.ranked) return last;
+  // a run of `per` neighbours per thread, and the weights before it
+  const int per = (n + kN - 1) / kN, i0 = min((int)threadIdx.x * per, n), i1 = min(i0 + per, n);
+  uint64_t mine = 0, all;
+  for (int i = i0; i < i1; ++i) mine += wt.key_whole((uint32_t)(list[i] >> 32));
+  const uint64_t before = p.above_w + block_exclusive<kN>(mine, lds, all);
+  if (p.by_k) last = (int)min((uint64_t)n, (uint64_t)a.top_k - p.above_n) - 1;
+  if (a.top_p < 1) {
+    if (threadIdx.x == 0) sh[1] = (uint64_t)last;
+    uint64_t run = before;
+    if (p.by_k) {  // the sum that top-p takes its share of
+      for (int i = i0; i < i1; ++i) {
+        run += wt.key_whole((uint32_t)(list[i] >> 32));
+        if (i == last) sh[0] = run;
+      }
+    } else if (threadIdx.x == 0) {
+      sh[0] = p.total;
+    }
+    __syncthreads();
+    const double mass = a.top_p * (double)sh[0];
+    run = before;
+    for (int i = i0; i < i1; ++i) {
+      const bool was = (double)run >= mass;
+      run += wt.key_whole((uint32_t)(list[i] >> 32));
+      if (i <= last && !was && (double)run >= mass) sh[1] = (uint64_t)i;
+    }
+    __syncthreads();
+    last = (int)sh[1];
+  }
+  return last;
+}
+
+// The border that the bits give, for a row whose list overflows.
+template <int kType, int kN = kThreads, typename W>
+DIP_DEV Cut search_row(const SampleArgs& a, const Plan& p, const char* row, const W& wt,
+                       uint32_t* hn, unsigned long long* hw, uint64_t* lds) {
+  Cut cut{0u, a.vocab};
+  auto kept = [&](uint32_t k, int64_t i) { return k > cut.key || (k == cut.key && i <= cut.index); };
+  if (p.by_k)
+    cut = search_bits<kType, kN>(a, row, wt, kept, (uint64_t)a.top_k, -1.0, hn, hw, lds);
+  if (a.top_p < 1) {
+    uint64_t w = 0;
+    each_token<kType, kN>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, float x) {
+      const uint32_t k = order_key(x);
+      if (kept(k, i)) w += wt.key_whole(k);
+    });
+    w = block_reduce<kN>(w, [](uint64_t x, uint64_t y) { return x + y; }, lds);
+    cut = search_bits<kType, kN>(a, row, wt, kept, 0, a.top_p * (double)w, hn, hw, lds);
+  }
+  return cut;
+}
+
+// u's place among `total`; u beyond 1 or NaN: the last.
+DIP_DEV uint64_t goal_of(double u, uint64_t total) {
+  const double t = u * (double)total;
+  return min(t < 0 ? 0 : t < (double)total ? (uint64_t)t : total - 1, total - 1);
 }
 
 template <int kType, bool kHist>
@@ -714,7 +782,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   if (kHist && n <= kListMax)
     for (int i = tid; i < n; i += kThreads) list[i] = st.list[i];
   const double u = a.u[r];
-  const Weigher wt(a, p.top, p.least, roots);
+  const Weigher<kType == DIP_F32> wt(a, p.top, p.least, roots);
   __syncthreads();
   constexpr int kSize = kType == DIP_F32 ? 4 : 2, kVec = 16 / kSize;
   const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15) / kSize;
@@ -722,17 +790,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   Cut cut{0u, a.vocab};
   auto kept = [&](uint32_t k, int64_t i) { return k > cut.key || (k == cut.key && i <= cut.index); };
   if (kHist && n > kListMax) {
-    if (p.by_k) cut = search_bits<kType>(a, row, wt, kept, (uint64_t)a.top_k, -1.0, hn, hw, lds);
-    if (a.top_p < 1) {
-      uint64_t w = 0;
-      each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab),
-                        [&](int64_t i, float x) {
-                          const uint32_t k = order_key(x);
-                          if (kept(k, i)) w += wt.key_whole(k);
-                        });
-      w = block_reduce(w, [](uint64_t x, uint64_t y) { return x + y; }, lds);
-      cut = search_bits<kType>(a, row, wt, kept, 0, a.top_p * (double)w, hn, hw, lds);
-    }
+    cut = search_row<kType>(a, p, row, wt, hn, hw, lds);
     if (tid < a.slices) sums[tid] = 0;
     __syncthreads();
     each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, float x) {
@@ -743,37 +801,8 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     });
   } else if (kHist && n > 0) {
     order_list(list, spare, n);
-    // a run of `per` neighbours per thread, and the weights before it
+    const int last = last_kept<kThreads>(a, p, wt, list, n, lds);
     const int per = (n + kThreads - 1) / kThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
-    int last = n - 1;  // of the list, kept by top-k and top-p
-    if (p.ranked) {
-      uint64_t mine = 0, all;
-      for (int i = i0; i < i1; ++i) mine += wt.key_whole((uint32_t)(list[i] >> 32));
-      const uint64_t before = p.above_w + block_exclusive(mine, lds, all);
-      if (p.by_k) last = (int)min((uint64_t)n, (uint64_t)a.top_k - p.above_n) - 1;
-      if (a.top_p < 1) {
-        if (tid == 0) sh[1] = (uint64_t)last;
-        uint64_t run = before;
-        if (p.by_k) {  // the sum that top-p takes its share of
-          for (int i = i0; i < i1; ++i) {
-            run += wt.key_whole((uint32_t)(list[i] >> 32));
-            if (i == last) sh[0] = run;
-          }
-        } else if (tid == 0) {
-          sh[0] = p.total;
-        }
-        __syncthreads();
-        const double mass = a.top_p * (double)sh[0];
-        run = before;
-        for (int i = i0; i < i1; ++i) {
-          const bool was = (double)run >= mass;
-          run += wt.key_whole((uint32_t)(list[i] >> 32));
-          if (i <= last && !was && (double)run >= mass) sh[1] = (uint64_t)i;
-        }
-        __syncthreads();
-        last = (int)sh[1];
-      }
-    }
     cut.key = (uint32_t)(list[last] >> 32);
     cut.index = (int64_t)(uint32_t)~(uint32_t)list[last];
     for (int i = i0; i < i1 && i <= last; ++i) {
@@ -786,10 +815,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   uint64_t total;
   const uint64_t mine = tid < a.slices ? sums[tid] : 0;
   const uint64_t before = block_exclusive(mine, lds, total);
-  // u beyond 1 or NaN: the last kept token
-  const double t = u * (double)total;
-  uint64_t goal = t < 0 ? 0 : t < (double)total ? (uint64_t)t : total - 1;
-  goal = min(goal, total - 1);
+  uint64_t goal = goal_of(u, total);
   if (goal >= before && goal - before < mine) {
     sh[0] = (uint64_t)tid;
     sh[1] = before;
@@ -839,6 +865,144 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   }
 }
 
+// The whole draw of a row of up to kRowPieces pieces per thread in one launch, a
+// workgroup per row, the row's pieces held in registers from the first pass to the
+// last: thread t has the neighbouring pieces from t * per on.
+constexpr int kRowPieces = 4;
+
+template <int kType, int kN, bool kHist>
+__global__ __launch_bounds__(kN) void sample_row_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[lds_words<kN>];
+  __shared__ double roots[64];
+  __shared__ uint64_t list[kHist ? kListMax : 1], spare[kHist ? kRankMax : 1];
+  __shared__ uint32_t hn[kHist ? kBins : 1], listed;
+  __shared__ unsigned long long hw[kHist ? kBins : 1];
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const char* row = row_of(a, r);
+  uint64_t* sh = lds + 2 * (kN / 64);
+  const int64_t vecs = row_vecs<kType>(row, a.vocab);
+  const int per = (int)((vecs + kN - 1) / kN);
+  Piece<kType> p[kRowPieces];
+#pragma unroll
+  for (int j = 0; j < kRowPieces; ++j) p[j] = Piece<kType>(row, a.vocab, (int64_t)tid * per + j);
+  const double u = a.u[r];
+  auto mine = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < kRowPieces; ++j)
+      if (j < per && (int64_t)tid * per + j < vecs) p[j].tokens(row, a.vocab, f);
+  };
+  if (kHist) {
+    for (int b = tid; b < kBins; b += kN) hn[b] = 0, hw[b] = 0;
+    if (tid == 0) listed = 0;
+  }
+
+  float most = -INFINITY, low = INFINITY;
+  int64_t at = 0;
+  mine([&](int64_t i, float x) {
+    at = x > most ? i : at;
+    most = fmaxf(most, x);
+    low = fminf(low, x == -INFINITY ? INFINITY : x);
+  });
+  uint64_t best = (uint64_t)order_key(most) << 32 | (uint32_t)~(uint32_t)at;
+  best = block_reduce<kN>(best, [](uint64_t x, uint64_t y) { return max(x, y); }, lds);
+  const uint32_t top = (uint32_t)(best >> 32);
+  if (top <= kKeyMinusInf || a.per_64th == 0) {  // nothing to choose from, or greedy
+    if (tid == 0) {
+      const bool some = top > kKeyMinusInf;
+      a.token[r] = some ? (int64_t)(uint32_t)~(uint32_t)best : 0;
+      if (a.prob) a.prob[r] = some ? 1.f : 0.f;
+    }
+    return;
+  }
+  const uint32_t least =
+      block_reduce<kN>(order_key(low), [](uint32_t x, uint32_t y) { return min(x, y); },
+                       reinterpret_cast<uint32_t*>(lds));
+  const Weigher<kType == DIP_F32> wt(a, top, least, roots);
+  __syncthreads();
+
+  Cut cut{0u, a.vocab};
+  Plan plan{top, least, kBins, kBins, 0, 0, 0, 0, 0};
+  if (kHist) {
+    mine([&](int64_t, float x) {
+      const float y = wt.value(x);
+      const unsigned long long w = wt.whole_of(y);
+      if (w == 0) return;
+      const int b = wt.bin(y);
+      atomicAdd(&hn[b], 1u);
+      atomicAdd(&hw[b], w);
+    });
+    __syncthreads();
+    plan = make_plan<kN>(a, hn, hw, wt, plan, lds);
+    if (plan.lo < kBins) {
+      mine([&](int64_t i, float x) {
+        const float y = wt.value(x);
+        const int b = wt.bin(y);
+        if (b < plan.lo || b > plan.hi || wt.whole_of(y) == 0) return;
+        const uint32_t to = atomicAdd(&listed, 1u);
+        if (to < kListMax) list[to] = (uint64_t)order_key(x) << 32 | (uint32_t)~(uint32_t)i;
+      });
+      __syncthreads();
+      const int n = (int)min(listed, (uint32_t)kListMax + 1);
+      if (n > kListMax) {
+        __syncthreads();
+        cut = search_row<kType, kN>(a, plan, row, wt, hn, hw, lds);
+      } else if (n > 0) {
+        order_list<kN>(list, spare, n);
+        const int last = last_kept<kN>(a, plan, wt, list, n, lds);
+        cut.key = (uint32_t)(list[last] >> 32);
+        cut.index = (int64_t)(uint32_t)~(uint32_t)list[last];
+      }
+    }
+  }
+
+  // running sums by index: threads, pieces and tokens come in it
+  auto weight = [&](int64_t i, float x) {
+    if (kHist) {
+      const uint32_t k = order_key(x);
+      if (!(k > cut.key || (k == cut.key && i <= cut.index))) return (uint64_t)0;
+    }
+    return (uint64_t)wt.kept_whole(wt.value(x));
+  };
+  uint64_t here = 0, total, in_run;
+  mine([&](int64_t i, float x) { here += weight(i, x); });
+  uint64_t run = block_exclusive<kN>(here, lds, total);
+  const uint64_t goal = goal_of(u, total);
+  if (goal >= run && goal - run < here) {
+    sh[0] = (uint64_t)tid;
+    sh[1] = goal - run;
+  }
+  __syncthreads();
+  // the run that the draw falls in, a token per thread
+  constexpr int kVec = Piece<kType>::kVec;
+  const int64_t first = (int64_t)sh[0] * per * kVec -
+                        (int)(reinterpret_cast<uintptr_t>(row) & 15) / Piece<kType>::kSize;
+  const int64_t i = first + tid;
+  const bool on = tid < per * kVec && i >= 0 && i < a.vocab;
+  const uint64_t left = sh[1];
+  const float x = on ? load_logit<kType>(row, i) : -INFINITY;
+  const uint64_t w = on ? weight(i, x) : 0;
+  const uint64_t before = block_exclusive<kN>(w, lds, in_run);
+  if (left >= before && left - before < w) {
+    a.token[r] = i;
+    if (a.prob) a.prob[r] = (float)(wt.scaled(wt.value(x)) / (double)total);
+  }
+}
+
+// Which rows are drawn in one launch: those of up to kOneLaunch pieces, and up to
+// the most that the launch takes where there are many rows or nothing to count (a
+// workgroup alone takes longer over a long row's histogram than slices do: one row
+// of 32003 bf16 logits, top-k 20, 32 us for 23; 250 such rows 35 for 51; without a
+// filter 17 for 17 and 18 for 28).  256 threads while they have two pieces each at
+// most, 1024 beyond (4000 bf16 logits 15 and 17 us, 8000 20 and 18).
+constexpr int64_t kSmallRow = 512;
+constexpr int64_t kOneLaunch = 2048;
+constexpr int64_t kMostPieces = 1024 * kRowPieces;
+constexpr int64_t kManyRows = 64;
+
+inline bool counts(const SampleArgs& a) {
+  return a.per_64th > 0 && ((a.top_k > 0 && a.top_k < a.vocab) || a.top_p < 1);
+}
+
 // Slices of a row: about a thousand workgroups in all, of 256 pieces at least.
 inline int slices_for(int64_t rows, int64_t vecs) {
   const int64_t want = max((int64_t)1, 1024 / rows), most = (vecs + 255) / 256;
@@ -846,8 +1010,20 @@ inline int slices_for(int64_t rows, int64_t vecs) {
 }
 inline int64_t max_vecs(int64_t vocab, int size) { return (vocab * size + 15) / 16 + 1; }
 
+template <int kType, int kN>
+int launch_row(const SampleArgs& a, int rows, hipStream_t s) {
+  if (counts(a))
+    hipLaunchKernelGGL((sample_row_kernel<kType, kN, true>), dim3(rows), dim3(kN), 0, s, a);
+  else
+    hipLaunchKernelGGL((sample_row_kernel<kType, kN, false>), dim3(rows), dim3(kN), 0, s, a);
+  return hip_status(hipGetLastError());
+}
+
 template <int kType>
-int launch_sample(const SampleArgs& a, int rows, hipStream_t s) {
+int launch_sample(const SampleArgs& a, int rows, int64_t vecs, hipStream_t s) {
+  if (vecs <= kSmallRow) return launch_row<kType, kThreads>(a, rows, s);
+  if (vecs <= kOneLaunch || (vecs <= kMostPieces && (rows >= kManyRows || !counts(a))))
+    return launch_row<kType, 1024>(a, rows, s);
   const dim3 slices((unsigned)rows * a.slices), each(rows), block(kThreads);
   if (a.per_64th == 0)
     hipLaunchKernelGGL((sample_max_kernel<kType, true>), slices, block, 0, s, a);
@@ -856,7 +1032,7 @@ int launch_sample(const SampleArgs& a, int rows, hipStream_t s) {
   const bool count = a.top_k > 0 && a.top_k < a.vocab;
   if (a.per_64th == 0) {
     hipLaunchKernelGGL(sample_greedy_kernel, each, block, 0, s, a);
-  } else if (count || a.top_p < 1) {
+  } else if (counts(a)) {
     if (count)
       hipLaunchKernelGGL((sample_hist_kernel<kType, true>), slices, block, 0, s, a);
     else
@@ -877,7 +1053,7 @@ using namespace dip;
 
 // For fp32 logits, which take the most slices.
 extern "C" size_t dip_sample_workspace_size(int64_t rows, int64_t vocab) {
-  if (rows <= 0 || vocab <= 0) return 0;
+  if (rows <= 0 || vocab <= 0 || max_vecs(vocab, 4) <= kOneLaunch) return 0;
   return (size_t)rows * (sizeof(RowState) +
                          (size_t)slices_for(rows, max_vecs(vocab, 4)) * kBins * sizeof(uint64_t));
 }
@@ -894,9 +1070,11 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
     return DIP_ERR_ARG;
   if (rows == 0) return DIP_OK;
   if (!logits || !u || !token) return DIP_ERR_NULL;
-  if (!workspace || ws_bytes < dip_sample_workspace_size(rows, vocab)) return DIP_ERR_WORKSPACE;
+  const size_t need = dip_sample_workspace_size(rows, vocab);
+  if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   const int size = dtype == DIP_F32 ? 4 : 2;
-  if (reinterpret_cast<uintptr_t>(logits) % size || !aligned16(workspace)) return DIP_ERR_ALIGN;
+  if (reinterpret_cast<uintptr_t>(logits) % size || (need && !aligned16(workspace)))
+    return DIP_ERR_ALIGN;
   int shift = 62;
   for (int64_t n = 1; n < vocab; n *= 2) --shift;
   shift = min(shift, 51);
@@ -923,7 +1101,7 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
   a.token = token;
   a.prob = prob;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == DIP_F32) return launch_sample<DIP_F32>(a, (int)rows, s);
-  if (dtype == DIP_F16) return launch_sample<DIP_F16>(a, (int)rows, s);
-  return launch_sample<DIP_BF16>(a, (int)rows, s);
+  if (dtype == DIP_F32) return launch_sample<DIP_F32>(a, (int)rows, vecs, s);
+  if (dtype == DIP_F16) return launch_sample<DIP_F16>(a, (int)rows, vecs, s);
+  return launch_sample<DIP_BF16>(a, (int)rows, vecs, s);
 }
