@@ -349,16 +349,31 @@ struct Plan {
   int64_t tiles, blocks;
   int splits;
   size_t work, bad, part;  // bytes
+  int64_t us100;           // about what the launches take, in hundredths of a microsecond
 };
 
-// As many workgroups as run at once, two per CU, a few steps each at least.
+// The splits of a tile's rows that take least, by estimates from measured times: 10
+// us, 0.12 ns per row and kv head to expand, and for a step of 64 rows 2.6 us where
+// a CU has one workgroup and 3 us where it has two; splits add 5 us and 0.21 ns for
+// each column's sums, which are written and read again.  (512 tokens of 64 / 8
+// heads: 2 splits 39 us, 1 split 23; 32 tokens behind 20010 rows: 32 splits 69 us, 16
+// splits 87.)
 Plan plan_for(int64_t tokens, int64_t start, int64_t nkv, int64_t group) {
   Plan p;
   p.tiles = (tokens * group + kTileCols - 1) / kTileCols;
-  p.blocks = (start + tokens + kTileRows - 1) / kTileRows * (kTileRows / kKvBlock);
-  const int64_t want = 2 * device_cus() / (p.tiles * nkv);
-  const int64_t most = (start + tokens + 4 * kTileRows - 1) / (4 * kTileRows);
-  p.splits = (int)max((int64_t)1, min(min(want, most), (int64_t)64));
+  p.blocks = (start + tokens + kTileRows - 1) / kTileRows * kStepBlocks;
+  const int64_t steps = (start + tokens + kTileRows - 1) / kTileRows, cus = device_cus();
+  p.us100 = INT64_MAX;
+  for (int64_t s = 1; s <= min((steps + 3) / 4, (int64_t)64); s = s < 8 ? s + 1 : s + s / 8) {
+    const int64_t wgs = p.tiles * nkv * s, per = (steps + s - 1) / s;
+    const int64_t us = 1000 + (start + tokens) * nkv * 12 / 1000 +
+                       per * (wgs <= cus ? 260 : 300 * ((wgs + 2 * cus - 1) / (2 * cus))) +
+                       (s == 1 ? 0 : 500 + tokens * group * nkv * s * 21 / 1000);
+    if (us < p.us100) {
+      p.us100 = us;
+      p.splits = (int)s;
+    }
+  }
   p.work = (size_t)nkv * p.blocks * kBlockVecs * 16;
   p.bad = ((size_t)nkv * p.blocks * 4 + 15) / 16 * 16;
   p.part = p.splits == 1 ? 0
@@ -373,16 +388,8 @@ size_t prompt_tiles_workspace(int64_t tokens, int64_t start, int64_t nkv, int64_
   return p.work + p.bad + p.part;
 }
 
-// About what the launches take, in hundredths of a microsecond, from measured
-// times: 10 us, 0.12 ns per row and kv head to expand, 3 us per step of a workgroup
-// with two of them on a CU, 5 us to add up splits (256 columns of 8 kv heads over
-// 20000 rows: 68 us, by this 64; 512 over 3000: 34, 33; 16 over 60000: 116, 118).
 int64_t prompt_tiles_us100(int64_t tokens, int64_t start, int64_t nkv, int64_t group) {
-  const Plan p = plan_for(tokens, start, nkv, group);
-  const int64_t slots = 2 * device_cus(), steps = (start + tokens + 63) / 64;
-  const int64_t rounds = (p.tiles * nkv * p.splits + slots - 1) / slots;
-  return 1000 + (start + tokens) * nkv * 12 / 1000 +
-         rounds * ((steps + p.splits - 1) / p.splits) * 300 + (p.splits > 1 ? 500 : 0);
+  return plan_for(tokens, start, nkv, group).us100;
 }
 
 int launch_prompt_tiles(Kv4AttnArgs a, void* workspace, hipStream_t stream) {
