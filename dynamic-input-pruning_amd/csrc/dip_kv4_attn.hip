@@ -23,6 +23,10 @@ DIP_DEV int blocks_per_wave(int rows, int waves) {
   return max(1, (blocks + waves - 1) / waves);
 }
 
+// How far (in powers of 2) a score may pass the maximum that the sums are taken
+// against before they are taken against a new one.
+constexpr float kSlack = 8.f;
+
 DIP_DEV float scale_lo(uint32_t w) { return __uint_as_float(w << 16); }
 DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
       }
     }
     mx = fmaxf(m, row_pair_max32(row_pair_max16(mx)));
-    if (__any(mx > m)) {
+    if (__any(mx > m + kSlack)) {
       const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);  // what the sums so far are worth
       den *= f;
 #pragma unroll
@@ -324,10 +328,10 @@ __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4A
 // How a launch cuts its tiles' rows.  Alone, a workgroup of 8 waves takes a tile's
 // and writes the result itself; otherwise twice `pairs` workgroups of 4 waves (two
 // to a CU) do, whose sums a second launch adds up.  `us` is about what it takes,
-// from measured times: 3 us, 5 us and 1.35 us per block of a wave for each round of
+// from measured times: 3 us, 5 us and 1.6 us per block of a wave for each round of
 // the workgroups, 6.5 us for the second launch (64 columns of 8 kv heads over 20000
-// rows: 26 us, by this 28; 512 columns over 8000 rows: 51, 51; 1024 over 1000: 26,
-// 26; 8 over 1000 in one launch 11, in two 13).  (Split tiles with 8 waves: 20011 rows of 64 / 8 heads 15.2 us for 11.6.)
+// rows: 26 us, by this 30; 512 columns over 8000 rows: 51, 59; 1024 over 1000: 26,
+// 29; 8 over 1000 in one launch 11, in two 13).  (Split tiles with 8 waves: 20011 rows of 64 / 8 heads 15.2 us for 11.6.)
 struct Cut {
   int pairs;
   int64_t us100;
@@ -342,7 +346,7 @@ inline Cut cut_for(int64_t tiles, int64_t nkv, int64_t max_rows) {
   for (int64_t s = 1; s <= most; s = s < 8 ? s + 1 : s + s / 8) {
     const int64_t rounds = (tiles * nkv * s + cus - 1) / cus;
     const int64_t per = (blocks + 8 * s - 1) / (8 * s);
-    const int64_t us = 300 + rounds * (500 + 135 * per) + (s > 1 ? 650 : 0);
+    const int64_t us = 300 + rounds * (500 + 160 * per) + (s > 1 ? 650 : 0);
     if (us < best.us100) best = Cut{(int)s, us};
   }
   return best;

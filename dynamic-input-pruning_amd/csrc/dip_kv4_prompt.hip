@@ -96,6 +96,12 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
   }
 }
 
+// How far (in powers of 2) a score may pass the maximum that the sums are taken
+// against before they are taken against a new one: with 32 columns to a wave some
+// column has a new maximum in most steps, and the sums' 64 products are a quarter of
+// a step's instructions (4096 tokens of 64 / 8 heads 350 us for 316).
+constexpr float kSlack = 8.f;
+
 // The steps of 64 rows that a split takes of a tile's.
 DIP_DEV int steps_per_split(int rows, int splits) {
   const int steps = (rows + kTileRows - 1) / kTileRows;
@@ -196,6 +202,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
     // does not attend
     const int behind = t * kTileRows + 4 * h - limit;
     if (masked) {
+      asm volatile("");  // a branch: 64 comparisons and selections that most steps skip
 #pragma unroll
       for (int b = 0; b < kStepBlocks; ++b)
 #pragma unroll
@@ -208,7 +215,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
     mx = fmaxf(m, row_pair_max32(mx) * c2);
-    if (__any(mx > m)) {
+    if (__any(mx > m + kSlack)) {
       const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);
       den *= f;
 #pragma unroll
@@ -223,6 +230,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = fast_exp2(fmaf(s[b][r], c2, -base));
     if (masked) {  // weights of 0, whatever a base of +inf or NaN made of them
+      asm volatile("");
 #pragma unroll
       for (int b = 0; b < kStepBlocks; ++b)
 #pragma unroll
@@ -354,7 +362,7 @@ struct Plan {
 
 // The splits of a tile's rows that take least, by estimates from measured times: 10
 // us, 0.12 ns per row and kv head to expand, and for a step of 64 rows 2.6 us where
-// a CU has one workgroup and 3 us where it has two; splits add 5 us and 0.21 ns for
+// a CU has one workgroup and 3 us where it has two; splits add 7 us and 0.12 ns for
 // each column's sums, which are written and read again.  (512 tokens of 64 / 8
 // heads: 2 splits 39 us, 1 split 23; 32 tokens behind 20010 rows: 32 splits 69 us, 16
 // splits 87.)
@@ -368,7 +376,7 @@ Plan plan_for(int64_t tokens, int64_t start, int64_t nkv, int64_t group) {
     const int64_t wgs = p.tiles * nkv * s, per = (steps + s - 1) / s;
     const int64_t us = 1000 + (start + tokens) * nkv * 12 / 1000 +
                        per * (wgs <= cus ? 260 : 300 * ((wgs + 2 * cus - 1) / (2 * cus))) +
-                       (s == 1 ? 0 : 500 + tokens * group * nkv * s * 21 / 1000);
+                       (s == 1 ? 0 : 700 + tokens * group * nkv * s * 12 / 1000);
     if (us < p.us100) {
       p.us100 = us;
       p.splits = (int)s;
