@@ -38,6 +38,7 @@ namespace dip {
 namespace {
 
 constexpr int kThreads = 256;  // of a slice's workgroup, and what kN stands at below
+constexpr int kDrawThreads = 512;  // (64 rows of 151936 fp32 logits: 256 13.8 us, 512 10.0, 1024 11.0)
 constexpr int kBins = 1024;
 constexpr int kListMax = 4096;
 constexpr int kRankMax = 512;  // longer lists are sorted, not ranked by comparing all pairs
@@ -530,7 +531,10 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
   RowState& st = row_state(a, r);
   const int64_t v0 = s * a.slice_vecs;
   const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
-  const Batch<kType> head(row, a.vocab, v0 + threadIdx.x);
+  // a short slice's tokens are fetched at once; a long one's only if some of them lie
+  // in the bins to list, which its own histogram tells
+  const bool early = !kHist || a.slice_vecs <= kAhead * kThreads;
+  Batch<kType> head(row, a.vocab, early ? v0 + threadIdx.x : INT32_MAX);
   uint64_t best;
   uint32_t least;
   row_ends(a, st, lds, best, least);
@@ -546,8 +550,15 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
   if (kHist) {
     p = make_plan(a, st.hn, st.hw, wt, p, lds);
     const unsigned long long* own = slice_hist(a, r, s);
-    for (int b = threadIdx.x; b < p.lo; b += kThreads) sure += own[b];
-    if (p.lo < kBins)
+    int some = 0;
+    for (int b = threadIdx.x; b <= min(p.hi, kBins - 1); b += kThreads) {
+      if (b < p.lo)
+        sure += own[b];
+      else
+        some |= own[b] != 0;
+    }
+    if (p.lo < kBins && __syncthreads_or(some)) {
+      if (!early) head = Batch<kType>(row, a.vocab, v0 + threadIdx.x);
       each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) {
         const float y = wt.value(x);
         const int b = wt.bin(y);
@@ -555,6 +566,7 @@ __global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
         const uint32_t at = atomicAdd(&st.listed, 1u);
         if (at < kListMax) st.list[at] = (uint64_t)order_key(x) << 32 | (uint32_t)~(uint32_t)i;
       });
+    }
   } else {
     const auto add = [&](int64_t, float x) { sure += wt.kept_whole(x); };
     if (wt.inf)
@@ -758,8 +770,8 @@ DIP_DEV uint64_t goal_of(double u, uint64_t total) {
 }
 
 template <int kType, bool kHist>
-__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
-  __shared__ uint64_t lds[kLdsWords];
+__global__ __launch_bounds__(kDrawThreads) void sample_draw_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[lds_words<kDrawThreads>];
   __shared__ double roots[64];
   __shared__ uint64_t list[kHist ? kListMax : 1], spare[kHist ? kRankMax : 1];
   __shared__ unsigned long long sums[kMaxSlices];
@@ -768,7 +780,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   const int r = blockIdx.x, tid = threadIdx.x;
   const char* row = row_of(a, r);
   const RowState& st = row_state(a, r);
-  uint64_t* sh = lds + 2 * (kThreads / 64);
+  uint64_t* sh = lds + 2 * (kDrawThreads / 64);
   const Plan p = st.plan;
   if (p.top <= kKeyMinusInf) {  // nothing to choose from
     if (tid == 0) {
@@ -780,7 +792,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   const int n = kHist && p.lo < kBins ? (int)min(st.listed, (uint32_t)kListMax + 1) : 0;
   if (tid < a.slices) sums[tid] = st.sure[tid];
   if (kHist && n <= kListMax)
-    for (int i = tid; i < n; i += kThreads) list[i] = st.list[i];
+    for (int i = tid; i < n; i += kDrawThreads) list[i] = st.list[i];
   const double u = a.u[r];
   const Weigher<kType == DIP_F32> wt(a, p.top, p.least, roots);
   __syncthreads();
@@ -790,19 +802,19 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   Cut cut{0u, a.vocab};
   auto kept = [&](uint32_t k, int64_t i) { return k > cut.key || (k == cut.key && i <= cut.index); };
   if (kHist && n > kListMax) {
-    cut = search_row<kType>(a, p, row, wt, hn, hw, lds);
+    cut = search_row<kType, kDrawThreads>(a, p, row, wt, hn, hw, lds);
     if (tid < a.slices) sums[tid] = 0;
     __syncthreads();
-    each_token<kType>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, float x) {
+    each_token<kType, kDrawThreads>(row, a.vocab, 0, row_vecs<kType>(row, a.vocab), [&](int64_t i, float x) {
       const uint32_t k = order_key(x);
       if (!kept(k, i)) return;
       const unsigned long long w = wt.key_kept(k);
       if (w) atomicAdd(&sums[slice_of(i)], w);
     });
   } else if (kHist && n > 0) {
-    order_list(list, spare, n);
-    const int last = last_kept<kThreads>(a, p, wt, list, n, lds);
-    const int per = (n + kThreads - 1) / kThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
+    order_list<kDrawThreads>(list, spare, n);
+    const int last = last_kept<kDrawThreads>(a, p, wt, list, n, lds);
+    const int per = (n + kDrawThreads - 1) / kDrawThreads, i0 = min(tid * per, n), i1 = min(i0 + per, n);
     cut.key = (uint32_t)(list[last] >> 32);
     cut.index = (int64_t)(uint32_t)~(uint32_t)list[last];
     for (int i = i0; i < i1 && i <= last; ++i) {
@@ -814,7 +826,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   // the slice, then the token in it: running sums by index
   uint64_t total;
   const uint64_t mine = tid < a.slices ? sums[tid] : 0;
-  const uint64_t before = block_exclusive(mine, lds, total);
+  const uint64_t before = block_exclusive<kDrawThreads>(mine, lds, total);
   uint64_t goal = goal_of(u, total);
   if (goal >= before && goal - before < mine) {
     sh[0] = (uint64_t)tid;
@@ -826,7 +838,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   goal -= sh[1];  // within the slice
   // a run of neighbouring pieces per thread; then the run that the draw falls in,
   // a token per thread
-  const int64_t per = (v1 - v0 + kThreads - 1) / kThreads;
+  const int64_t per = (v1 - v0 + kDrawThreads - 1) / kDrawThreads;
   const int64_t w0 = min(v0 + tid * per, v1), w1 = min(w0 + per, v1);
   uint64_t here = 0, in_slice;
   for (int64_t v = w0; v < w1; v += kAhead) {
@@ -841,7 +853,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
           if (kept(k, i)) here += wt.key_kept(k);
         });
   }
-  const uint64_t run = block_exclusive(here, lds, in_slice);
+  const uint64_t run = block_exclusive<kDrawThreads>(here, lds, in_slice);
   if (goal >= run && goal - run < here) {
     sh[0] = (uint64_t)w0;
     sh[1] = goal - run;
@@ -850,12 +862,12 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
   const int64_t first = (int64_t)sh[0] * kVec - off;
   const int64_t end = min(first + per * kVec, a.vocab);
   goal = sh[1];
-  for (int64_t i0 = max(first, (int64_t)0); i0 < end; i0 += kThreads) {
+  for (int64_t i0 = max(first, (int64_t)0); i0 < end; i0 += kDrawThreads) {
     const int64_t i = i0 + tid;
     const uint32_t k = i < end ? order_key(load_logit<kType>(row, i)) : 0u;
     const uint64_t w = i < end && kept(k, i) ? wt.key_kept(k) : 0ull;
     uint64_t all;
-    const uint64_t sum = block_exclusive(w, lds, all);
+    const uint64_t sum = block_exclusive<kDrawThreads>(w, lds, all);
     if (goal >= sum && goal - sum < w) {
       a.token[r] = i;
       if (a.prob) a.prob[r] = (float)(wt.key_scaled(k) / (double)total);
@@ -1024,7 +1036,7 @@ int launch_sample(const SampleArgs& a, int rows, int64_t vecs, hipStream_t s) {
   if (vecs <= kSmallRow) return launch_row<kType, kThreads>(a, rows, s);
   if (vecs <= kOneLaunch || (vecs <= kMostPieces && (rows >= kManyRows || !counts(a))))
     return launch_row<kType, 1024>(a, rows, s);
-  const dim3 slices((unsigned)rows * a.slices), each(rows), block(kThreads);
+  const dim3 slices((unsigned)rows * a.slices), each(rows), block(kThreads), draw(kDrawThreads);
   if (a.per_64th == 0)
     hipLaunchKernelGGL((sample_max_kernel<kType, true>), slices, block, 0, s, a);
   else
@@ -1038,10 +1050,10 @@ int launch_sample(const SampleArgs& a, int rows, int64_t vecs, hipStream_t s) {
     else
       hipLaunchKernelGGL((sample_hist_kernel<kType, false>), slices, block, 0, s, a);
     hipLaunchKernelGGL((sample_gather_kernel<kType, true>), slices, block, 0, s, a);
-    hipLaunchKernelGGL((sample_draw_kernel<kType, true>), each, block, 0, s, a);
+    hipLaunchKernelGGL((sample_draw_kernel<kType, true>), each, draw, 0, s, a);
   } else {
     hipLaunchKernelGGL((sample_gather_kernel<kType, false>), slices, block, 0, s, a);
-    hipLaunchKernelGGL((sample_draw_kernel<kType, false>), each, block, 0, s, a);
+    hipLaunchKernelGGL((sample_draw_kernel<kType, false>), each, draw, 0, s, a);
   }
   return hip_status(hipGetLastError());
 }
