@@ -1060,7 +1060,9 @@ def kv4_decode_attention_workspace_bytes(n_heads: int, n_kv_heads: int, max_len:
 
 def kv4_decode_attention(q, cache: KV4Cache, pos, out, scale: float, ws=None):
     """Grouped-query attention of one token (q, n_heads * 128 values) over rows
-    0 .. pos of one layer's 4-bit cache -> out (new if None)."""
+    0 .. pos of one layer's 4-bit cache -> out (new if None).  ws: a workspace of
+    kv4_decode_attention_workspace_bytes, one for each call that may run at once
+    (None: the call's own)."""
     dev, nkv, max_len, n = _kv4(cache, q), cache.n_kv_heads, cache.max_len, q.numel()
     nh = n // 128
     if n != nh * 128 or nh < 1 or nh % nkv:
@@ -1086,7 +1088,8 @@ def kv4_decode_attention(q, cache: KV4Cache, pos, out, scale: float, ws=None):
 def kv4_prompt_attention(q, cache: KV4Cache, start: int, out, scale: float, ws=None):
     """Grouped-query attention of a prompt's tokens (q [tokens, n_heads * 128] at
     positions start ..), token t over rows 0 .. start + t of one layer's 4-bit
-    cache -> out (new if None)."""
+    cache -> out (new if None).  ws: as in kv4_decode_attention; its size depends on
+    start and the number of tokens."""
     dev, nkv, max_len, n = _kv4(cache, q), cache.n_kv_heads, cache.max_len, q.numel()
     if q.dim() != 2 or q.shape[1] % (128 * nkv) or not q.shape[1]:
         raise RuntimeError(f"q must be [tokens, a multiple of {nkv} heads of 128 values]")
@@ -1136,7 +1139,10 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
     the fewest whose weights reach top_p of their sum, of those the ones with at
     least min_p of the largest weight.  The token is where the running sum of the
     kept weights, by index, exceeds u times their sum.  temperature 0 is greedy.
-    NaN counts as -inf; a row of nothing else gives token 0, probability 0."""
+    NaN counts as -inf; a row of nothing else gives token 0, probability 0.
+
+    out, prob and ws (uint8) may be given; calls that may run at once, or graphs
+    that do, need a ws each, as they have if it is None."""
     check_sampling(temperature, top_k, top_p, min_p)
     dev = _dev(logits, u)
     kind = _LOGIT_TYPES.get(logits.dtype)

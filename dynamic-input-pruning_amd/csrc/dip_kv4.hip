@@ -60,9 +60,11 @@ struct Kv4WriteArgs {
 // A values' task: lane l holds dimensions 2 l and 2 l + 1 of each row, a scale
 // group is 16 lanes.  A heads' task: 16 lanes per head, lane i the dimensions
 // 8 i .. 8 i + 7 (one 16-byte load), which are one word of a key; a scale group is
-// four lanes, and rotate_half's partner dimension is in lane i ^ 8.  (A wave per
-// head, two dimensions per lane and the sum by lane shuffles: 4099 tokens of
-// 64 / 8 heads 133 us.)
+// four lanes, and rotate_half's partner dimension is in lane i ^ 8.
+//
+// Memory bounds a prompt's: 4099 tokens of 64 / 8 heads move 158 MB in 41 us, 3.9
+// TB/s.  (A wave per head, two dimensions per lane and the sum by lane shuffles:
+// 133 us.)  One token's 3.2 us are the launch and three waits for memory.
 //
 // The norm's mean and root are taken in 64 bits, and x * r is the 64-bit
 // product's fp32 rounding (r in two parts): a key next to a border between two of
@@ -189,7 +191,8 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
 }
 
 // Rows start .. start + rows - 1 as bf16 [rows, nkv, 128]: a wave per (block,
-// lane quarter, kv head), 8 rows each, as the values are written.
+// lane quarter, kv head), 8 rows each, as the values are written.  (4099 rows of 8
+// heads, 4.7 MB read and 16.8 written: 8.4 us.)
 __global__ __launch_bounds__(64 * kWriteWaves) void kv4_read_kernel(
     const uint32_t* __restrict__ kc, const uint32_t* __restrict__ vc,
     const uint16_t* __restrict__ sc, uint32_t* __restrict__ k_out, uint32_t* __restrict__ v_out,

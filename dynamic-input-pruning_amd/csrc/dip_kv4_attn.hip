@@ -46,6 +46,11 @@ DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 //     bf16 is off by 2^-9 of itself, as any bf16 weight is.)
 // Rows past a column's last get weight and scale 0, so what they hold, NaN
 // scales too, does not count.
+// A long cache is bound by memory: 131071 rows of 8 kv heads, 151 MB, 33 us (4.6
+// TB/s, 93 % of a copy's rate).  Shorter ones by what comes before and after their
+// few blocks of a wave: 20011 rows, 23 MB, 11 us; 701 rows in one launch, 16 blocks
+// of rows to 8 waves, 9 us.  (With the MFMAs' sums in the accumulator half of the
+// registers and every block masked 45 us at 131071 rows.)
 template <int W>
 __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
   __shared__ float wm[W][kCols], wl[W][kCols];
@@ -265,7 +270,8 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
 // The splits of one column added up, in a fixed order: one workgroup per (kv
 // head, column), kCombine groups of 128 threads, each of which takes every
 // kCombine-th split's value sums; its first loads are in flight while the splits'
-// weights are worked out.
+// weights are worked out.  (20011 rows, 64 columns: 4 us; one group of 128 threads
+// over all splits in turn 18 to 22.)
 constexpr int kCombine = 8, kAhead = 8;
 
 __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4AttnArgs a,
@@ -331,7 +337,8 @@ __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4A
 // from measured times: 3 us, 5 us and 1.6 us per block of a wave for each round of
 // the workgroups, 6.5 us for the second launch (64 columns of 8 kv heads over 20000
 // rows: 26 us, by this 30; 512 columns over 8000 rows: 51, 59; 1024 over 1000: 26,
-// 29; 8 over 1000 in one launch 11, in two 13).  (Split tiles with 8 waves: 20011 rows of 64 / 8 heads 15.2 us for 11.6.)
+// 29; 8 over 1000 in one launch 11, in two 13).  (Split tiles with 8 waves: 20011
+// rows of 64 / 8 heads 15.2 us for 11.6.)
 struct Cut {
   int pairs;
   int64_t us100;
@@ -394,8 +401,8 @@ using namespace dip;
 
 extern "C" size_t dip_kv4_decode_attention_workspace_size(int64_t n_heads, int64_t n_kv_heads,
                                                           int64_t head_dim, int64_t max_len) {
-  if (head_dim != kKvHeadDim || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
-      max_len <= 0)
+  if (head_dim != kKvHeadDim || n_heads <= 0 || n_heads > 4096 || n_kv_heads <= 0 ||
+      n_heads % n_kv_heads != 0 || max_len <= 0 || max_len > (1 << 30))
     return 0;
   const int64_t tiles = col_tiles(1, n_heads / n_kv_heads);
   return part_bytes(tiles, n_kv_heads, cut_for(tiles, n_kv_heads, max_len).splits());
@@ -437,8 +444,8 @@ inline bool by_tiles(int64_t tokens, int64_t start, int64_t nkv, int64_t group) 
 extern "C" size_t dip_kv4_prompt_attention_workspace_size(int64_t tokens, int64_t start,
                                                           int64_t n_heads, int64_t n_kv_heads,
                                                           int64_t head_dim) {
-  if (head_dim != kKvHeadDim || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 ||
-      tokens <= 0 || start < 0 || start > (1 << 30) || tokens > (1 << 30))
+  if (head_dim != kKvHeadDim || n_heads <= 0 || n_heads > 4096 || n_kv_heads <= 0 ||
+      n_heads % n_kv_heads != 0 || tokens <= 0 || start < 0 || start > (1 << 30) || tokens > (1 << 30))
     return 0;
   const int64_t group = n_heads / n_kv_heads;
   if (by_tiles(tokens, start, n_kv_heads, group))

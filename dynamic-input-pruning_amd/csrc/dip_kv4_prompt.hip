@@ -4,8 +4,9 @@
 // columns.
 //
 // Every tile of columns reads every earlier row, so unpacking in the tiles would
-// be done tokens * group / 128 times; once costs 16 bytes of memory traffic per 9
-// of cache, a few per cent of the products' time from some hundred columns on.
+// be done tokens * group / 128 times; once costs two passes over 512 bytes per row
+// and kv head, a few per cent of the products' time from some hundred columns on
+// (4096 rows of 8 heads 8 us).
 #include "dip_kv4.h"
 
 namespace dip {
@@ -41,9 +42,8 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
     return;
   }
   const size_t row0 = (size_t)kvh * max_len + b * kKvBlock;
-  if (tid < 128) {
+  if (tid < 128)
     scales[tid >> 2][tid & 3] = reinterpret_cast<const uint32_t*>(sc + row0 * kKvScaleVals)[tid];
-  }
   __syncthreads();
   auto scale = [&](int row, int g) {  // g 0 .. 3 keys, 4 .. 7 values
     const uint32_t w = scales[row][g >> 1];
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
 // How far (in powers of 2) a score may pass the maximum that the sums are taken
 // against before they are taken against a new one: with 32 columns to a wave some
 // column has a new maximum in most steps, and the sums' 64 products are a quarter of
-// a step's instructions (4096 tokens of 64 / 8 heads 350 us for 316).
+// a step's instructions (4096 tokens of 64 / 8 heads 350 us for 343).
 constexpr float kSlack = 8.f;
 
 // The steps of 64 rows that a split takes of a tile's.
@@ -124,11 +124,16 @@ typedef const __attribute__((address_space(1))) void global_void;
 //   softmax in fp32 with a running maximum (lanes l and l ^ 32 share a column);
 //   out^T += V^T P^T, the weights rounded to bf16 in place: they are the operand
 //     as they lie.  (Off by 2^-8 of itself at most, as any bf16 weight is.)
+// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 300 to 335 us, 0.82
+// to 0.92 PFLOP/s, where a large product of matrices reaches 1.15 to 1.37.  The MFMAs
+// are busy 49 % of the time and the VALU, the softmax mostly, 56 %; without the fetch
+// it took 240 us, without the exponentials 336, without the second product 290 (of
+// 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
+// buffers 353; rows through registers into LDS 493; 32 rows to a step and three
+// workgroups to a CU 340 to 346.)
 template <bool kSplit>
-__global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(Kv4AttnArgs a,
-                                                                        const uint4* work,
-                                                                        const uint32_t* bad,
-                                                                        int blocks, int tiles) {
+__global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
+    Kv4AttnArgs a, const uint4* work, const uint32_t* bad, int blocks, int tiles) {
   __shared__ uint4 buf_a[kStepBlocks * kBlockVecs], buf_b[kStepBlocks * kBlockVecs];
   __shared__ int bad_row[kKvGroups];
   const int kvh = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv;
@@ -156,7 +161,8 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       uint4 w = qp[2 * k + h];
-      if (a.scale < 0.f) w.x ^= 0x80008000u, w.y ^= 0x80008000u, w.z ^= 0x80008000u, w.w ^= 0x80008000u;
+      const uint32_t sign = a.scale < 0.f ? 0x80008000u : 0u;
+      w.x ^= sign, w.y ^= sign, w.z ^= sign, w.w ^= sign;
       bq[k] = __builtin_bit_cast(bf16x8_t, u32x4_t{w.x, w.y, w.z, w.w});
     }
   }
@@ -168,8 +174,8 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
     for (int i = 0; i < kStepBlocks * kBlockVecs / 256; ++i) {
       const int at = i * 256 + wave * 64;
       __builtin_amdgcn_global_load_lds(
-          (global_void*)(src + (size_t)t * kStepBlocks * kBlockVecs + at + l), (lds_void*)(buf + at), 16, 0,
-          0);
+          (global_void*)(src + (size_t)t * kStepBlocks * kBlockVecs + at + l),
+          (lds_void*)(buf + at), 16, 0, 0);
     }
   };
 

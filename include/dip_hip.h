@@ -675,7 +675,7 @@ int dip_qk_norm_rope_kv4_rows(const uint16_t* qkv, const uint16_t* q_norm_w,
  * out [tokens, n_heads, head_dim].
  * Products of bf16 numbers summed in fp32, softmax and its sums in fp32, the
  * weights (times the values' scales) rounded to bf16, bf16 results.  The
- * workspaces need no clearing.
+ * workspaces need no clearing; calls that may run at once need one each.
  */
 size_t dip_kv4_decode_attention_workspace_size(int64_t n_heads, int64_t n_kv_heads,
                                                int64_t head_dim, int64_t max_len);
@@ -702,10 +702,15 @@ int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache, const int
  * the first by index at which the running sum of the kept weights exceeds u
  * times their sum (the last kept one for u beyond 1 or NaN).  temperature 0: the
  * largest logit, the lowest index among equals.  NaN counts as -inf, -inf is never
- * drawn; a row of nothing else gives token 0 with probability 0.  Sums and
- * weights in 64 bits.  temperature >= 0, top_k >= 0, top_p in (0, 1], min_p in
- * [0, 1] (else DIP_ERR_ARG).  The reference decodes greedily
- * (gen_utils.py:40-46) and has no counterpart.
+ * drawn; a row of nothing else gives token 0 with probability 0; where the largest
+ * is +inf, its equals alone count.  A weight is a whole number of 2^-shift, off by
+ * 4e-10 of itself beyond that, with shift 44 at 150000 tokens (51 at 2048 and fewer,
+ * one less for every doubling): sums are exact, and a weight below half a step is 0
+ * and never drawn, nor is a logit whose distance from the largest is beyond fp32.  A
+ * temperature between 0 and 1e-30 counts as 1e-30.  temperature in [0, 1e300], top_k >= 0, top_p in (0, 1], min_p in [0, 1]
+ * (else DIP_ERR_ARG).  The workspace needs no clearing; calls that may run at once
+ * need one each.  The reference decodes greedily (gen_utils.py:40-46) and has no
+ * counterpart.
  */
 enum { DIP_BF16 = 0, DIP_F16 = 1, DIP_F32 = 2 };
 size_t dip_sample_workspace_size(int64_t rows, int64_t vocab);
