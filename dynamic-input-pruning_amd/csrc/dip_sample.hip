@@ -1107,8 +1107,11 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
   a.row_bytes = row_stride * size;
   a.u = u;
   a.top_p = top_p;
-  // (0: greedy; a temperature below 1e-30 counts as that)
-  a.per_64th = temperature > 0 ? 64 * 1.4426950408889634074 / fmax(temperature, 1e-30) : 0;
+  // 0: greedy, which top-k 1 is at any temperature (one row of 151936 bf16 logits 25
+  // us by way of its weights, 5 greedily); a temperature below 1e-30 counts as that
+  a.per_64th = temperature > 0 && top_k != 1
+                   ? 64 * 1.4426950408889634074 / fmax(temperature, 1e-30)
+                   : 0;
   a.per_hi = (float)a.per_64th;
   a.per_lo = (float)(a.per_64th - a.per_hi);
   a.least = min_p * (double)(1ull << shift);
