@@ -31,7 +31,7 @@
 // and a choice among its results.  Short rows go through all of it in one launch.
 //
 // 64 rows of 151936 fp32 logits (39 MB), top-p: 9 us for max, at the memory's rate;
-// 19 for hist, where some 70 instructions make and bin each weight; 12 for gather,
+// 19 for hist, which makes and bins each weight; 12 for gather,
 // half of which is finding the borders; 10 for draw.  One row of bf16: 3, 7, 7, 7 us,
 // all waits on memory and barriers.
 #include "dip_common.h"
@@ -228,6 +228,7 @@ struct Weigher {
   float most, per_hi, per_lo;  // 64ths of an octave per logit, in two parts
   bool inf;                    // the largest is +inf, and only its equals count
   double least;                // min-p * 2^shift
+  float cap;                   // 61 octaves of weight, in the logit
   float bins_per_logit;
   const double* roots;         // 2^(shift - j / 64), in LDS
 
@@ -239,6 +240,7 @@ struct Weigher {
     most = key_value(top_key);
     inf = most == INFINITY;
     if (inf) most = 0.f;
+    cap = 64.f * 61 / per_hi;
     // bins reach down to the smallest logit, or to the weight that counts as 0
     const float range = fminf(most - key_value(least_key), 64.f * (a.shift + 1) / per_hi);
     bins_per_logit = range > 0.f && !inf ? fminf(kBins / range, 3e38f) : 0.f;
@@ -247,24 +249,27 @@ struct Weigher {
   DIP_DEV float value(float x) const {
     return !inf ? x : x == INFINITY ? 0.f : -INFINITY;
   }
-  // w * 2^shift; 0 for -inf.
+  // w * 2^shift; less than 1 / 2, a whole number of 0, beyond `cap` and for -inf.
   DIP_DEV double scaled(float x) const {
-    const float hi = most - x, n = rintf(hi * per_hi);
-    float low = hi * per_lo;
+    float hi = most - x, low = 0.f;
     if (kExact) {
       const float part = hi - most;  // most - x = hi + lo exactly
-      const float lo = (most - (hi - part)) - (x + part);
-      low = fmaf(lo, per_hi, low);
+      low = ((most - (hi - part)) - (x + part)) * per_hi;
     }
-    const float f = fmaf(-hi, per_hi, n) - low;
+    const bool far = kExact && !(hi <= cap);
+    if (!kExact) hi = fminf(hi, cap);
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are n
+    const float t = fmaf(hi, per_hi, kRound), n = t - kRound;
+    const float f = fmaf(-hi, per_lo, fmaf(-hi, per_hi, n)) - low;
     constexpr float c = 0.69314718055994530942f / 64;
     const float q = f * fmaf(f, fmaf(f, c * c * c / 6, c * c / 2), c);
-    const int i = (int)fminf(n, 4096.f);
+    const uint32_t i = __float_as_uint(t);
     const double r = roots[i & 63];
     // the octaves off the exponent (a root's is 2^shift or less, 2^-14 at the least)
-    const uint64_t w = __builtin_bit_cast(uint64_t, fma(r, (double)q, r)) -
-                       ((uint64_t)((uint32_t)(i & ~63) << 14) << 32);
-    return n <= 64.f * 60 ? __builtin_bit_cast(double, w) : 0.0;  // (not for -inf)
+    const uint64_t w = __builtin_bit_cast(uint64_t, fma(r, (double)q, r));
+    const uint32_t top = (uint32_t)(w >> 32) - ((i << 14) & 0xFFF00000u);
+    const uint64_t v = (uint64_t)top << 32 | (uint32_t)w;
+    return far ? 0.0 : __builtin_bit_cast(double, v);
   }
   // Rounded to a whole number: below 2^52, so the sum's low bits are it.
   DIP_DEV static unsigned long long whole(double w) {
@@ -1108,9 +1113,9 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
   a.u = u;
   a.top_p = top_p;
   // 0: greedy, which top-k 1 is at any temperature (one row of 151936 bf16 logits 25
-  // us by way of its weights, 5 greedily); a temperature below 1e-30 counts as that
+  // us by way of its weights, 5 greedily); temperatures beyond 1e-30 and 1e30 count as these
   a.per_64th = temperature > 0 && top_k != 1
-                   ? 64 * 1.4426950408889634074 / fmax(temperature, 1e-30)
+                   ? 64 * 1.4426950408889634074 / fmin(fmax(temperature, 1e-30), 1e30)
                    : 0;
   a.per_hi = (float)a.per_64th;
   a.per_lo = (float)(a.per_64th - a.per_hi);

@@ -1,0 +1,53 @@
+"""GPU: temperatures and logits at the ends of their ranges."""
+import math
+
+import pytest
+import torch
+
+from kv4_util import drawn
+
+pytestmark = pytest.mark.gpu
+
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.parametrize("how", [dict(), dict(top_p=0.6), dict(top_k=7, min_p=0.5),
+                                 dict(top_k=300, top_p=0.5)])
+@pytest.mark.parametrize("temperature", [1e-300, 1e-35, 1e-12, 1e-8, 1e3, 1e29, 1e35, 1e300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [777, 40009])
+def test_temperatures(vocab, dtype, temperature, how):
+    """Where every distance is many times the temperature or next to nothing of it."""
+    import _dip_hip as K
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (2.5 * torch.randn(4, vocab, device="cuda", generator=g)).to(dtype)
+    x[1, ::3] = -math.inf
+    x[2, 1::2] = math.nan
+    x[3, 5:90] = 40.0  # equals at the top
+    u = torch.tensor([0.1, 0.9999, 0.37, 0.62], device="cuda")
+    print(f"sample {vocab} {dtype} temperature {temperature} {how}", flush=True)
+    token, prob = K.sample(x, u, temperature=temperature, **how)
+    # up to 40 apart, a weight at 1e30 is off from one at any higher by 4e-29
+    taken = min(max(temperature, 1e-30), 1e30)
+    for r in range(4):
+        t, p, w = drawn(x[r].double().cpu().numpy(), float(u[r]), temperature=taken, **how)
+        assert w[int(token[r])] > 0
+        assert abs(float(prob[r]) - p) <= 2.0 ** -21 * p
+        if temperature < 1e3:  # weights far apart or equal: sums are not near u
+            assert int(token[r]) == t, r
+
+
+@pytest.mark.parametrize("vocab", [700, 40009])
+@pytest.mark.parametrize("how", [dict(), dict(top_p=0.9), dict(top_k=5), dict(min_p=0.01)])
+def test_masks_of_the_lowest_value(vocab, how):
+    """Masked with the type's lowest value, next to very large logits and alone."""
+    import _dip_hip as K
+    x = torch.full((3, vocab), LOWEST, device="cuda")
+    x[0, 3], x[0, 600] = 3e38, 3e38
+    x[1, 5], x[1, 650] = -1.0, -1.5
+    u = torch.tensor([0.6, 0.2, 0.999], device="cuda")
+    token, prob = K.sample(x, u, **how)
+    for r in range(3):
+        t, p, _ = drawn(x[r].double().cpu().numpy(), float(u[r]), **how)
+        assert int(token[r]) == t
+        assert abs(float(prob[r]) - p) <= 2.0 ** -22 * p
