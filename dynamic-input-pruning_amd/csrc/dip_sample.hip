@@ -31,9 +31,9 @@
 // and a choice among its results.  Short rows go through all of it in one launch.
 //
 // 64 rows of 151936 fp32 logits (39 MB), top-p: 9 us for max, at the memory's rate;
-// 19 for hist, which makes and bins each weight; 12 for gather,
-// half of which is finding the borders; 10 for draw.  One row of bf16: 3, 7, 7, 7 us,
-// all waits on memory and barriers.
+// 19 for hist, which makes and bins each weight; 13 for gather, most of which is
+// finding the borders; 9 for draw.  One row of bf16: 3, 6.5, 7 and 7.5 us, all waits
+// on memory and barriers.
 #include "dip_common.h"
 #include "dip_internal.h"
 
