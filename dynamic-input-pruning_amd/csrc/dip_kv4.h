@@ -120,6 +120,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // 2^x; results below the normal range are 0.
 DIP_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Whether the cache has the rows first .. first + tokens - 1 (tokens >= 0), for any
+// first: a position on the device may hold the type's ends.
+__host__ DIP_DEV bool rows_in_cache(int64_t first, int tokens, int max_len) {
+  return first >= 0 && first <= (int64_t)max_len - tokens;
+}
+
 // Cache rows that the token at position pos attends: 0 .. pos.
 DIP_DEV int rows_at(int64_t pos, int max_len) {
   return pos < 0 ? 0 : (pos < (int64_t)max_len ? (int)pos + 1 : max_len);

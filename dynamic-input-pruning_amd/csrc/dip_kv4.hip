@@ -76,7 +76,7 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
   const int l = threadIdx.x & 63;
   const int64_t task = (int64_t)blockIdx.x * kWriteWaves + (threadIdx.x >> 6);
   const int64_t first = a.pos ? *a.pos : a.start;
-  const bool ok = first >= 0 && first + a.tokens <= a.max_len;  // (a.pos may lie outside)
+  const bool ok = rows_in_cache(first, a.tokens, a.max_len);  // (a.pos may lie outside)
   const int64_t vtasks = (int64_t)a.vblocks * 4 * a.nkv;
   if (task < vtasks) {
     if (!ok) return;

@@ -341,3 +341,8 @@ def test_refusals():
     assert K.kv4_prompt_attention(q.view(1, -1)[:0], cache, 64, None, SCALE).shape == (0, 512)
     assert K.kv4_read(cache, 64)[0].shape == (0, 2, 128)
     K.kv4_write(x[:0], x[:0], cache, start=64)
+
+
+@pytest.mark.parametrize("pos", [2 ** 63 - 1, 2 ** 63 - 2, -2 ** 63])
+def test_token_at_the_ends_of_int64_writes_no_row(pos):
+    test_token_outside_the_cache_writes_no_row(pos)
