@@ -50,10 +50,22 @@ DIP_DEV uint32_t f32x2_to_bf16x2(float lo, float hi) {
 
 // The same without making NaN canonical, for values whose NaN bits nobody
 // sees: the conversion keeps a NaN a NaN.
+//
+// Both are inline asm, round which the compiler keeps none of the waits that it
+// keeps round an instruction it knows: two between the result and an MFMA or DPP
+// that reads it, one behind a v_exp, v_rcp or the like that wrote an argument.
+// Code that depends on them takes cvt_bf16x2; in the transposed prompt GEMM, whose
+// registers that one spills, the build has them (tests/test_asm_waits.py).
 DIP_DEV uint32_t f32x2_to_bf16x2_nan(float lo, float hi) {
   uint32_t r;
   asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(lo), "v"(hi));
   return r;
+}
+
+// f32x2_to_bf16x2_nan as the compiler's own conversion, the same instruction.
+DIP_DEV uint32_t cvt_bf16x2(float lo, float hi) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{lo, hi}, bf16x2_t));
 }
 
 // |v| as the bf16 key the top-k orders by: sign dropped, subnormal

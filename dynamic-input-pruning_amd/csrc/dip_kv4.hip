@@ -142,7 +142,7 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
     const uint32_t sn[4] = {sv.x, sv.y, sv.z, sv.w};
     auto lo = [](uint32_t v) { return __uint_as_float(v << 16); };
     auto hi = [](uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); };
-    auto pack = [](float u, float v) { return f32x2_to_bf16x2_nan(u, v); };
+    auto pack = [](float u, float v) { return cvt_bf16x2(u, v); };
     double ss = 0.0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {

@@ -186,10 +186,10 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
           ps[t][r] = ok[t][r] ? p[t][r] * v : 0.f;
         }
       const bf16x8_t bp = __builtin_bit_cast(
-          bf16x8_t, u32x4_t{f32x2_to_bf16x2_nan(ps[0][0], ps[0][1]),
-                            f32x2_to_bf16x2_nan(ps[0][2], ps[0][3]),
-                            f32x2_to_bf16x2_nan(ps[1][0], ps[1][1]),
-                            f32x2_to_bf16x2_nan(ps[1][2], ps[1][3])});
+          bf16x8_t, u32x4_t{cvt_bf16x2(ps[0][0], ps[0][1]),
+                            cvt_bf16x2(ps[0][2], ps[0][3]),
+                            cvt_bf16x2(ps[1][0], ps[1][1]),
+                            cvt_bf16x2(ps[1][2], ps[1][3])});
 #pragma unroll
       for (int t = 2 * g; t < 2 * g + 2; ++t)
         acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va[t], bp, acc[t], 0, 0, 0);

@@ -59,8 +59,8 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
       uint32_t o[4];
 #pragma unroll
       for (int m = 0; m < 4; ++m)
-        o[m] = f32x2_to_bf16x2_nan((float)kv4_nibble(x[g], kv4_shift(2 * m)) * s,
-                                   (float)kv4_nibble(x[g], kv4_shift(2 * m + 1)) * s);
+        o[m] = cvt_bf16x2((float)kv4_nibble(x[g], kv4_shift(2 * m)) * s,
+                          (float)kv4_nibble(x[g], kv4_shift(2 * m + 1)) * s);
       out[(4 * g + c) * 32 + row] = make_uint4(o[0], o[1], o[2], o[3]);
     }
   } else if (tid < 132) {
@@ -88,8 +88,8 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         const int r = 16 * c + 4 * h + 2 * m, j = 4 * c + 2 * m;
-        o[m] = f32x2_to_bf16x2_nan(value(lo, r, j), value(lo, r + 1, j + 1));
-        o[2 + m] = f32x2_to_bf16x2_nan(value(hi, r + 8, j), value(hi, r + 9, j + 1));
+        o[m] = cvt_bf16x2(value(lo, r, j), value(lo, r + 1, j + 1));
+        o[2 + m] = cvt_bf16x2(value(hi, r + 8, j), value(hi, r + 9, j + 1));
       }
       out[512 + (c * 2 + h) * 128 + d] = make_uint4(o[0], o[1], o[2], o[3]);
     }
@@ -252,10 +252,10 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const bf16x8_t p = __builtin_bit_cast(
-            bf16x8_t, u32x4_t{f32x2_to_bf16x2_nan(s[b][8 * c], s[b][8 * c + 1]),
-                              f32x2_to_bf16x2_nan(s[b][8 * c + 2], s[b][8 * c + 3]),
-                              f32x2_to_bf16x2_nan(s[b][8 * c + 4], s[b][8 * c + 5]),
-                              f32x2_to_bf16x2_nan(s[b][8 * c + 6], s[b][8 * c + 7])});
+            bf16x8_t, u32x4_t{cvt_bf16x2(s[b][8 * c], s[b][8 * c + 1]),
+                              cvt_bf16x2(s[b][8 * c + 2], s[b][8 * c + 3]),
+                              cvt_bf16x2(s[b][8 * c + 4], s[b][8 * c + 5]),
+                              cvt_bf16x2(s[b][8 * c + 6], s[b][8 * c + 7])});
 #pragma unroll
         for (int d = 0; d < 4; ++d)
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
@@ -315,9 +315,8 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
     const float f = bad_row[d] < limit ? NAN : inv;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      o[8 * d + 2 * i + h] = make_uint2(f32x2_to_bf16x2_nan(acc[d][4 * i] * f, acc[d][4 * i + 1] * f),
-                                        f32x2_to_bf16x2_nan(acc[d][4 * i + 2] * f,
-                                                            acc[d][4 * i + 3] * f));
+      o[8 * d + 2 * i + h] = make_uint2(cvt_bf16x2(acc[d][4 * i] * f, acc[d][4 * i + 1] * f),
+                                        cvt_bf16x2(acc[d][4 * i + 2] * f, acc[d][4 * i + 3] * f));
   }
 }
 
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(256) void kv4_prompt_combine_kernel(Kv4AttnArgs a) 
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   reinterpret_cast<uint32_t*>(a.out)[((size_t)(cc / a.group) * a.nkv * a.group +
                                       kvh * a.group + cc % a.group) * 64 + l] =
-      f32x2_to_bf16x2_nan(o0 * inv, o1 * inv);
+      cvt_bf16x2(o0 * inv, o1 * inv);
 }
 
 struct Plan {
