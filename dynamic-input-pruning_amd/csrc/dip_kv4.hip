@@ -25,12 +25,14 @@ DIP_DEV double sum16_64(double v) {
   return v + dpp_mov64<0x140>(v);
 }
 
-// 1 / sqrt(x) in 64 bits, x > 0 and normal: two Newton steps on the hardware's
-// estimate (2^-26 or better).
+// 1 / sqrt(x) in 64 bits, x normal, or 0, infinite or NaN (inf, 0, NaN): two Newton
+// steps on the hardware's estimate (2^-26 or better), which is the result itself
+// where x is infinite and the steps would make inf * 0 of it.
 DIP_DEV double rsqrt64(double x) {
-  double r = __builtin_amdgcn_rsq(x);
+  const double e = __builtin_amdgcn_rsq(x);
+  double r = fma(e * 0.5, fma(-x * e, e, 1.0), e);
   r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
-  return fma(r * 0.5, fma(-x * r, r, 1.0), r);
+  return x > 0.0 && x < INFINITY ? r : e;
 }
 
 struct Kv4WriteArgs {
@@ -150,12 +152,16 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
       ss = fma(u, u, ss);
       ss = fma(v, v, ss);
     }
-    const double r = rsqrt64(fma(sum16_64(ss), 1.0 / kKvHeadDim, (double)a.eps));
+    double r = rsqrt64(fma(sum16_64(ss), 1.0 / kKvHeadDim, (double)a.eps));
+    // (without an eps, subnormal numbers alone take r past fp32's range)
+    const float up = r > 0x1p100 ? 0x1p64f : 1.f;
+    r = r > 0x1p100 ? r * 0x1p-64 : r;
     const float r0 = (float)r, r1 = (float)(r - (double)r0);
     uint32_t y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t n = pack(fmaf(lo(x[e]), r0, lo(x[e]) * r1), fmaf(hi(x[e]), r0, hi(x[e]) * r1));
+      const float u = lo(x[e]) * up, v = hi(x[e]) * up;
+      const uint32_t n = pack(fmaf(u, r0, u * r1), fmaf(v, r0, v * r1));
       y[e] = pack(lo(w[e]) * lo(n), hi(w[e]) * hi(n));
     }
     // rotate_half: dims [0, 64) take -y[d + 64], dims [64, 128) take y[d - 64]

@@ -1,0 +1,69 @@
+"""GPU: the 4-bit cache and its attention at the ends of the numbers' range, against
+the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from kv4_util import quantised
+from test_gpu_kv4 import _gen, _rope_reference, _same
+
+pytestmark = pytest.mark.gpu
+
+
+def _tables(max_len):
+    ang = torch.arange(max_len, device="cuda")[:, None] * 0.37 ** torch.arange(
+        64, device="cuda")[None] * 3.0
+    return [torch.cat((f(ang), f(ang)), -1).to(torch.bfloat16) for f in (torch.cos, torch.sin)]
+
+
+def _norm_rope(x, nh, nkv, eps):
+    """(q, k, v) of the fused form as tensors, the token's form and the rows' alike."""
+    import _dip_hip as K
+    tokens = x.shape[0]
+    w = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    cos, sin = _tables(64)
+    cache, one = K.kv4_cache(nkv, 64), K.kv4_cache(nkv, 64)
+    q, q1 = (torch.empty(tokens, nh, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    K.qk_norm_rope_kv4_rows(x.view(tokens, -1), w, w, cos, sin, q.view(tokens, -1), cache, nh, nkv,
+                            eps, start=5)
+    for t in range(tokens):
+        K.qk_norm_rope_kv4(x[t].view(-1), w, w, cos, sin, torch.tensor([5 + t], device="cuda"),
+                           q1[t].view(-1), one, nh, nkv, eps)
+    k, v = K.kv4_read(cache, 5, tokens)
+    k1, v1 = K.kv4_read(one, 5, tokens)
+    for a, b in ((q, q1), (k, k1), (v, v1)):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+    c, s = (t[5:5 + tokens, None].cpu() for t in (cos, sin))
+    ref = _rope_reference(x.cpu(), w.cpu(), c, s, eps)
+    return q, k, v, ref[:, :nh], ref[:, nh:nh + nkv]
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_norm_of_a_head_with_an_infinity(value):
+    """An infinite mean makes the finite dimensions 0 and the infinite ones NaN; a NaN
+    makes all of them NaN."""
+    nh, nkv = 4, 2
+    x = torch.randn(3, nh + 2 * nkv, 128, device="cuda", generator=_gen(0)).to(torch.bfloat16)
+    x[0, 1, 70] = x[1, nh, 3] = x[2, nh + 1, 127] = value
+    q, k, v, want_q, want_k = _norm_rope(x, nh, nkv, 1e-6)
+    for (t, h), got, want in (((0, 1), q, want_q), ((1, 0), k, want_k), ((2, 1), k, want_k)):
+        if got is k:
+            want = quantised(want.to(torch.bfloat16))
+        assert _same(got[t, h], want[t, h])
+        assert bool(got[t, h].isnan().all()) == math.isnan(value)
+
+
+def test_norm_of_tiny_heads_without_eps():
+    """Subnormal numbers alone: the root's reciprocal is past fp32's largest."""
+    nh, nkv = 4, 2
+    n = torch.randint(-7, 8, (9, nh + 2 * nkv, 128), device="cuda", generator=_gen(1))
+    n[..., 0] = 3  # (no head of zeros)
+    x = (n.double() * 2.0 ** -133).to(torch.bfloat16)
+    assert bool((x.double() == n.double() * 2.0 ** -133).all())
+    q, k, v, want_q, want_k = _norm_rope(x, nh, nkv, 0.0)
+    # q's sums of rounded products are taken in fp32 before they are rounded
+    err = (q.double().cpu() - want_q).abs()
+    assert bool((err <= 2.0 ** -7 * want_q.abs().max()).all())
+    assert (err != 0).double().mean() < 1e-3
+    assert _same(k, quantised(want_k.to(torch.bfloat16)))
