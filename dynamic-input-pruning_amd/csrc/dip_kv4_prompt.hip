@@ -21,6 +21,10 @@ constexpr int kStepBlocks = 2;   // blocks of 32 cache rows of a step
 constexpr int kTileRows = 32 * kStepBlocks;
 constexpr int kBlockVecs = 1024; // 16-byte pieces of an expanded block: 512 of keys, 512 of values
 
+// The largest scale of finite values: bf16's largest over 7, cut to 5 bits.  (Times 7
+// it is still a bf16 number.)
+constexpr float kMaxScale = 0x1.2p125f;
+
 // The expanded cache: per kv head and block of 32 rows
 //   keys   [16][32 rows] pieces: piece (u, row) holds dimensions 8 u .. 8 u + 7;
 //   values [2][2][128 dims] pieces: piece (c, h, d) holds dimension d of rows
@@ -28,7 +32,8 @@ constexpr int kBlockVecs = 1024; // 16-byte pieces of an expanded block: 512 of 
 // each the order in which the lanes of a 32x32x16 MFMA take their operand.  Blocks
 // in pairs; what lies behind the cache's end is 0.  bad[kv head][block]: a byte per
 // value group, the first row of the block whose group is not finite (255: none).
-// Those values are 0 here, so that a weight of 0 makes them 0.
+// Those values are 0 here, and a number of -8, which nobody writes, is -7: whatever
+// the rows that nobody has written hold, a weight of 0 makes 0 of it.
 __global__ __launch_bounds__(256) void kv4_expand_kernel(
     const uint32_t* __restrict__ kc, const uint32_t* __restrict__ vc,
     const uint16_t* __restrict__ sc, uint4* __restrict__ work, uint32_t* __restrict__ bad,
@@ -67,7 +72,7 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
     const int g = tid - 128;
     uint32_t first = 255;
     for (int r = kKvBlock - 1; r >= 0; --r)
-      if (!(fabsf(scale(r, 4 + g)) <= 4e37f)) first = r;  // 8 * s would not be finite
+      if (!(fabsf(scale(r, 4 + g)) <= kMaxScale)) first = r;
     const uint32_t w = first << (8 * g);
     uint32_t all = w;
     all |= __shfl_xor(all, 1, 64);
@@ -80,7 +85,7 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
     const uint32_t lo = blk[kv4_value_word(d, h)], hi = blk[kv4_value_word(d, 2 + h)];
     auto value = [&](uint32_t w, int row, int j) {
       const float s = scale(row, g);
-      return fabsf(s) <= 4e37f ? (float)kv4_nibble(w, kv4_shift(j)) * s : 0.f;
+      return fabsf(s) <= kMaxScale ? (float)max(kv4_nibble(w, kv4_shift(j)), -7) * s : 0.f;
     };
 #pragma unroll
     for (int c = 0; c < 2; ++c) {

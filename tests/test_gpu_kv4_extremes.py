@@ -5,10 +5,12 @@ import math
 import pytest
 import torch
 
-from kv4_util import quantised
-from test_gpu_kv4 import _gen, _rope_reference, _same
+from kv4_util import attention, attention_bound, quantised, scale_of
+from test_gpu_kv4 import SCALE, _gen, _kv, _rope_reference, _same
 
 pytestmark = pytest.mark.gpu
+
+BIG = torch.finfo(torch.bfloat16).max
 
 
 def _tables(max_len):
@@ -67,3 +69,59 @@ def test_norm_of_tiny_heads_without_eps():
     assert bool((err <= 2.0 ** -7 * want_q.abs().max()).all())
     assert (err != 0).double().mean() < 1e-3
     assert _same(k, quantised(want_k.to(torch.bfloat16)))
+
+
+def _check(out, q, k, v):
+    """Of the first and the last head."""
+    tokens, nh = q.shape[:2]
+    rows, nkv = k.shape[:2]
+    limits = [rows - tokens + t + 1 for t in range(tokens)]
+    kd, vd = quantised(k), quantised(v)
+    for h, kv in ((0, 0), (nh - 1, nkv - 1)):
+        ref, size = attention(q[:, h:h + 1], kd[:, kv:kv + 1], vd[:, kv:kv + 1], limits, SCALE)
+        err = (out.view(q.shape)[:, h:h + 1].double().cpu() - ref).abs()
+        assert bool((err <= attention_bound(ref, size, scale_of(v).max())).all()), float(err.max())
+
+
+# one token, its rows in one launch and split; a prompt's tokens in 16 columns to a
+# tile; in 128 over the expanded cache; the same with the rows split
+ROUTES = [("token", 16, 2, 200, 1), ("token", 16, 2, 3000, 1), ("columns", 8, 2, 200, 3),
+          ("tiles", 64, 1, 150, 130), ("splits", 64, 1, 630, 130)]
+
+
+def _route(K, tokens, start, nh, nkv):
+    """Which kernels a prompt goes through, from its workspace: none or some sums of 16
+    columns, or the expanded rows, alone or followed by sums of 128 columns."""
+    nbytes = K.lib.dip_kv4_prompt_attention_workspace_size(tokens, start, nh, nkv, 128)
+    blocks = -(-(start + tokens) // 64) * 2 * nkv
+    sums = nbytes - blocks * 16384 - -(-blocks * 4 // 16) * 16
+    one = -(-tokens * (nh // nkv) // 128) * nkv * 128 * 130 * 4
+    return "tiles" if sums == 0 else "splits" if sums > 0 and sums % one == 0 else "columns"
+
+
+def _attend(route, q, k, v):
+    """Attention of the last tokens by one route; the rows behind hold anything."""
+    import _dip_hip as K
+    rows, nkv = k.shape[:2]
+    tokens, nh = q.shape[:2]
+    cache = K.kv4_cache(nkv, rows + 70)
+    cache.scales[:] = BIG  # finite, times each number (-8) beyond the largest
+    cache.k[:], cache.v[:] = -120, -120
+    K.kv4_write(k, v, cache)
+    if route == "token":
+        return K.kv4_decode_attention(q.view(-1), cache, torch.tensor([rows - 1], device="cuda"),
+                                      None, SCALE)
+    assert _route(K, tokens, rows - tokens, nh, nkv) == route, "these sizes take another route"
+    return K.kv4_prompt_attention(q.view(tokens, -1), cache, rows - tokens, None, SCALE)
+
+
+@pytest.mark.parametrize("size", [2.97e38, 2.99e38, BIG])
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_a_row_of_the_largest_values(route, nh, nkv, rows, tokens, size):
+    """Even weights over one such row and many others: on either side of the group
+    scale of 2^125."""
+    g = _gen(2)
+    k, v = _kv(g, rows, nkv)
+    v[7] = size
+    q = torch.zeros(tokens, nh, 128, dtype=torch.bfloat16, device="cuda")
+    _check(_attend(route, q, k, v), q, k, v)
