@@ -117,6 +117,16 @@ struct Kv4AttnArgs {
 constexpr int kKvPart = 2 + kKvHeadDim;  // max, sum, value sum of one column
 constexpr float kLog2e = 1.44269504088896340736f;
 
+// The attention kernels' weights are 2^(score - base), against a base that follows the
+// running maximum: it is raised to kDown above a new one that passes the old by more
+// than kSlack (powers of 2; score in them too), so that the sums are seldom taken
+// against a new base.  Weights then lie below 2^(kSlack - kDown), and the sums of 2^18
+// of them times the largest values within fp32, where with weights of about 1 two
+// rows of large values were beyond it.  kDown cancels in the division.  (At the small
+// end a weight of 2^-n of the largest rounds coarser in value groups of a scale below
+// 2^(n - 100), the least that scales are.)
+constexpr float kSlack = 8.f, kDown = 26.f;
+
 // 2^x; results below the normal range are 0.
 DIP_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

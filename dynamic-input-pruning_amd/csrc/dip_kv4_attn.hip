@@ -23,10 +23,6 @@ DIP_DEV int blocks_per_wave(int rows, int waves) {
   return max(1, (blocks + waves - 1) / waves);
 }
 
-// How far (in powers of 2) a score may pass the maximum that the sums are taken
-// against before they are taken against a new one.
-constexpr float kSlack = 8.f;
-
 DIP_DEV float scale_lo(uint32_t w) { return __uint_as_float(w << 16); }
 DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
@@ -38,8 +34,8 @@ DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 //     so the result is (1 / 16) sum q x exactly as numbers go; the group's scale
 //     multiplies it, and the sum over the four groups is a score.  Lane (c, col)
 //     ends up with the scores of rows 4 c + r and 16 + 4 c + r;
-//   softmax with a running maximum (the columns' lanes agree on it by two lane
-//     swaps) in fp32;
+//   softmax against a base that follows the running maximum (the columns' lanes
+//     agree on it by two lane swaps) in fp32;
 //   values^T: B = bf16(weight * the row's value scale) of the group, where the
 //     score is; A = 16 dimensions of the 32 rows as 1.5 + q / 16, and ones, whose
 //     product is the sum that the 1.5 must not add.  (Rounding weight * scale to
@@ -102,7 +98,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
   for (int t = 0; t < 8; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int g = 0; g < kKvGroups; ++g) bias[g] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, den = 0.f;  // den: this lane's rows only
+  float m = -INFINITY, den = 0.f;  // m: the base; den: this lane's rows only
 
   struct Raw {
     uint4 kw[2], vw[2], sw[2][4];
@@ -144,7 +140,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
         mx = fmaxf(mx, s[t][r]);
       }
     }
-    mx = fmaxf(m, row_pair_max32(row_pair_max16(mx)));
+    mx = fmaxf(m, row_pair_max32(row_pair_max16(mx)) + kDown);
     if (__any(mx > m + kSlack)) {
       const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);  // what the sums so far are worth
       den *= f;

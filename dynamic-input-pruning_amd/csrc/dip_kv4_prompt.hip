@@ -101,12 +101,6 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
   }
 }
 
-// How far (in powers of 2) a score may pass the maximum that the sums are taken
-// against before they are taken against a new one: with 32 columns to a wave some
-// column has a new maximum in most steps, and the sums' 64 products are a quarter of
-// a step's instructions (4096 tokens of 64 / 8 heads 350 us for 343).
-constexpr float kSlack = 8.f;
-
 // The steps of 64 rows that a split takes of a tile's.
 DIP_DEV int steps_per_split(int rows, int splits) {
   const int steps = (rows + kTileRows - 1) / kTileRows;
@@ -126,7 +120,8 @@ typedef const __attribute__((address_space(1))) void global_void;
 // h = l / 32:
 //   scores^T = K Q^T: 32x32x16 MFMAs, the queries' operand held in registers for
 //     good; lane (h, column) gets the scores of rows 8 i + 4 h + 0 .. 3;
-//   softmax in fp32 with a running maximum (lanes l and l ^ 32 share a column);
+//   softmax in fp32 against a base that follows the running maximum (lanes l and
+//     l ^ 32 share a column);
 //   out^T += V^T P^T, the weights rounded to bf16 in place: they are the operand
 //     as they lie.  (Off by 2^-8 of itself at most, as any bf16 weight is.)
 // 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 300 to 335 us, 0.82
@@ -190,7 +185,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
-  float m = -INFINITY, den = 0.f;  // den: this lane's rows only
+  float m = -INFINITY, den = 0.f;  // m: the base; den: this lane's rows only
 
   auto step = [&](const uint4* buf, int t) {
     if (t * kTileRows >= most) return;  // every row lies behind this wave's columns
@@ -225,7 +220,10 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
     for (int b = 0; b < kStepBlocks; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[b][r]);
-    mx = fmaxf(m, row_pair_max32(mx) * c2);
+    mx = fmaxf(m, row_pair_max32(mx) * c2 + kDown);
+    // kSlack: with 32 columns to a wave some column has a new maximum in most steps, and
+    // the sums' 64 products are a quarter of a step's instructions (4096 tokens of 64 / 8
+    // heads 350 us for 343)
     if (__any(mx > m + kSlack)) {
       const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);
       den *= f;

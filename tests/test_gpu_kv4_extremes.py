@@ -125,3 +125,39 @@ def test_a_row_of_the_largest_values(route, nh, nkv, rows, tokens, size):
     v[7] = size
     q = torch.zeros(tokens, nh, 128, dtype=torch.bfloat16, device="cuda")
     _check(_attend(route, q, k, v), q, k, v)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 118, 2.99e38, BIG])
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_values_up_to_the_largest(route, nh, nkv, rows, tokens, size):
+    """Group scales up to the largest one that finite values have."""
+    g = _gen(rows)
+    k, _ = _kv(g, rows, nkv)
+    v = (torch.rand(rows, nkv, 128, device="cuda", generator=g) * 2 - 1).mul(size)
+    v[:, :, ::32] = size  # every group's largest
+    v = v.to(torch.bfloat16)
+    q = torch.randn(tokens, nh, 128, device="cuda", generator=g).to(torch.bfloat16)
+    _check(_attend(route, q, k, v), q, k, v)
+
+
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_large_values_behind_a_small_maximum(route, nh, nkv, rows, tokens):
+    """The first rows' scores are just low enough for the sums not to be taken against
+    a new maximum: all later weights are above 1 until the division."""
+    g = _gen(3)
+    c = torch.full((rows,), 7.5 / (128 * SCALE * math.log2(math.e)), device="cuda")
+    c[:32] = 0
+    k = c[:, None, None].expand(rows, nkv, 128).to(torch.bfloat16)
+    v = torch.full((rows, nkv, 128), 2.0 ** 127, dtype=torch.bfloat16, device="cuda")
+    q = torch.ones(tokens, nh, 128, dtype=torch.bfloat16, device="cuda")
+    _check(_attend(route, q, k, v), q, k, v)
+
+
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_tiny_values(route, nh, nkv, rows, tokens):
+    """2^-70 and the numbers just below it, as accurate as any."""
+    g = _gen(4)
+    k, v = _kv(g, rows, nkv)
+    v = (v.double() * 2.0 ** -70).to(torch.bfloat16)
+    q = torch.randn(tokens, nh, 128, device="cuda", generator=g).to(torch.bfloat16)
+    _check(_attend(route, q, k, v), q, k, v)
