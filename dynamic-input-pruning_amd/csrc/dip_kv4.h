@@ -55,15 +55,22 @@ DIP_DEV int kv4_value_word(int d, int c) {
 DIP_DEV int kv4_row_quarter(int r) { return (r >> 2) & 3; }
 DIP_DEV int kv4_row_elem(int r) { return 4 * (r >> 4) + (r & 3); }
 
-// One word as an MFMA operand of 8 bf16 values 1.5 + q / 16 (exact).
+// One word as an MFMA operand of 8 bf16 values (1.5 + q / 16) * 2^-kDown (exact).
+template <int kDown = 0>
 DIP_DEV bf16x8_t kv4_biased(uint32_t w) {
+  constexpr uint32_t kFlip = kPairMagicFlip - kDown * 0x00800080u;
   u32x4_t r;
-  r.x = (w & kPairMask) ^ kPairMagicFlip;
-  r.y = ((w >> 4) & kPairMask) ^ kPairMagicFlip;
-  r.z = ((w >> 8) & kPairMask) ^ kPairMagicFlip;
-  r.w = (__builtin_amdgcn_alignbit(w, w, 12) & kPairMask) ^ kPairMagicFlip;
+  r.x = (w & kPairMask) ^ kFlip;
+  r.y = ((w >> 4) & kPairMask) ^ kFlip;
+  r.z = ((w >> 8) & kPairMask) ^ kFlip;
+  r.w = (__builtin_amdgcn_alignbit(w, w, 12) & kPairMask) ^ kFlip;
   return __builtin_bit_cast(bf16x8_t, r);
 }
+
+// Keys are taken 2^-8 lower, so that the 1.5 times 32 of bf16's largest queries stays
+// finite.
+constexpr int kKeyDown = 8;
+constexpr float kKeyUnit = 1.f / (1 << kKeyDown);
 
 // Nibble at `shift` as a signed number.
 DIP_DEV int kv4_nibble(uint32_t w, int shift) {

@@ -29,10 +29,10 @@ DIP_DEV float scale_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 // A tile of 16 columns, each a (token, query head) of one kv head, over the
 // rows of one split, cut over the W waves of the workgroup.  Per block of 32
 // rows a wave computes, all in registers:
-//   scores^T: A = 16 keys as 1.5 + q / 16, B = the columns' queries, one MFMA per
-//     group of 32 dimensions with -1.5 * (sum of the query's group) as its start,
-//     so the result is (1 / 16) sum q x exactly as numbers go; the group's scale
-//     multiplies it, and the sum over the four groups is a score.  Lane (c, col)
+//   scores^T: A = 16 keys as (1.5 + q / 16) / 256, B = the columns' queries, one MFMA
+//     per group of 32 dimensions with -1.5 / 256 * (sum of the query's group) as its
+//     start, so the result is (1 / 4096) sum q x exactly as numbers go; the group's
+//     scale multiplies it, and the sum over the four groups is a score.  Lane (c, col)
 //     ends up with the scores of rows 4 c + r and 16 + 4 c + r;
 //   softmax against a base that follows the running maximum (the columns' lanes
 //     agree on it by two lane swaps) in fp32;
@@ -82,11 +82,12 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
       const uint32_t x[4] = {w.x, w.y, w.z, w.w};
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s += scale_lo(x[e]) + scale_hi(x[e]);
+      for (int e = 0; e < 4; ++e)
+        s = fmaf(scale_hi(x[e]), kKeyUnit, fmaf(scale_lo(x[e]), kKeyUnit, s));
       qs[g] = -kPairBias * row_pair_sum32(row_pair_sum16(s));
     }
   }
-  const float sc2 = a.scale * kLog2e * kPairScale;
+  const float sc2 = a.scale * kLog2e * (kPairScale / kKeyUnit);
   const uint32_t* kc = a.kc + (size_t)kvh * a.max_len * (kKvKeyBytes / 4);
   const uint32_t* vc = a.vc + (size_t)kvh * (a.max_len / kKvBlock) * kKvBlockWords;
   const uint4* sc = reinterpret_cast<const uint4*>(a.sc + (size_t)kvh * a.max_len * kKvScaleVals);
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
       for (int g = 0; g < kKvGroups; ++g) {
         const floatx4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            kv4_biased(w[g]), bq[g], floatx4{qs[g], qs[g], qs[g], qs[g]}, 0, 0, 0);
+            kv4_biased<kKeyDown>(w[g]), bq[g], floatx4{qs[g], qs[g], qs[g], qs[g]}, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t z = g < 2 ? sw[t][r].x : sw[t][r].y;
@@ -156,13 +157,18 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
     }
     float p[2][4];
     const float base = m == -INFINITY ? 0.f : m;  // (no score above -inf yet: weights 0, or NaN)
+    {
+      // Not one multiply-add from v: the base comes from the rounded scores, and beyond
+      // 2^31 the rounding alone is further than weights reach.
+#pragma clang fp contract(off)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        p[t][r] = ok[t][r] ? fast_exp2(s[t][r] - base) : 0.f;
-        den += p[t][r];
-      }
+        for (int r = 0; r < 4; ++r) {
+          p[t][r] = ok[t][r] ? fast_exp2(s[t][r] - base) : 0.f;
+          den += p[t][r];
+        }
+    }
     bf16x8_t va[8];
     {
       const uint32_t w[8] = {vw[0].x, vw[0].y, vw[0].z, vw[0].w,

@@ -161,3 +161,30 @@ def test_tiny_values(route, nh, nkv, rows, tokens):
     v = (v.double() * 2.0 ** -70).to(torch.bfloat16)
     q = torch.randn(tokens, nh, 128, device="cuda", generator=g).to(torch.bfloat16)
     _check(_attend(route, q, k, v), q, k, v)
+
+
+@pytest.mark.parametrize("size", [1e10, 2e37, 3e38])
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_queries_up_to_the_largest(route, nh, nkv, rows, tokens, size):
+    """Scores far apart, and none beyond fp32: the row with the largest takes all."""
+    g = _gen(5)
+    c = torch.rand(rows, 1, 1, device="cuda", generator=g) * 0.001 - 0.0005
+    c[0] = 0.002  # the largest, of any token
+    k = c.expand(rows, nkv, 128).to(torch.bfloat16)
+    _, v = _kv(g, rows, nkv)
+    q = torch.full((tokens, nh, 128), size, device="cuda").to(torch.bfloat16)
+    out = _attend(route, q, k, v).view(tokens, nkv, nh // nkv, 128)
+    # one weight of 1 and the others 0: the row's values, off by the fp32 sums alone
+    want = quantised(v)[0].view(1, nkv, 1, 128)
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -11 * scale_of(v)[0].max()
+    assert bool(((out.double().cpu() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("size", [1e9, 1e13, 3e38])
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_equal_scores_of_large_queries(route, nh, nkv, rows, tokens, size):
+    """Rows with the same key share the weight evenly, however large the score."""
+    _, v = _kv(_gen(8), rows, nkv)
+    k = torch.full((rows, nkv, 128), 0.0017, device="cuda").to(torch.bfloat16)
+    q = torch.full((tokens, nh, 128), size, device="cuda").to(torch.bfloat16)
+    _check(_attend(route, q, k, v), q, k, v)
