@@ -252,7 +252,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
       o1 = fmaf(f, wacc[w][cl][d + 1], o1);
     }
     if (direct) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;  // no rows: 0
+      const float inv = rows == 0 ? 0.f : 1.f / sum;  // (a sum of 0: every score is -inf)
       reinterpret_cast<uint32_t*>(a.out)[((size_t)(cc / a.group) * a.nkv * a.group +
                                           kvh * a.group + cc % a.group) * (kKvHeadDim / 2) +
                                          d / 2] =
@@ -329,7 +329,7 @@ __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4A
     for (int w = 0; w < kCombine * kKvHeadDim / 64; ++w) sum += red[w][1];
 #pragma unroll
     for (int w = 0; w < kCombine; ++w) r += so[w][tid];
-    a.out[o + tid] = (uint16_t)f32_to_bf16(sum == 0.f ? 0.f : r / sum);
+    a.out[o + tid] = (uint16_t)f32_to_bf16(r / sum);
   }
 }
 

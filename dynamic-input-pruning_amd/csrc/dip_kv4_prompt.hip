@@ -328,7 +328,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
     }
     return;
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den;
+  const float inv = 1.f / den;  // (a sum of 0: every score is -inf, which makes NaN)
   uint2* o = reinterpret_cast<uint2*>(a.out + ((size_t)tok * a.nkv * a.group + head) * kKvHeadDim);
 #pragma unroll
   for (int d = 0; d < 4; ++d) {
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(256) void kv4_prompt_combine_kernel(Kv4AttnArgs a) 
       o1 = fmaf(w, v[u].y, o1);
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = 1.f / sum;
   reinterpret_cast<uint32_t*>(a.out)[((size_t)(cc / a.group) * a.nkv * a.group +
                                       kvh * a.group + cc % a.group) * 64 + l] =
       cvt_bf16x2(o0 * inv, o1 * inv);

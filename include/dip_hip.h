@@ -674,7 +674,11 @@ int dip_qk_norm_rope_kv4_rows(const uint16_t* qkv, const uint16_t* q_norm_w,
  * positions start .. start + tokens - 1, token t over rows 0 .. start + t, into
  * out [tokens, n_heads, head_dim].
  * Products of bf16 numbers summed in fp32, softmax and its sums in fp32, the
- * weights (times the values' scales) rounded to bf16, bf16 results.  The
+ * weights (times the values' scales) rounded to bf16, bf16 results.  Finite
+ * queries, keys and values give finite results while the sums q . k fit in fp32
+ * and the rows times the largest value stay below 2^146 (bf16's largest over
+ * 2^18 rows).  NaN in a query or an attended key, or no score above -inf, makes
+ * a head's result NaN; in a value group, those dimensions of it.  The
  * workspaces need no clearing; calls that may run at once need one each.
  */
 size_t dip_kv4_decode_attention_workspace_size(int64_t n_heads, int64_t n_kv_heads,

@@ -188,3 +188,18 @@ def test_equal_scores_of_large_queries(route, nh, nkv, rows, tokens, size):
     k = torch.full((rows, nkv, 128), 0.0017, device="cuda").to(torch.bfloat16)
     q = torch.full((tokens, nh, 128), size, device="cuda").to(torch.bfloat16)
     _check(_attend(route, q, k, v), q, k, v)
+
+
+@pytest.mark.parametrize("route,nh,nkv,rows,tokens", ROUTES)
+def test_no_score_above_minus_infinity(route, nh, nkv, rows, tokens):
+    """An infinity in the query against keys of the other sign: every score is -inf,
+    whose softmax is NaN, where a token without rows gives zeros."""
+    g = _gen(6)
+    k, v = _kv(g, rows, nkv)
+    k[:, :, 9] = -3.0
+    q = torch.randn(tokens, nh, 128, device="cuda", generator=g).to(torch.bfloat16)
+    q[0, 1, 9] = math.inf
+    nan = _attend(route, q, k, v).view(tokens, nh, 128).isnan()
+    want = torch.zeros_like(nan)
+    want[0, 1] = True
+    assert torch.equal(nan, want)
