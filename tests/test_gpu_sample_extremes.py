@@ -51,3 +51,24 @@ def test_masks_of_the_lowest_value(vocab, how):
         t, p, _ = drawn(x[r].double().cpu().numpy(), float(u[r]), **how)
         assert int(token[r]) == t
         assert abs(float(prob[r]) - p) <= 2.0 ** -22 * p
+
+
+@pytest.mark.parametrize("dtype,most,other,temperature", [
+    (torch.bfloat16, 16.25, 1.1e-4, 1.0), (torch.bfloat16, 16.25, -1.1e-4, 0.9),
+    (torch.bfloat16, 3e-6, -13.9, 0.8), (torch.bfloat16, 4096.0, 0.3, 300.0),
+    (torch.bfloat16, 1e30, 7.0, 1e29), (torch.float16, 18.0, 3.3e-4, 1.0),
+    (torch.float16, 30000.0, 0.77, 2000.0), (torch.float32, 17.000001, 1.2345678e-5, 1.0)])
+@pytest.mark.parametrize("vocab", [2, 40009])
+def test_logits_far_apart_in_magnitude(vocab, dtype, most, other, temperature):
+    """The difference of two logits has more bits than fp32: a weight carries its
+    rounding along.  A number beyond 1 draws the last token with a weight."""
+    import _dip_hip as K
+    x = torch.full((1, vocab), -math.inf, device="cuda")
+    x[0, 0], x[0, vocab - 1] = most, other
+    x = x.to(dtype)
+    token, prob = K.sample(x, torch.tensor([7.0], device="cuda"), temperature=temperature)
+    t, p, _ = drawn(x[0].double().cpu().numpy(), 7.0, temperature=temperature)
+    assert int(token) == t == vocab - 1
+    # the probability's rounding to fp32, the weight's 4e-10 and half a step of it
+    shift = 62 - max(11, math.ceil(math.log2(vocab)))
+    assert abs(float(prob) - p) <= (2.0 ** -24 + 1e-9 + 2.0 ** -1 / (p * 2.0 ** shift)) * p
