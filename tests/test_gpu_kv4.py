@@ -346,3 +346,37 @@ def test_refusals():
 @pytest.mark.parametrize("pos", [2 ** 63 - 1, 2 ** 63 - 2, -2 ** 63])
 def test_token_at_the_ends_of_int64_writes_no_row(pos):
     test_token_outside_the_cache_writes_no_row(pos)
+
+
+@pytest.mark.parametrize("rows", [8320, 8353, 16641, 32768, 65500])
+def test_decode_attention_over_many_splits(rows):
+    """Up to 256 splits, which are added up 64 at a time: half of every head's weight
+    lies on an early row, half on one of the same key in a later round's split."""
+    import _dip_hip as K
+    nh, nkv, max_len = 8, 1, 65536
+    splits = K.kv4_decode_attention_workspace_bytes(nh, nkv, max_len) // (16 * 130 * 4)
+    assert splits == 256
+    per = 4 * -(-(-(-rows // 32)) // (4 * splits)) * 32  # rows of a split
+    assert -(-rows // per) > 64
+    g = _gen(rows)
+    k, v = _kv(g, rows, nkv)
+    late = [64 * per, 64 * per + 31, min(100 * per + 7, rows - 5), rows * 9 // 10, rows - per - 1,
+            rows - 33, rows - 2, rows - 1]
+    early = [0, 17, per, 20 * per + 5, 63 * per + 1, 40 * per, 8 * per, 3 * per - 1]
+    k[late] = k[early]
+    cache = K.kv4_cache(nkv, max_len)
+    K.kv4_write(k, v, cache)
+    kd, vd = quantised(k), quantised(v)
+    q = (6 * kd[early, 0] / kd[early, 0].norm(dim=-1, keepdim=True)).to(torch.bfloat16).cuda()
+    _poison(cache, rows)
+    out = K.kv4_decode_attention(q.view(-1), cache, torch.tensor([rows - 1], device="cuda"), None,
+                                 2.0)
+    ref, size = attention(q[None], kd, vd, [rows], 2.0)
+    for h, (a, b) in enumerate(zip(late, early)):
+        w = torch.softmax(2.0 * (kd[:, 0] @ q[h].double().cpu()), 0)
+        assert float(w[a]) > 0.45 and float(w[b]) > 0.45
+    # scores of up to 2 * 6 * 40, off by 136 roundings of themselves: so much of a weight
+    slack = 2 * 136 * 2.0 ** -24 * 480
+    err = (out.view(1, nh, 128).double().cpu() - ref).abs()
+    bound = attention_bound(ref, size, scale_of(v).max()) + slack * size
+    assert bool((err <= bound).all()), float((err / bound).max())

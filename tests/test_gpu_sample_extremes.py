@@ -72,3 +72,24 @@ def test_logits_far_apart_in_magnitude(vocab, dtype, most, other, temperature):
     # the probability's rounding to fp32, the weight's 4e-10 and half a step of it
     shift = 62 - max(11, math.ceil(math.log2(vocab)))
     assert abs(float(prob) - p) <= (2.0 ** -24 + 1e-9 + 2.0 ** -1 / (p * 2.0 ** shift)) * p
+
+
+@pytest.mark.parametrize("temperature", [1e3, 1e29, 1e35, 1e300])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [777, 40009])
+def test_draws_of_nearly_equal_weights(vocab, dtype, temperature):
+    """At high temperatures the token drawn is the one at u of the running sum, to
+    within a token at either end where the sum is next to u."""
+    import _dip_hip as K
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (2.5 * torch.randn(5, vocab, device="cuda", generator=g)).to(dtype)
+    x[1, ::3] = -math.inf
+    u = torch.tensor([0.1, 0.9999, 0.37, 0.0, 0.62], device="cuda")
+    token, _ = K.sample(x, u, temperature=temperature)
+    taken = min(temperature, 1e30)
+    for r in range(5):
+        _, _, w = drawn(x[r].double().cpu().numpy(), float(u[r]), temperature=taken)
+        run, t, goal = w.cumsum(), int(token[r]), float(u[r]) * w.sum()
+        # a sum of n weights in steps of 2^-44 at least, each off by 4e-10 of itself
+        slack = vocab * (1e-9 + 2.0 ** -44)
+        assert w[t] > 0 and run[t] - w[t] - slack <= goal <= run[t] + slack
