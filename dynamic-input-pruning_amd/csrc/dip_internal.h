@@ -172,6 +172,9 @@ int device_cus();
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// HIP takes launches of less than 2^32 threads.
+inline bool launch_fits(int64_t grid, int threads) { return grid <= UINT32_MAX / threads; }
+
 inline int hip_status(hipError_t e) { return e == hipSuccess ? DIP_OK : (int)e; }
 
 // Lets `kernel` take up to `bytes` of dynamic LDS on the current device.

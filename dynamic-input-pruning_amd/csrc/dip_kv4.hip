@@ -247,7 +247,7 @@ int launch_write(Kv4WriteArgs a, hipStream_t stream) {
   const int64_t tasks = (int64_t)a.vblocks * 4 * a.nkv +
                         (int64_t)a.tokens * (((kNorm ? a.nh + a.nkv : a.nkv) + 3) / 4);
   const int64_t grid = (tasks + kWriteWaves - 1) / kWriteWaves;
-  if (grid > INT32_MAX) return DIP_ERR_SHAPE;
+  if (!launch_fits(grid, 64 * kWriteWaves)) return DIP_ERR_SHAPE;
   hipLaunchKernelGGL((kv4_write_kernel<kNorm>), dim3((unsigned)grid), dim3(64 * kWriteWaves), 0,
                      stream, a);
   return hip_status(hipGetLastError());
@@ -344,7 +344,7 @@ extern "C" int dip_kv4_read(const int8_t* k_cache, const int8_t* v_cache,
   if (!aligned16(k_out) || !aligned16(v_out)) return DIP_ERR_ALIGN;
   const int64_t blocks = touched(start, rows);
   const int64_t grid = blocks * n_kv_heads;  // four tasks of a block and head to a workgroup
-  if (grid > INT32_MAX) return DIP_ERR_SHAPE;
+  if (!launch_fits(grid, 64 * kWriteWaves)) return DIP_ERR_SHAPE;
   hipLaunchKernelGGL(kv4_read_kernel, dim3((unsigned)grid), dim3(64 * kWriteWaves), 0,
                      (hipStream_t)stream, reinterpret_cast<const uint32_t*>(k_cache),
                      reinterpret_cast<const uint32_t*>(v_cache), kv_scales,

@@ -385,14 +385,17 @@ int check_attn(const void* q, const void* kc, const void* vc, const void* sc, co
 int launch_attn(Kv4AttnArgs a, int64_t tiles, Cut cut, hipStream_t stream) {
   a.splits = cut.splits();
   const int64_t grid = tiles * a.nkv * a.splits;
-  if (grid > INT32_MAX || (int64_t)a.tokens * a.group * a.nkv > INT32_MAX) return DIP_ERR_SHAPE;
+  const int64_t cols = (int64_t)a.tokens * a.group * a.nkv;
+  if (!launch_fits(grid, 64 * cut.waves()) || cols > INT32_MAX ||
+      (a.splits > 1 && !launch_fits(cols, kCombine * kKvHeadDim)))
+    return DIP_ERR_SHAPE;
   if (cut.waves() == 8)
     hipLaunchKernelGGL((kv4_attn_kernel<8>), dim3((unsigned)grid), dim3(512), 0, stream, a);
   else
     hipLaunchKernelGGL((kv4_attn_kernel<4>), dim3((unsigned)grid), dim3(256), 0, stream, a);
   if (a.splits > 1)
-    hipLaunchKernelGGL(kv4_combine_kernel, dim3((unsigned)(a.tokens * a.group * a.nkv)),
-                       dim3(kCombine * kKvHeadDim), 0, stream, a, cut.waves());
+    hipLaunchKernelGGL(kv4_combine_kernel, dim3((unsigned)cols), dim3(kCombine * kKvHeadDim), 0,
+                       stream, a, cut.waves());
   return hip_status(hipGetLastError());
 }
 

@@ -429,7 +429,9 @@ int launch_prompt_tiles(Kv4AttnArgs a, void* workspace, hipStream_t stream) {
   const Plan p = plan_for(a.tokens, a.start, a.nkv, a.group);
   const int64_t expand = a.nkv * p.blocks, grid = p.tiles * a.nkv * p.splits;
   const int64_t cols = (int64_t)a.tokens * a.group * a.nkv;
-  if (expand > INT32_MAX || grid > INT32_MAX || cols > INT32_MAX) return DIP_ERR_SHAPE;
+  if (!launch_fits(expand, 256) || !launch_fits(grid, kPromptWaves * 64) || cols > INT32_MAX ||
+      !launch_fits((cols + 3) / 4, 256))
+    return DIP_ERR_SHAPE;
   char* w = static_cast<char*>(workspace);
   uint4* work = reinterpret_cast<uint4*>(w);
   uint32_t* bad = reinterpret_cast<uint32_t*>(w + p.work);

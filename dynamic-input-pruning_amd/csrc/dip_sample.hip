@@ -1063,7 +1063,7 @@ extern "C" int dip_sample(const void* logits, int dtype, int64_t rows, int64_t v
                           double top_p, double min_p, int64_t* token, float* prob,
                           void* workspace, size_t ws_bytes, void* stream) {
   if (dtype != DIP_BF16 && dtype != DIP_F16 && dtype != DIP_F32) return DIP_ERR_UNSUPPORTED;
-  if (rows < 0 || rows > (1 << 22) || vocab <= 0 || vocab > (1 << 30) || row_stride < 0)
+  if (rows < 0 || !launch_fits(rows, 1024) || vocab <= 0 || vocab > (1 << 30) || row_stride < 0)
     return DIP_ERR_SHAPE;
   if (!(temperature >= 0) || temperature > 1e300 || top_k < 0 || !(top_p > 0 && top_p <= 1) ||
       !(min_p >= 0 && min_p <= 1))

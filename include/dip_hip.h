@@ -710,9 +710,10 @@ int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache, const int
  * is +inf, its equals alone count.  A weight is a whole number of 2^-shift, off by
  * 4e-10 of itself beyond that, with shift 44 at 150000 tokens (51 at 2048 and fewer,
  * one less for every doubling): sums are exact, and a weight below half a step is 0
- * and never drawn.  Temperatures above 0 are taken between 1e-30 and 1e30.  temperature in [0, 1e300], top_k >= 0, top_p in (0, 1], min_p in [0, 1]
- * (else DIP_ERR_ARG).  The workspace needs no clearing; calls that may run at once
- * need one each.  The reference decodes greedily (gen_utils.py:40-46) and has no
+ * and never drawn.  temperature in [0, 1e300], taken between 1e-30 and 1e30 where it
+ * is not 0, top_k >= 0, top_p in (0, 1], min_p in [0, 1] (else DIP_ERR_ARG).  Fewer
+ * than 2^22 rows, of 2^30 logits at most.  The workspace needs no clearing; calls
+ * that may run at once need one each.  The reference decodes greedily (gen_utils.py:40-46) and has no
  * counterpart.
  */
 enum { DIP_BF16 = 0, DIP_F16 = 1, DIP_F32 = 2 };

@@ -49,6 +49,20 @@ def test_read(p):
     assert L.dip_kv4_read(p, p, p, None, None, 64, 0, 2, 128, 64, None) == 0
 
 
+def test_launches_of_two_to_the_32_threads(p):
+    """HIP takes none of these: refused as too large, not passed on."""
+    L = K.lib
+    big = 1 << 30
+    assert _write(p, nkv=8, max_len=big, tokens=1 << 26) == -2
+    assert L.dip_kv4_read(p, p, p, p, p, 0, big, 1, 128, big, None) == -2
+    assert L.dip_qk_norm_rope_kv4_rows(p, p, p, p, p, 0, p, p, p, p, 1 << 23, 64, 8, 128, big, 1e-6,
+                                       None) == -2
+    assert L.dip_sample(p, 2, 1 << 22, 5000, 5000, p, 1.0, 0, 1.0, 0.0, p, p, p, 1 << 62,
+                        None) == -2
+    n = L.dip_kv4_prompt_attention_workspace_size(big, 0, 64, 8, 128)
+    assert L.dip_kv4_prompt_attention(p, p, p, p, 0, p, big, 64, 8, 128, big, 0.1, p, n, None) == -2
+
+
 def test_norm_rope(p):
     L = K.lib
     one = lambda pos=1, hd=128, ml=64, eps=1e-6, nh=4: L.dip_qk_norm_rope_kv4(
