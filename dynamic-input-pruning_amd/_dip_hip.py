@@ -15,7 +15,6 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
 import os
 import threading
 from pathlib import Path
@@ -1118,8 +1117,8 @@ _LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def check_sampling(temperature: float, top_k: int, top_p: float, min_p: float) -> None:
     """Raise where sample would."""
-    if not (math.isfinite(temperature) and temperature >= 0):
-        raise RuntimeError(f"temperature must be finite and >= 0, got {temperature}")
+    if not 0 <= temperature <= 1e300:
+        raise RuntimeError(f"temperature must be in [0, 1e300], got {temperature}")
     if top_k < 0 or int(top_k) != top_k:
         raise RuntimeError(f"top_k must be a whole number >= 0, got {top_k}")
     if not 0 < top_p <= 1:

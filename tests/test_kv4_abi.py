@@ -117,3 +117,14 @@ def test_sampling_settings(args):
     K.check_sampling(**ok)
     with pytest.raises(RuntimeError):
         K.check_sampling(**{**ok, **args})
+
+
+@pytest.mark.parametrize("temperature", [math.nan, 1.1e300, -1e-300])
+def test_sampling_temperature_is_the_librarys(p, temperature):
+    """check_sampling refuses what the library does: generate asks it before it runs the
+    prompt."""
+    assert K.lib.dip_sample(p, 0, 1, 8, 8, p, temperature, 0, 1.0, 0.0, p, p, p, 1 << 30,
+                            None) == -6
+    with pytest.raises(RuntimeError):
+        K.check_sampling(temperature, 0, 1.0, 0.0)
+    K.check_sampling(1e300, 0, 1.0, 0.0)
