@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 import os
 import threading
 from pathlib import Path
@@ -1119,7 +1120,7 @@ def check_sampling(temperature: float, top_k: int, top_p: float, min_p: float) -
     """Raise where sample would."""
     if not 0 <= temperature <= 1e300:
         raise RuntimeError(f"temperature must be in [0, 1e300], got {temperature}")
-    if top_k < 0 or int(top_k) != top_k:
+    if not math.isfinite(top_k) or top_k < 0 or int(top_k) != top_k:
         raise RuntimeError(f"top_k must be a whole number >= 0, got {top_k}")
     if not 0 < top_p <= 1:
         raise RuntimeError(f"top_p must be in (0, 1], got {top_p}")
@@ -1166,7 +1167,7 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
         ws_p, nbytes, ws = _scratch(lib.dip_sample_workspace_size(rows, vocab), ws, dev,
                                     "sampling")
         _check(lib.dip_sample(logits.data_ptr(), kind, rows, vocab, logits.stride(0),
-                              u.data_ptr(), temperature, int(top_k), top_p, min_p,
+                              u.data_ptr(), temperature, min(int(top_k), vocab), top_p, min_p,
                               token.data_ptr(), prob.data_ptr(), ws_p, nbytes, _stream(dev)),
                "dip_sample")
     return token, prob

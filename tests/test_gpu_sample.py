@@ -166,3 +166,13 @@ def test_refusals():
             f()
     token, prob = K.sample(x[:0], u[:0])
     assert token.numel() == prob.numel() == 0
+
+
+def test_top_k_past_the_vocabulary():
+    """Numbers past 64 bits keep all tokens, as any past the vocabulary do."""
+    import _dip_hip as K
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x, u = torch.randn(8, 300, device="cuda", generator=g), torch.rand(8, device="cuda", generator=g)
+    want, _ = K.sample(x, u)
+    for k in (300, 301, 2 ** 63, 2 ** 64 + 1):
+        assert torch.equal(K.sample(x, u, top_k=k)[0], want), k

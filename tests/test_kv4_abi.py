@@ -128,3 +128,9 @@ def test_sampling_temperature_is_the_librarys(p, temperature):
     with pytest.raises(RuntimeError):
         K.check_sampling(temperature, 0, 1.0, 0.0)
     K.check_sampling(1e300, 0, 1.0, 0.0)
+
+
+@pytest.mark.parametrize("top_k", [math.inf, math.nan])
+def test_sampling_refuses_a_top_k_without_end(top_k):
+    with pytest.raises(RuntimeError):
+        K.check_sampling(1.0, top_k, 1.0, 0.0)
