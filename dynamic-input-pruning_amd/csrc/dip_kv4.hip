@@ -153,15 +153,18 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv4_write_kernel(Kv4WriteArg
       ss = fma(v, v, ss);
     }
     double r = rsqrt64(fma(sum16_64(ss), 1.0 / kKvHeadDim, (double)a.eps));
-    // (without an eps, subnormal numbers alone take r past fp32's range)
-    const float up = r > 0x1p100 ? 0x1p64f : 1.f;
-    r = r > 0x1p100 ? r * 0x1p-64 : r;
+    if (__builtin_expect(__any(r > 0x1p100), 0)) {
+      // without an eps, subnormal numbers alone take r past fp32's range
+      const float up = r > 0x1p100 ? 0x1p64f : 1.f;
+      r = r > 0x1p100 ? r * 0x1p-64 : r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = pack(lo(x[e]) * up, hi(x[e]) * up);
+    }
     const float r0 = (float)r, r1 = (float)(r - (double)r0);
     uint32_t y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float u = lo(x[e]) * up, v = hi(x[e]) * up;
-      const uint32_t n = pack(fmaf(u, r0, u * r1), fmaf(v, r0, v * r1));
+      const uint32_t n = pack(fmaf(lo(x[e]), r0, lo(x[e]) * r1), fmaf(hi(x[e]), r0, hi(x[e]) * r1));
       y[e] = pack(lo(w[e]) * lo(n), hi(w[e]) * hi(n));
     }
     // rotate_half: dims [0, 64) take -y[d + 64], dims [64, 128) take y[d - 64]
