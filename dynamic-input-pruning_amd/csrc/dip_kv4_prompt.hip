@@ -125,11 +125,11 @@ typedef const __attribute__((address_space(1))) void global_void;
 //     l ^ 32 share a column);
 //   out^T += V^T P^T, the weights rounded to bf16 in place: they are the operand
 //     as they lie.  (Off by 2^-8 of itself at most, as any bf16 weight is.)
-// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 300 to 335 us, 0.82
-// to 0.92 PFLOP/s, where a large product of matrices reaches 1.15 to 1.37.  The MFMAs
-// are busy 49 % of the time and the VALU, the softmax mostly, 56 %; without the fetch
-// it took 240 us, without the exponentials 336, without the second product 290 (of
-// 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
+// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 294 us a call, the
+// expansion's 8 with it, 0.94 PFLOP/s, where a large product of matrices reaches 1.15
+// to 1.37 (a trace of 30 calls alone has this launch at 297 to 334).  The MFMAs are busy
+// 49 % of the time and the VALU, the softmax mostly, 56 %; without the fetch it took 240
+// us, without the exponentials 336, without the second product 290 (of 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
 // buffers 353; rows through registers into LDS 493; 32 rows to a step and three
 // workgroups to a CU 340 to 346.)
 template <bool kSplit>

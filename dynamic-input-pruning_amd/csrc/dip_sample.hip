@@ -989,11 +989,14 @@ __global__ __launch_bounds__(kN) void sample_row_kernel(SampleArgs a) {
 }
 
 // Which rows are drawn in one launch: those of up to kOneLaunch pieces, and up to
-// the most that the launch takes where there are many rows or nothing to count (a
-// workgroup alone takes longer over a long row's histogram than slices do: one row
-// of 32003 bf16 logits, top-k 20, 32 us for 23; 250 such rows 35 for 51; without a
-// filter 17 for 17 and 18 for 28).  256 threads while they have two pieces each at
-// most, 1024 beyond (4000 bf16 logits 15 and 17 us, 8000 20 and 18).
+// the most that the launch takes where there are many rows or nothing to count: a
+// workgroup alone takes longer over a long row's histogram than slices do, and slices
+// are more work.  Rows of 32003 bf16 logits in one launch and in slices, us, top-k 20
+// and top-p 0.9: 1 row 31 for 21, 37 for 24; 48 rows 32 for 32, 39 for 33; 64 rows 32
+// for 35, 39 for 35; 96 rows 32 for 41, 39 for 41; 256 rows 33 for 48, 40 for 51.  (Of
+// 20001 they cross at 48 rows, of 9001 fp32 logits from the first.)  Without a filter
+// 17 for 17 and, of 250 rows, 18 for 28.  256 threads while they have two pieces each
+// at most, 1024 beyond (4000 bf16 logits 15 and 17 us, 8000 20 and 18).
 constexpr int64_t kSmallRow = 512;
 constexpr int64_t kOneLaunch = 2048;
 constexpr int64_t kMostPieces = 1024 * kRowPieces;

@@ -18,9 +18,9 @@ host: embedding, per layer RMSNorm -> q/k/v projections (int4 GEMV)
 -> q/k RMSNorm -> rotary embedding from a precomputed table -> cache write
 at the device-side position -> attention over the static cache with a
 position mask -> o projection -> RMSNorm -> DIP MLP, then the final norm,
-lm_head and argmax.  With ``use_graph`` the step up to the final norm (and
+lm_head and the token's choice.  With ``use_graph`` the step up to the final norm (and
 the position update) is captured once in a HIP graph and replayed per token;
-lm_head and argmax run after each replay on the same stream.
+these two run after each replay on the same stream.
 The step uses the model's own modules, so the decode math is the HF model's
 (transformers' Qwen3DecoderLayer / Qwen3Attention forward).
 """
@@ -617,7 +617,8 @@ class DIPDecoder:
     @torch.no_grad()
     def step(self) -> torch.Tensor:
         """Decode the token in `self.tok` at position `self.pos`; afterwards
-        `self.tok` holds the argmax and `self.pos` has advanced by one.
+        `self.tok` holds the argmax (within a `generate` that draws its tokens,
+        the one drawn) and `self.pos` has advanced by one.
         Returns the logits."""
         if not self.use_graph or self.graph is None:
             h = self._body()
@@ -641,8 +642,9 @@ class DIPDecoder:
     def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
         """Run the prompt [1, P] through the model (with the fused kernels
         where they serve, else the HF forward, whose key/value cache is copied
-        into the static cache), set `tok` to the argmax of the last logits and
-        `pos` to P.  Returns the last logits."""
+        into the static cache), set `tok` to the argmax of the last logits (or
+        the token drawn from them, as in step) and `pos` to P.  Returns the last
+        logits."""
         from transformers import DynamicCache
         ids = input_ids.to(self.device).view(1, -1)
         plen = ids.shape[1]
