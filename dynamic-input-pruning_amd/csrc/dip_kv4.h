@@ -55,10 +55,10 @@ DIP_DEV int kv4_value_word(int d, int c) {
 DIP_DEV int kv4_row_quarter(int r) { return (r >> 2) & 3; }
 DIP_DEV int kv4_row_elem(int r) { return 4 * (r >> 4) + (r & 3); }
 
-// One word as an MFMA operand of 8 bf16 values (1.5 + q / 16) * 2^-kDown (exact).
-template <int kDown = 0>
+// One word as an MFMA operand of 8 bf16 values (1.5 + q / 16) * 2^-kLower (exact).
+template <int kLower = 0>
 DIP_DEV bf16x8_t kv4_biased(uint32_t w) {
-  constexpr uint32_t kFlip = kPairMagicFlip - kDown * 0x00800080u;
+  constexpr uint32_t kFlip = kPairMagicFlip - kLower * 0x00800080u;
   u32x4_t r;
   r.x = (w & kPairMask) ^ kFlip;
   r.y = ((w >> 4) & kPairMask) ^ kFlip;
@@ -69,8 +69,8 @@ DIP_DEV bf16x8_t kv4_biased(uint32_t w) {
 
 // Keys are taken 2^-8 lower, so that the 1.5 times 32 of bf16's largest queries stays
 // finite.
-constexpr int kKeyDown = 8;
-constexpr float kKeyUnit = 1.f / (1 << kKeyDown);
+constexpr int kKeyLower = 8;
+constexpr float kKeyUnit = 1.f / (1 << kKeyLower);
 
 // Nibble at `shift` as a signed number.
 DIP_DEV int kv4_nibble(uint32_t w, int shift) {

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
       for (int g = 0; g < kKvGroups; ++g) {
         const floatx4 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            kv4_biased<kKeyDown>(w[g]), bq[g], floatx4{qs[g], qs[g], qs[g], qs[g]}, 0, 0, 0);
+            kv4_biased<kKeyLower>(w[g]), bq[g], floatx4{qs[g], qs[g], qs[g], qs[g]}, 0, 0, 0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const uint32_t z = g < 2 ? sw[t][r].x : sw[t][r].y;
