@@ -108,6 +108,17 @@ _SIGS = {
     "dip_kv4_prompt_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64], _sz),
     "dip_kv4_prompt_attention": ([_p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
                                   ctypes.c_float, _p, _sz, _p], _i32),
+    "dip_kv8_write": ([_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _p,
+                       _i64, _i64, _i64, _i64, _p], _i32),
+    "dip_kv8_read": ([_p, _p, _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _p], _i32),
+    "dip_qk_norm_rope_kv8": ([_p, _p, _p, _p, _p, _i64, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64,
+                              _i64, _i64, _i64, _i64, ctypes.c_float, _p], _i32),
+    "dip_kv8_decode_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64], _sz),
+    "dip_kv8_decode_attention": ([_p, _p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64,
+                                  _i64, ctypes.c_float, _p, _sz, _p], _i32),
+    "dip_kv8_prompt_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64], _sz),
+    "dip_kv8_prompt_attention": ([_p, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64,
+                                  ctypes.c_float, _p, _sz, _p], _i32),
     "dip_sample_workspace_size": ([_i64, _i64], _sz),
     "dip_sample": ([_p, _i32, _i64, _i64, _i64, _p, ctypes.c_double, _i64, ctypes.c_double,
                     ctypes.c_double, _p, _p, _p, _sz, _p], _i32),
@@ -118,7 +129,7 @@ _SIGS = {
 # The argument lists above follow this version of include/dip_hip.h
 # (DIP_VERSION); a library built from another one would be called with
 # shifted arguments, or lack an entry point, so it is refused here.
-ABI_VERSION = 306
+ABI_VERSION = 307
 if lib.dip_version() != ABI_VERSION:
     raise ImportError(f"{LIB_PATH} reports ABI version {lib.dip_version()}, these bindings "
                       f"are written for {ABI_VERSION}; rebuild the library")
@@ -1110,6 +1121,226 @@ def kv4_prompt_attention(q, cache: KV4Cache, start: int, out, scale: float, ws=N
                                             cache.scales.data_ptr(), start, out_p, tokens, nh,
                                             nkv, 128, max_len, scale, ws_p, nbytes, _stream(dev)),
                "dip_kv4_prompt_attention")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# the paged 8-bit key/value cache of several sequences, and its attention
+# ---------------------------------------------------------------------------
+KV8_PAGE = 64  # positions of a page
+
+
+class KV8Cache:
+    """A paged 8-bit key/value cache (kv8_cache makes one): one layer's arrays, or with
+    a leading dimension every layer's, of which ``layer(i)`` is one.
+
+      k       uint8 [pages, n_kv_heads, 64, 128]   e4m3 numbers
+      v       uint8 [pages, n_kv_heads, 128, 64]   e4m3 numbers, rows in the kernels' order
+      scales  fp32  [pages, n_kv_heads, 2]         powers of two: the keys', the values'
+
+    A sequence's row of an int32 table (on the device) has the numbers of its pages of
+    64 positions each, in their order; a number outside [0, pages) is no page.  Which
+    page is whose is the caller's to keep.  Zero the arrays of a page, or write it from
+    its first row, before it is read.  The arrays are checked here, once, so that a call
+    need not."""
+
+    __slots__ = ("k", "v", "scales", "device", "n_kv_heads", "pages", "one_layer")
+
+    def __init__(self, k, v, scales):
+        dev = _dev(k, v, scales)
+        if k.dim() not in (4, 5) or not k.numel():
+            raise RuntimeError("cache arrays must be as kv8_cache makes them")
+        *lead, pages, nkv, _, _ = k.shape
+        for t, dt, shape in ((k, torch.uint8, (KV8_PAGE, 128)), (v, torch.uint8, (128, KV8_PAGE)),
+                             (scales, torch.float32, (2,))):
+            if t.dtype != dt or tuple(t.shape) != (*lead, pages, nkv, *shape) \
+                    or not t.is_contiguous() or t.data_ptr() % (8 if t is scales else 16):
+                raise RuntimeError("cache arrays must be as kv8_cache makes them")
+        self.k, self.v, self.scales = k, v, scales
+        self.device, self.n_kv_heads, self.pages = dev, nkv, pages
+        self.one_layer = not lead
+
+    def layer(self, i: int) -> "KV8Cache":
+        return KV8Cache(self.k[i], self.v[i], self.scales[i])
+
+    def __iter__(self):
+        return iter((self.k, self.v, self.scales))
+
+
+def kv8_cache(n_kv_heads: int, pages: int, device="cuda", layers=None) -> KV8Cache:
+    """An empty (zero) paged 8-bit cache, for one layer, or for `layers` of them."""
+    if n_kv_heads < 1 or pages < 1 or (layers is not None and layers < 1):
+        raise RuntimeError("a cache needs at least one head, page and layer")
+    lead = (pages, n_kv_heads) if layers is None else (layers, pages, n_kv_heads)
+    return KV8Cache(torch.zeros(*lead, KV8_PAGE, 128, dtype=torch.uint8, device=device),
+                    torch.zeros(*lead, 128, KV8_PAGE, dtype=torch.uint8, device=device),
+                    torch.zeros(*lead, 2, dtype=torch.float32, device=device))
+
+
+def _kv8(cache: KV8Cache, table, *ts):
+    """(device, table, its width) of a call over one layer's cache; the tensors must be
+    on the cache's device."""
+    if not isinstance(cache, KV8Cache) or not cache.one_layer:
+        raise RuntimeError("cache must be one layer's KV8Cache")
+    dev = cache.device
+    for t in (table, *ts):
+        if t.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
+    if table.dtype is not torch.int32 or table.dim() not in (1, 2) or not table.shape[-1]:
+        raise RuntimeError("table must be int32 [seqs, pages of a sequence]")
+    return dev, table.contiguous(), table.shape[-1]
+
+
+def _positions(pos, table) -> torch.Tensor:
+    if table.dim() != 2 or pos.dtype is not torch.int64 or pos.numel() != table.shape[0]:
+        raise RuntimeError("table must be [seqs, pages], pos int64 with a position for each")
+    return pos.contiguous()
+
+
+def kv8_write(k, v, cache: KV8Cache, table, pos) -> None:
+    """Round k and v (bf16 [seqs, tokens, n_kv_heads, 128], any strides of the first
+    three dimensions) into one layer's cache, at the positions from pos (int64 [seqs]) on
+    of the sequences whose pages table (int32 [seqs, ..]) has.  A negative position
+    leaves a sequence out; no two may write to one page.  Rows of a page behind the last
+    written no longer stand for anything."""
+    dev, table, width = _kv8(cache, table, k, v, pos)
+    pos, nkv = _positions(pos, table), cache.n_kv_heads
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != table.shape[0] \
+            or tuple(k.shape[2:]) != (nkv, 128) \
+            or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise RuntimeError(f"k and v must be bf16 [{table.shape[0]}, tokens, {nkv}, 128]")
+    if k.numel() == 0:
+        return
+    # a last dimension that is not dense, odd strides and pointers: a dense copy
+    k, v = (t if t.stride(3) == 1 and not (t.stride(0) | t.stride(1) | t.stride(2)) & 1
+            and not t.data_ptr() & 3 else t.clone(memory_format=torch.contiguous_format)
+            for t in (k, v))
+    with _on(dev):
+        _check(lib.dip_kv8_write(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+                                 cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
+                                 cache.pages, table.data_ptr(), width, pos.data_ptr(), k.shape[0],
+                                 k.shape[1], nkv, 128, _stream(dev)), "dip_kv8_write")
+
+
+def kv8_read(cache: KV8Cache, table, pos, tokens: int):
+    """(k, v) bf16 [seqs, tokens, n_kv_heads, 128]: what the rows of the positions from
+    pos (int64 [seqs]) on stand for in one layer's cache, exactly; 0 where a sequence has
+    no page, or pos is negative."""
+    dev, table, width = _kv8(cache, table, pos)
+    pos, nkv, tokens = _positions(pos, table), cache.n_kv_heads, int(tokens)
+    if tokens < 0:
+        raise RuntimeError("tokens must not be negative")
+    k, v = torch.empty(2, table.shape[0], tokens, nkv, 128, dtype=torch.bfloat16,
+                       device=dev).unbind(0)
+    if k.numel() == 0:
+        return k, v
+    with _on(dev):
+        _check(lib.dip_kv8_read(cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
+                                cache.pages, table.data_ptr(), width, pos.data_ptr(),
+                                k.data_ptr(), v.data_ptr(), table.shape[0], tokens, nkv, 128,
+                                _stream(dev)), "dip_kv8_read")
+    return k, v
+
+
+def qk_norm_rope_kv8(qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out, cache: KV8Cache, table,
+                     n_heads: int, n_kv_heads: int, eps: float):
+    """qk_norm_rope_cache for the tokens of several sequences, into their pages of one
+    layer's 8-bit cache: qkv [seqs, tokens, ..], the first token of each at the position
+    in pos (int64 [seqs], on the device), q to q_out [seqs, tokens, n_heads * 128].  A
+    token at a position that the tables of pages or of cos and sin do not have is left
+    out, as is a sequence whose position is negative: its row of q_out stays as it is."""
+    dev, table, width = _kv8(cache, table, qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out)
+    pos, nkv = _positions(pos, table), cache.n_kv_heads
+    if n_kv_heads != nkv or n_heads < 1:
+        raise RuntimeError(f"the cache has {nkv} kv heads, the call {n_kv_heads}")
+    if qkv.dim() != 3 or qkv.shape[0] != table.shape[0]:
+        raise RuntimeError(f"qkv must be [{table.shape[0]}, tokens, ..]")
+    rows = cos.numel() // 128
+    if cos.shape != sin.shape or cos.shape[-1] != 128:
+        raise RuntimeError("cos and sin must be tables of as many rows of 128 values")
+    seqs, tokens = qkv.shape[:2]
+    ptrs = (_dense(qkv, seqs * tokens * (n_heads + 2 * nkv) * 128, "qkv"),
+            _dense(q_norm_w, 128, "q_norm_w"), _dense(k_norm_w, 128, "k_norm_w"),
+            _dense(cos, rows * 128, "cos"), _dense(sin, rows * 128, "sin"))
+    q_p = _dense(q_out, seqs * tokens * n_heads * 128, "q_out")
+    if seqs * tokens == 0:
+        return q_out
+    with _on(dev):
+        _check(lib.dip_qk_norm_rope_kv8(*ptrs, rows, pos.data_ptr(), q_p, cache.k.data_ptr(),
+                                        cache.v.data_ptr(), cache.scales.data_ptr(), cache.pages,
+                                        table.data_ptr(), width, seqs, tokens, n_heads, nkv, 128,
+                                        eps, _stream(dev)), "dip_qk_norm_rope_kv8")
+    return q_out
+
+
+def kv8_decode_attention_workspace_bytes(seqs: int, tokens: int, n_heads: int, n_kv_heads: int,
+                                         table_width: int) -> int:
+    return lib.dip_kv8_decode_attention_workspace_size(seqs, tokens, n_heads, n_kv_heads, 128,
+                                                       table_width)
+
+
+def kv8_decode_attention(q, cache: KV8Cache, table, pos, out, scale: float, ws=None):
+    """Grouped-query attention of one or a few tokens of each of several sequences: q
+    [seqs, tokens, n_heads * 128], token t of sequence s over rows 0 .. pos[s] + t of its
+    pages in one layer's 8-bit cache -> out (new if None).  A sequence whose position is
+    negative gives zeros.  The work is cut by the table's width: one no wider than the
+    longest sequence's pages is the fastest.  ws: a workspace of
+    kv8_decode_attention_workspace_bytes, one for each call that may run at once (None:
+    the call's own)."""
+    dev, table, width = _kv8(cache, table, q, pos)
+    pos, nkv, n = _positions(pos, table), cache.n_kv_heads, q.numel()
+    if q.dim() != 3 or q.shape[0] != table.shape[0] or q.shape[2] % (128 * nkv) or not q.shape[2]:
+        raise RuntimeError(f"q must be [{table.shape[0]}, tokens, a multiple of {nkv} heads of "
+                           "128 values]")
+    seqs, tokens, nh = q.shape[0], q.shape[1], q.shape[2] // 128
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.device != dev:
+        raise RuntimeError("out must be on q's device")
+    q_p, out_p = _dense(q, n, "q"), _dense(out, n, "out")
+    if n == 0:
+        return out
+    with _on(dev):
+        ws_p, nbytes, ws = _scratch(
+            lib.dip_kv8_decode_attention_workspace_size(seqs, tokens, nh, nkv, 128, width), ws,
+            dev, "attention")
+        _check(lib.dip_kv8_decode_attention(q_p, cache.k.data_ptr(), cache.v.data_ptr(),
+                                            cache.scales.data_ptr(), cache.pages,
+                                            table.data_ptr(), width, pos.data_ptr(), out_p, seqs,
+                                            tokens, nh, nkv, 128, scale, ws_p, nbytes,
+                                            _stream(dev)), "dip_kv8_decode_attention")
+    return out
+
+
+def kv8_prompt_attention(q, cache: KV8Cache, table, start: int, out, scale: float, ws=None):
+    """Grouped-query attention of a prompt's tokens (q [tokens, n_heads * 128] at
+    positions start ..), token t over rows 0 .. start + t of the pages in table (int32
+    [pages]) of one layer's 8-bit cache -> out (new if None).  ws: as in
+    kv8_decode_attention; its size depends on start and the number of tokens."""
+    dev, table, width = _kv8(cache, table, q)
+    nkv, n = cache.n_kv_heads, q.numel()
+    if table.dim() != 1:
+        raise RuntimeError("table must be one sequence's, int32 [pages]")
+    if q.dim() != 2 or q.shape[1] % (128 * nkv) or not q.shape[1]:
+        raise RuntimeError(f"q must be [tokens, a multiple of {nkv} heads of 128 values]")
+    nh = q.shape[1] // 128
+    start, tokens = _rows_in(start, q.shape[0], width * KV8_PAGE)
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.device != dev:
+        raise RuntimeError("out must be on q's device")
+    q_p, out_p = _dense(q, n, "q"), _dense(out, n, "out")
+    if tokens == 0:
+        return out
+    with _on(dev):
+        ws_p, nbytes, ws = _scratch(
+            lib.dip_kv8_prompt_attention_workspace_size(tokens, start, nh, nkv, 128), ws, dev,
+            "attention")
+        _check(lib.dip_kv8_prompt_attention(q_p, cache.k.data_ptr(), cache.v.data_ptr(),
+                                            cache.scales.data_ptr(), cache.pages,
+                                            table.data_ptr(), width, start, out_p, tokens, nh,
+                                            nkv, 128, scale, ws_p, nbytes, _stream(dev)),
+               "dip_kv8_prompt_attention")
     return out
 
 

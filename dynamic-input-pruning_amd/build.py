@@ -43,7 +43,7 @@ COMMON = [
 # instructions use (by default they move through the accumulator half of the
 # register file, 130 of a cache block's 630 instructions).
 _VGPR_SUMS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-EXTRA = {"dip_kv4_attn": _VGPR_SUMS, "dip_kv4_prompt": _VGPR_SUMS}
+EXTRA = {"dip_kv4_attn": _VGPR_SUMS, "dip_kv4_prompt": _VGPR_SUMS, "dip_kv8_attn": _VGPR_SUMS}
 
 
 def _run(cmd):

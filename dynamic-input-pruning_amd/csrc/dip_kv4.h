@@ -29,20 +29,17 @@
 // 2 m + 1), the first pair where it lies, the others after one shift.
 #pragma once
 
-#include "dip_common.h"
+#include "dip_attn.h"
+#include "dip_head_rope.h"
 #include "dip_internal.h"
 
 namespace dip {
 
-constexpr int kKvHeadDim = 128;
 constexpr int kKvGroups = 4;           // scale groups of a row
 constexpr int kKvKeyBytes = 64;        // a row's packed keys
 constexpr int kKvScaleVals = 8;        // a row's scales (keys, then values)
 constexpr int kKvBlock = 32;           // rows of a value block
 constexpr int kKvBlockWords = 512;
-
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 // Element j of a word, as a shift; the last one's nibble wraps around.
 DIP_DEV int kv4_shift(int j) { return 4 * ((j >> 1) + 4 * (j & 1)) + 3; }
@@ -121,36 +118,13 @@ struct Kv4AttnArgs {
   float scale;
 };
 
-constexpr int kKvPart = 2 + kKvHeadDim;  // max, sum, value sum of one column
-constexpr float kLog2e = 1.44269504088896340736f;
-
-// The attention kernels' weights are 2^(score - base), against a base that follows the
-// running maximum: it is raised to kDown above a new one that passes the old by more
-// than kSlack (powers of 2; score in them too), so that the sums are seldom taken
-// against a new base.  Weights then lie below 2^(kSlack - kDown), and the sums of 2^18
-// of them times the largest values within fp32, where with weights of about 1 two
-// rows of large values were beyond it.  kDown cancels in the division.  (At the small
-// end a weight of 2^-n of the largest rounds coarser in value groups of a scale below
-// 2^(n - 100), the least that scales are.)
-constexpr float kSlack = 8.f, kDown = 26.f;
-
-// 2^x; results below the normal range are 0.
-DIP_DEV float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
 // Whether the cache has the rows first .. first + tokens - 1 (tokens >= 0), for any
 // first: a position on the device may hold the type's ends.
 __host__ DIP_DEV bool rows_in_cache(int64_t first, int tokens, int max_len) {
   return first >= 0 && first <= (int64_t)max_len - tokens;
 }
 
-// Cache rows that the token at position pos attends: 0 .. pos.
-DIP_DEV int rows_at(int64_t pos, int max_len) {
-  return pos < 0 ? 0 : (pos < (int64_t)max_len ? (int)pos + 1 : max_len);
-}
-
 // A prompt's attention over the cache expanded to bf16 (dip_kv4_prompt.hip).
-size_t prompt_tiles_workspace(int64_t tokens, int64_t start, int64_t nkv, int64_t group);
-int64_t prompt_tiles_us100(int64_t tokens, int64_t start, int64_t nkv, int64_t group);
-int launch_prompt_tiles(Kv4AttnArgs a, void* workspace, hipStream_t stream);
+int launch_kv4_prompt_tiles(const Kv4AttnArgs& a, void* workspace, hipStream_t stream);
 
 }  // namespace dip

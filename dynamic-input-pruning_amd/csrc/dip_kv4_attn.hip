@@ -10,7 +10,6 @@ namespace {
 
 constexpr int kCols = 16;                  // (token, query head) pairs of a tile: MFMA columns
 constexpr int kPart = kKvPart;
-constexpr int kMaxSplits = 256;
 
 // The tile's last token's rows, and the blocks of 32 rows that a wave of `waves`
 // takes of them.
@@ -269,68 +268,19 @@ __global__ __launch_bounds__(W * 64) void kv4_attn_kernel(Kv4AttnArgs a) {
   }
 }
 
-// The splits of one column added up, in a fixed order: one workgroup per (kv
-// head, column), kCombine groups of 128 threads, each of which takes every
-// kCombine-th split's value sums; its first loads are in flight while the splits'
-// weights are worked out.  (20011 rows, 64 columns: 4 us; one group of 128 threads
-// over all splits in turn 18 to 22.)
-constexpr int kCombine = 8, kAhead = 8;
-
+// The splits of a column added up: one workgroup per (kv head, column).
 __global__ __launch_bounds__(kCombine * kKvHeadDim) void kv4_combine_kernel(Kv4AttnArgs a,
                                                                             int waves) {
-  __shared__ float wgt[kMaxSplits];
-  __shared__ float red[kCombine * kKvHeadDim / 64][2];
-  __shared__ float so[kCombine][kKvHeadDim];
-  const int kvh = blockIdx.x % a.nkv, cc = blockIdx.x / a.nkv, tid = threadIdx.x;
-  const int tile = cc / kCols, cl = cc % kCols, d = tid % kKvHeadDim, p = tid / kKvHeadDim;
+  const int kvh = blockIdx.x % a.nkv, cc = blockIdx.x / a.nkv;
+  const int tile = cc / kCols, cl = cc % kCols;
   const int64_t first = a.pos ? *a.pos : a.start;
   const int rows = tile_rows(a, first, tile);
   const int per = waves * blocks_per_wave(rows, a.splits * waves);  // blocks of a split
   const int ns = ((rows + kKvBlock - 1) / kKvBlock + per - 1) / per;
-  const size_t o = ((size_t)(cc / a.group) * a.nkv * a.group + kvh * a.group + cc % a.group) *
-                   kKvHeadDim;
-  if (ns == 0) {  // no rows
-    if (tid < kKvHeadDim) a.out[o + tid] = 0;
-    return;
-  }
-  const float* base = a.part + ((size_t)(tile * a.nkv + kvh) * a.splits * kCols + cl) * kPart;
-  const size_t stride = (size_t)kCols * kPart;
-  const float ms = tid < ns ? base[tid * stride] : -INFINITY;
-  const float ls = tid < ns ? base[tid * stride + 1] : 0.f;
-  float v[kAhead];
-#pragma unroll
-  for (int u = 0; u < kAhead; ++u) v[u] = base[min(p + kCombine * u, ns - 1) * stride + 2 + d];
-  float mx = group_max<64>(ms);
-  if ((tid & 63) == 0) red[tid >> 6][0] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kCombine * kKvHeadDim / 64; ++w) mx = fmaxf(mx, red[w][0]);
-  // (a split without a score above -inf has sums of 0, or NaN, which must count)
-  const float f = tid >= ns ? 0.f : ms == -INFINITY ? 1.f : fast_exp2(ms - mx);
-  if (tid < kMaxSplits) wgt[tid] = f;
-  const float part = group_sum<64>(f * ls);
-  if ((tid & 63) == 0) red[tid >> 6][1] = part;
-  __syncthreads();
-  float acc = 0.f;
-  for (int s0 = p; s0 < ns; s0 += kCombine * kAhead) {
-    if (s0 != p) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) v[u] = base[min(s0 + kCombine * u, ns - 1) * stride + 2 + d];
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (s0 + kCombine * u < ns) acc = fmaf(wgt[s0 + kCombine * u], v[u], acc);
-  }
-  so[p][d] = acc;
-  __syncthreads();
-  if (tid < kKvHeadDim) {
-    float sum = 0.f, r = 0.f;
-#pragma unroll
-    for (int w = 0; w < kCombine * kKvHeadDim / 64; ++w) sum += red[w][1];
-#pragma unroll
-    for (int w = 0; w < kCombine; ++w) r += so[w][tid];
-    a.out[o + tid] = (uint16_t)f32_to_bf16(r / sum);
-  }
+  combine_splits(a.part + ((size_t)(tile * a.nkv + kvh) * a.splits * kCols + cl) * kPart,
+                 (size_t)kCols * kPart, ns,
+                 a.out + ((size_t)(cc / a.group) * a.nkv * a.group + kvh * a.group +
+                          cc % a.group) * kKvHeadDim);
 }
 
 // How a launch cuts its tiles' rows.  Alone, a workgroup of 8 waves takes a tile's
@@ -480,6 +430,6 @@ extern "C" int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache
   if (need && (!workspace || ws_bytes < need)) return DIP_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return DIP_ERR_ALIGN;
   if (by_tiles(tokens, start, n_kv_heads, group))
-    return launch_prompt_tiles(a, workspace, (hipStream_t)stream);
+    return launch_kv4_prompt_tiles(a, workspace, (hipStream_t)stream);
   return launch_attn(a, tiles, cut_for(tiles, n_kv_heads, start + tokens), (hipStream_t)stream);
 }

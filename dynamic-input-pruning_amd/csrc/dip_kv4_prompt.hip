@@ -1,39 +1,17 @@
-// dip_kv4_prompt.hip — a prompt's attention over the 4-bit key/value cache
-// (dip_kv4.h): the rows expanded once to bf16 in the order the matrix
-// instructions read them, then attention in tiles of 128 (token, query head)
-// columns.
-//
-// Every tile of columns reads every earlier row, so unpacking in the tiles would
-// be done tokens * group / 128 times; once costs two passes over 512 bytes per row
-// and kv head, a few per cent of the products' time from some hundred columns on
-// (4096 rows of 8 heads 8 us).
+// dip_kv4_prompt.hip — a prompt's attention over a quantised cache's rows expanded to
+// bf16 (dip_attn.h), in tiles of 128 (token, query head) columns, and the expansion of
+// the 4-bit cache (dip_kv4.h; 4096 rows of 8 heads in 8 us).
 #include "dip_kv4.h"
 
 namespace dip {
 namespace {
 
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-
-constexpr int kTileCols = 128;   // columns of a workgroup, 32 to a wave
-constexpr int kPromptWaves = 4;
-constexpr int kMinWgs = 2;
-constexpr int kStepBlocks = 2;   // blocks of 32 cache rows of a step
-constexpr int kTileRows = 32 * kStepBlocks;
-constexpr int kBlockVecs = 1024; // 16-byte pieces of an expanded block: 512 of keys, 512 of values
-
 // The largest scale of finite values: bf16's largest over 7, cut to 5 bits.  (Times 7
 // it is still a bf16 number.)
 constexpr float kMaxScale = 0x1.2p125f;
 
-// The expanded cache: per kv head and block of 32 rows
-//   keys   [16][32 rows] pieces: piece (u, row) holds dimensions 8 u .. 8 u + 7;
-//   values [2][2][128 dims] pieces: piece (c, h, d) holds dimension d of rows
-//          16 c + 4 h + 0 .. 3 and 16 c + 8 + 4 h + 0 .. 3,
-// each the order in which the lanes of a 32x32x16 MFMA take their operand.  Blocks
-// in pairs; what lies behind the cache's end is 0.  bad[kv head][block]: a byte per
-// value group, the first row of the block whose group is not finite (255: none).
-// Those values are 0 here, and a number of -8, which nobody writes, is -7: whatever
-// the rows that nobody has written hold, a weight of 0 makes 0 of it.
+// The expanded form is dip_attn.h's.  A number of -8, which nobody writes, is -7:
+// whatever the rows that nobody has written hold, a weight of 0 makes 0 of it.
 __global__ __launch_bounds__(256) void kv4_expand_kernel(
     const uint32_t* __restrict__ kc, const uint32_t* __restrict__ vc,
     const uint16_t* __restrict__ sc, uint4* __restrict__ work, uint32_t* __restrict__ bad,
@@ -102,12 +80,21 @@ __global__ __launch_bounds__(256) void kv4_expand_kernel(
   }
 }
 
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+constexpr int kTileCols = 128;   // columns of a workgroup, 32 to a wave
+constexpr int kPromptWaves = 4;
+constexpr int kMinWgs = 2;
+constexpr int kStepBlocks = 2;   // blocks of 32 cache rows of a step
+constexpr int kTileRows = 32 * kStepBlocks;
+constexpr int kGroups = kKvHeadDim / 32;  // of dimensions
+
 // The steps of 64 rows that a split takes of a tile's.
 DIP_DEV int steps_per_split(int rows, int splits) {
   const int steps = (rows + kTileRows - 1) / kTileRows;
   return (steps + splits - 1) / splits;
 }
-DIP_DEV int tile_end(const Kv4AttnArgs& a, int tile) {
+DIP_DEV int tile_end(const PromptArgs& a, int tile) {
   const int last = min((tile * kTileCols + kTileCols - 1) / a.group, a.tokens - 1);
   return (int)(a.start + last + 1);
 }
@@ -126,20 +113,20 @@ typedef const __attribute__((address_space(1))) void global_void;
 //   out^T += V^T P^T, the weights rounded to bf16 in place: they are the operand
 //     as they lie.  (Off by 2^-8 of itself at most, as any bf16 weight is.)
 // 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 294 us a call, the
-// expansion's 8 with it, 0.94 PFLOP/s, where a large product of matrices reaches 1.15
-// to 1.37 (a trace of 30 calls alone has this launch at 297 to 334).  The MFMAs are busy
-// 49 % of the time and the VALU, the softmax mostly, 56 %; without the fetch it took 240
-// us, without the exponentials 336, without the second product 290 (of 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
+// 4-bit cache's expansion of 8 with it, 0.94 PFLOP/s, where a large product of matrices
+// reaches 1.15 to 1.37 (a trace of 30 calls alone has this launch at 297 to 334).  The
+// MFMAs are busy 49 % of the time and the VALU, the softmax mostly, 56 %; without the
+// fetch it took 240 us, without the exponentials 336, without the second product 290 (of
+// 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
 // buffers 353; rows through registers into LDS 493; 32 rows to a step and three
 // workgroups to a CU 340 to 346.)
 template <bool kSplit>
-__global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
-    Kv4AttnArgs a, const uint4* work, const uint32_t* bad, int blocks, int tiles) {
+__global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void prompt_kernel(PromptArgs a) {
   __shared__ uint4 buf_a[kStepBlocks * kBlockVecs], buf_b[kStepBlocks * kBlockVecs];
-  __shared__ int bad_row[kKvGroups];
+  __shared__ int bad_row[kGroups];
   const int kvh = blockIdx.x % a.nkv, rest = blockIdx.x / a.nkv;
   const int split = kSplit ? rest % a.splits : 0;
-  const int tile = tiles - 1 - (kSplit ? rest / a.splits : rest);  // the longest first
+  const int tile = a.tiles - 1 - (kSplit ? rest / a.splits : rest);  // the longest first
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l = threadIdx.x & 63, l32 = l & 31, h = l >> 5;
   const int rows = tile_end(a, tile);
@@ -167,9 +154,9 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
       bq[k] = __builtin_bit_cast(bf16x8_t, u32x4_t{w.x, w.y, w.z, w.w});
     }
   }
-  if (threadIdx.x < kKvGroups) bad_row[threadIdx.x] = INT32_MAX;
+  if (threadIdx.x < kGroups) bad_row[threadIdx.x] = INT32_MAX;
 
-  const uint4* src = work + (size_t)kvh * blocks * kBlockVecs;
+  const uint4* src = a.work + (size_t)kvh * a.blocks * kBlockVecs;
   auto fetch = [&](uint4* buf, int t) {
 #pragma unroll
     for (int i = 0; i < kStepBlocks * kBlockVecs / 256; ++i) {
@@ -303,11 +290,11 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
   // the first row of each group of values that is not finite
   __syncthreads();
   for (int b = kStepBlocks * t0 + (int)threadIdx.x; b < kStepBlocks * t1; b += kPromptWaves * 64) {
-    const uint32_t w = bad[(size_t)kvh * blocks + b];
+    const uint32_t w = a.bad[(size_t)kvh * a.blocks + b];
     if (w == 0xFFFFFFFFu) continue;
-    for (int g = 0; g < kKvGroups; ++g)
+    for (int g = 0; g < kGroups; ++g)
       if (((w >> (8 * g)) & 255u) != 255u)
-        atomicMin(&bad_row[g], b * kKvBlock + (int)((w >> (8 * g)) & 255u));
+        atomicMin(&bad_row[g], b * kExpandRows + (int)((w >> (8 * g)) & 255u));
   }
   __syncthreads();
   den = row_pair_sum32(den);
@@ -341,7 +328,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void kv4_prompt_kernel(
 }
 
 // The splits of a column added up in their order: a wave per (kv head, column).
-__global__ __launch_bounds__(256) void kv4_prompt_combine_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256) void prompt_combine_kernel(PromptArgs a) {
   const int l = threadIdx.x & 63;
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= (int64_t)a.tokens * a.group * a.nkv) return;
@@ -425,30 +412,43 @@ int64_t prompt_tiles_us100(int64_t tokens, int64_t start, int64_t nkv, int64_t g
   return plan_for(tokens, start, nkv, group).us100;
 }
 
-int launch_prompt_tiles(Kv4AttnArgs a, void* workspace, hipStream_t stream) {
+int prompt_tiles_plan(PromptArgs& a, void* workspace) {
   const Plan p = plan_for(a.tokens, a.start, a.nkv, a.group);
-  const int64_t expand = a.nkv * p.blocks, grid = p.tiles * a.nkv * p.splits;
+  const int64_t grid = p.tiles * a.nkv * p.splits;
   const int64_t cols = (int64_t)a.tokens * a.group * a.nkv;
-  if (!launch_fits(expand, 256) || !launch_fits(grid, kPromptWaves * 64) || cols > INT32_MAX ||
-      !launch_fits((cols + 3) / 4, 256))
+  if (!launch_fits(a.nkv * p.blocks, 256) || !launch_fits(grid, kPromptWaves * 64) ||
+      cols > INT32_MAX || !launch_fits((cols + 3) / 4, 256))
     return DIP_ERR_SHAPE;
   char* w = static_cast<char*>(workspace);
-  uint4* work = reinterpret_cast<uint4*>(w);
-  uint32_t* bad = reinterpret_cast<uint32_t*>(w + p.work);
+  a.work = reinterpret_cast<uint4*>(w);
+  a.bad = reinterpret_cast<uint32_t*>(w + p.work);
   a.part = reinterpret_cast<float*>(w + p.work + p.bad);
+  a.blocks = (int)p.blocks;
+  a.tiles = (int)p.tiles;
   a.splits = p.splits;
-  hipLaunchKernelGGL(kv4_expand_kernel, dim3((unsigned)expand), dim3(256), 0, stream, a.kc, a.vc,
-                     a.sc, work, bad, a.max_len, (int)p.blocks);
-  if (p.splits > 1) {
-    hipLaunchKernelGGL((kv4_prompt_kernel<true>), dim3((unsigned)grid), dim3(kPromptWaves * 64), 0,
-                       stream, a, work, bad, (int)p.blocks, (int)p.tiles);
-    hipLaunchKernelGGL(kv4_prompt_combine_kernel, dim3((unsigned)((cols + 3) / 4)), dim3(256), 0,
+  return DIP_OK;
+}
+
+int launch_prompt_tiles(const PromptArgs& a, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.tiles * a.nkv * a.splits)), block(kPromptWaves * 64);
+  const int64_t cols = (int64_t)a.tokens * a.group * a.nkv;
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((prompt_kernel<true>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL(prompt_combine_kernel, dim3((unsigned)((cols + 3) / 4)), dim3(256), 0,
                        stream, a);
   } else {
-    hipLaunchKernelGGL((kv4_prompt_kernel<false>), dim3((unsigned)grid), dim3(kPromptWaves * 64),
-                       0, stream, a, work, bad, (int)p.blocks, (int)p.tiles);
+    hipLaunchKernelGGL((prompt_kernel<false>), grid, block, 0, stream, a);
   }
   return hip_status(hipGetLastError());
+}
+
+int launch_kv4_prompt_tiles(const Kv4AttnArgs& a, void* workspace, hipStream_t stream) {
+  PromptArgs p{a.q, a.out, a.start, a.tokens, a.nkv, a.group, a.scale};
+  if (int st = prompt_tiles_plan(p, workspace)) return st;
+  hipLaunchKernelGGL(kv4_expand_kernel, dim3((unsigned)(a.nkv * (int64_t)p.blocks)), dim3(256), 0,
+                     stream, a.kc, a.vc, a.sc, const_cast<uint4*>(p.work),
+                     const_cast<uint32_t*>(p.bad), a.max_len, p.blocks);
+  return launch_prompt_tiles(p, stream);
 }
 
 }  // namespace dip

@@ -52,7 +52,8 @@ const char* dip_status_string(int status);
  * Library version as an integer (major * 10000 + minor * 100 + patch).  The
  * minor number changes whenever an entry point's argument list changes, so
  * a binding written against this header checks dip_version() == DIP_VERSION
- * before its first call.  0.3.6 adds the 4-bit key/value cache (dip_kv4_*,
+ * before its first call.  0.3.7 adds the paged 8-bit key/value cache (dip_kv8_*,
+ * dip_qk_norm_rope_kv8).  0.3.6 adds the 4-bit key/value cache (dip_kv4_*,
  * dip_qk_norm_rope_kv4*) and dip_sample.  0.3.5 adds dip_int4_gemm_swiglu, dip_swiglu,
  * dip_dequant_t, dip_stream_rows, dip_add_rmsnorm_rows and
  * dip_qk_norm_rope_cache_rows.  0.3.4: dip_int4_gather_down_by_channel takes
@@ -64,7 +65,7 @@ const char* dip_status_string(int status);
  * down_t_sc_gm to the decode and gather-down entry points and g_len to
  * dip_ca_fused_gemv.
  */
-#define DIP_VERSION 306
+#define DIP_VERSION 307
 int dip_version(void);
 
 /* Highest row count the top-k supports (its keys are staged in LDS). */
@@ -695,6 +696,101 @@ int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache, const int
                              int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
                              int64_t head_dim, int64_t max_len, float scale, void* workspace,
                              size_t ws_bytes, void* stream);
+
+/*
+ * The paged 8-bit key/value cache, for several sequences of any lengths at once.  The
+ * reference decodes one sequence over transformers' bf16 cache and has no counterpart
+ * of these.
+ *
+ * A page holds 64 consecutive positions (rows) of one sequence, of every kv head.  The
+ * keys of a page and head share a scale s, a power of two, and so do the values; each
+ * is an e4m3 number n and stands for n * s, which is a bf16 number.  With a the largest
+ * magnitude of the rows written s is 2^(floor(log2 a) - 7) (at least 2^-100; 0 while
+ * all are 0), and n is x / s rounded to the nearest even: off by 2^-4 of x at most, or
+ * by 2^-10 s where x is below 2^-6 s.  A group of 32 dimensions of a row with an
+ * infinity or a NaN stands for NaN and does not count in a.  A layer's cache is three
+ * device arrays (the order of their bytes is csrc/dip_kv8.h's), to be zero before
+ * their first use:
+ *   k_cache   [pages, n_kv_heads, 64 * 128] bytes
+ *   v_cache   [pages, n_kv_heads, 64 * 128] bytes
+ *   kv_scales fp32 [pages, n_kv_heads, 2]
+ * 257 bytes per position and kv head, where bf16 takes 512.  table int32
+ * [seqs, table_width] (on the device): the number of the page that holds the positions
+ * 64 j .. 64 j + 63 of sequence s at [s][j].  pos int64 [seqs] (on the device): the
+ * position of a sequence's first token of the call, its others follow it.  A negative
+ * position: the sequence is left out.  A number outside [0, pages): the sequence has no
+ * such page; what would be written there is not, and its rows are taken as zeros.
+ * pages at most 2^28, table_width 2^24, head_dim 128 (else DIP_ERR_UNSUPPORTED).
+ *
+ * Writes.  Position p of a sequence goes to row p % 64 of its page; positions beyond
+ * the table's are left out.  A write that begins at row 0 of a page takes the page's
+ * scales from its own rows; one that begins behind row 0 keeps the larger of the page's
+ * scale and its own rows', and rounds the earlier rows' numbers again where that is
+ * larger than the page's was.  Rows of the page behind those written no longer stand
+ * for anything.  So two sequences may share pages that neither writes, and a sequence
+ * may go back to an earlier position and write on from there.  Two writers of one page
+ * must be ordered on a stream, and no two sequences of a call may write to one page.
+ *
+ * dip_kv8_write: k and v bf16, token t's head h of sequence s at k + s * k_seq_stride
+ * + t * k_tok_stride + h * k_head_stride (in values; even, pointers 4-byte aligned).
+ */
+int dip_kv8_write(const uint16_t* k, const uint16_t* v, int64_t k_seq_stride,
+                  int64_t k_tok_stride, int64_t k_head_stride, int64_t v_seq_stride,
+                  int64_t v_tok_stride, int64_t v_head_stride, uint8_t* k_cache,
+                  uint8_t* v_cache, float* kv_scales, int64_t pages, const int32_t* table,
+                  int64_t table_width, const int64_t* pos, int64_t seqs, int64_t tokens,
+                  int64_t n_kv_heads, int64_t head_dim, void* stream);
+
+/* k_out, v_out bf16 [seqs, tokens, n_kv_heads, head_dim]: what the rows of positions
+ * pos .. pos + tokens - 1 of each sequence stand for, exactly; 0 for positions without a
+ * page, and for a sequence whose pos is negative or beyond its table. */
+int dip_kv8_read(const uint8_t* k_cache, const uint8_t* v_cache, const float* kv_scales,
+                 int64_t pages, const int32_t* table, int64_t table_width, const int64_t* pos,
+                 uint16_t* k_out, uint16_t* v_out, int64_t seqs, int64_t tokens,
+                 int64_t n_kv_heads, int64_t head_dim, void* stream);
+
+/* dip_qk_norm_rope_cache_rows for the tokens of several sequences and their pages: qkv
+ * [seqs, tokens, (n_heads + 2 n_kv_heads) * head_dim] -> q_out [seqs, tokens, n_heads *
+ * head_dim] and the cache.  cos_table and sin_table have table_rows positions; a token
+ * at a position that they or the page table do not have is left out, its q_out too.  The
+ * norm's mean and root are taken in 64 bits, so a row depends on its token and its
+ * page's scales alone. */
+int dip_qk_norm_rope_kv8(const uint16_t* qkv, const uint16_t* q_norm_w, const uint16_t* k_norm_w,
+                         const uint16_t* cos_table, const uint16_t* sin_table,
+                         int64_t table_rows, const int64_t* pos, uint16_t* q_out,
+                         uint8_t* k_cache, uint8_t* v_cache, float* kv_scales, int64_t pages,
+                         const int32_t* table, int64_t table_width, int64_t seqs, int64_t tokens,
+                         int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float eps,
+                         void* stream);
+
+/*
+ * dip_kv8_decode_attention: token t of sequence s (q [seqs, tokens, n_heads, head_dim])
+ * attends rows 0 .. pos[s] + t of its pages (all that the table has where that is
+ * more), out as q; n_heads at most 4096, a multiple of n_kv_heads.  A sequence with a
+ * negative position attends nothing and gives zeros.
+ * dip_kv8_prompt_attention: the tokens of one sequence (q [tokens, n_heads, head_dim],
+ * table [table_width]) at positions start .. start + tokens - 1, which the table must
+ * have, token t over rows 0 .. start + t.
+ * Types, sums and what is not finite as with dip_kv4_decode_attention, but for the
+ * weights: they are rounded to bf16 without the values' scales.  Workspaces need no
+ * clearing; calls that may run at once need one each.
+ */
+size_t dip_kv8_decode_attention_workspace_size(int64_t seqs, int64_t tokens, int64_t n_heads,
+                                               int64_t n_kv_heads, int64_t head_dim,
+                                               int64_t table_width);
+int dip_kv8_decode_attention(const uint16_t* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                             const float* kv_scales, int64_t pages, const int32_t* table,
+                             int64_t table_width, const int64_t* pos, uint16_t* out, int64_t seqs,
+                             int64_t tokens, int64_t n_heads, int64_t n_kv_heads,
+                             int64_t head_dim, float scale, void* workspace, size_t ws_bytes,
+                             void* stream);
+size_t dip_kv8_prompt_attention_workspace_size(int64_t tokens, int64_t start, int64_t n_heads,
+                                               int64_t n_kv_heads, int64_t head_dim);
+int dip_kv8_prompt_attention(const uint16_t* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                             const float* kv_scales, int64_t pages, const int32_t* table,
+                             int64_t table_width, int64_t start, uint16_t* out, int64_t tokens,
+                             int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
+                             void* workspace, size_t ws_bytes, void* stream);
 
 /*
  * token[r] (int64) drawn from row r of logits [rows, vocab] (DIP_BF16, DIP_F16
