@@ -122,6 +122,9 @@ _SIGS = {
     "dip_sample_workspace_size": ([_i64, _i64], _sz),
     "dip_sample": ([_p, _i32, _i64, _i64, _i64, _p, ctypes.c_double, _i64, ctypes.c_double,
                     ctypes.c_double, _p, _p, _p, _sz, _p], _i32),
+    "dip_verify_workspace_size": ([_i64, _i64, _i64, _i32], _sz),
+    "dip_verify": ([_p, _i32, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, ctypes.c_double, _i64,
+                    ctypes.c_double, ctypes.c_double, _p, _p, _p, _sz, _p], _i32),
     "dip_set_tuning": ([_i32, _i32], _i32),
     "dip_timeline_read": ([_i32, _p], _i32),
     "dip_get_tuning": ([_i32], _i32),
@@ -1402,6 +1405,74 @@ def sample(logits, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1
                               token.data_ptr(), prob.data_ptr(), ws_p, nbytes, _stream(dev)),
                "dip_sample")
     return token, prob
+
+
+def _logit_rows(t, vocab: int):
+    """t as rows [.., vocab] that are dense, an even stride apart."""
+    t = t.reshape(-1, vocab)
+    if vocab > 1 and t.stride(1) != 1 or t.stride(0) < 0:
+        t = t.contiguous()
+    return t
+
+
+def verify(logits, drafted, u, draft_logits=None, temperature: float = 1.0, top_k: int = 0,
+           top_p: float = 1.0, min_p: float = 0.0, out=None, accepted=None, ws=None):
+    """(tokens int64 [seqs, n + 1], accepted int64 [seqs]): which of the n drafted tokens
+    (int64 [seqs, n]) of each sequence the target's logits [seqs, n + 1, vocab] (bf16,
+    fp16 or fp32; row t those behind t drafts) accept, with the numbers u (fp32 [seqs,
+    n + 1], in [0, 1)), and the token that follows them.
+
+    With p_t the probabilities that sample draws with from row t, with these filters, and
+    q_t those of row t of draft_logits [seqs, n, vocab] (what drew the drafts, with the
+    same filters; None: 1 at the draft, for drafts made without chance), draft t is
+    accepted while u[t] * q_t < p_t at it.  The next token is drawn with u[n]: from
+    max(p_t - q_t, 0) at the first refused t, from p_n behind the last.  So the tokens are
+    distributed as sample would draw them from the target alone.  A draft outside the
+    vocabulary, such as -1, is none: the next token is drawn from p there.  tokens: the
+    accepted drafts, the drawn token, then -1.  Greedy (temperature 0, top_k 1): drafts
+    are accepted while they are the target's largest logits.
+
+    out, accepted and ws (uint8) may be given; calls that may run at once, or graphs that
+    do, need a ws each, as they have if it is None."""
+    check_sampling(temperature, top_k, top_p, min_p)
+    dev = _dev(logits, drafted, u)
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    if kind is None or logits.dim() != 3 or logits.shape[1] < 1 or logits.shape[2] < 1:
+        raise RuntimeError("logits must be bf16, fp16 or fp32 [seqs, drafts + 1, vocab]")
+    seqs, n, vocab = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    if drafted.dtype is not torch.int64 or tuple(drafted.shape) != (seqs, n):
+        raise RuntimeError(f"drafted must be an int64 tensor [{seqs}, {n}]")
+    if u.dtype is not torch.float32 or tuple(u.shape) != (seqs, n + 1):
+        raise RuntimeError(f"u must be a float32 tensor [{seqs}, {n + 1}]")
+    drafted, u = drafted.contiguous(), u.contiguous()
+    rows, draft = _logit_rows(logits, vocab), None
+    if draft_logits is not None:
+        if draft_logits.dtype is not logits.dtype or tuple(draft_logits.shape) != (seqs, n, vocab):
+            raise RuntimeError(f"draft_logits must be {logits.dtype} [{seqs}, {n}, {vocab}]")
+        if draft_logits.device != dev:
+            raise RuntimeError("draft_logits must be on the logits' device")
+        draft = _logit_rows(draft_logits, vocab) if n else None
+    for name, t, shape in (("out", out, (seqs, n + 1)), ("accepted", accepted, (seqs,))):
+        if t is not None and (t.dtype is not torch.int64 or tuple(t.shape) != shape
+                              or not t.is_contiguous() or t.device != dev):
+            raise RuntimeError(f"{name} must be a contiguous int64 tensor {list(shape)} on the "
+                               "logits' device")
+    if out is None:
+        out = torch.empty(seqs, n + 1, dtype=torch.int64, device=dev)
+    if accepted is None:
+        accepted = torch.empty(seqs, dtype=torch.int64, device=dev)
+    if seqs == 0:
+        return out, accepted
+    with _on(dev):
+        ws_p, nbytes, ws = _scratch(
+            lib.dip_verify_workspace_size(seqs, n, vocab, draft is not None), ws, dev,
+            "verification")
+        _check(lib.dip_verify(rows.data_ptr(), kind, seqs, n, vocab, rows.stride(0),
+                              drafted.data_ptr(), _ptr(draft),
+                              0 if draft is None else draft.stride(0), u.data_ptr(), temperature,
+                              min(int(top_k), vocab), top_p, min_p, out.data_ptr(),
+                              accepted.data_ptr(), ws_p, nbytes, _stream(dev)), "dip_verify")
+    return out, accepted
 
 
 def mlp_decode_rmsnorm(gate_qw, gate_sc, up_qw, up_sc, down_t_qw, down_t_sc, res, add, norm_w,

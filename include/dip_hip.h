@@ -53,7 +53,7 @@ const char* dip_status_string(int status);
  * minor number changes whenever an entry point's argument list changes, so
  * a binding written against this header checks dip_version() == DIP_VERSION
  * before its first call.  0.3.7 adds the paged 8-bit key/value cache (dip_kv8_*,
- * dip_qk_norm_rope_kv8).  0.3.6 adds the 4-bit key/value cache (dip_kv4_*,
+ * dip_qk_norm_rope_kv8) and dip_verify.  0.3.6 adds the 4-bit key/value cache (dip_kv4_*,
  * dip_qk_norm_rope_kv4*) and dip_sample.  0.3.5 adds dip_int4_gemm_swiglu, dip_swiglu,
  * dip_dequant_t, dip_stream_rows, dip_add_rmsnorm_rows and
  * dip_qk_norm_rope_cache_rows.  0.3.4: dip_int4_gather_down_by_channel takes
@@ -817,6 +817,35 @@ size_t dip_sample_workspace_size(int64_t rows, int64_t vocab);
 int dip_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
                const float* u, double temperature, int64_t top_k, double top_p, double min_p,
                int64_t* token, float* prob, void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Verification of drafted tokens (speculative decoding).  Row t of a sequence's
+ * tokens + 1 rows of target logits (row s * (tokens + 1) + t, row_stride values apart)
+ * is the target's behind t of its drafted tokens (int64 [seqs, tokens]); p_t are the
+ * probabilities that dip_sample draws with of it, with these filters.  q_t are those of
+ * row s * tokens + t of draft_logits (of the same type), or, where that is NULL, 1 at the
+ * drafted token and 0 elsewhere.  With u fp32 [seqs, tokens + 1] in [0, 1):
+ *   drafted token t is accepted while u[s][t] * q_t(it) < p_t(it);
+ *   the token behind the accepted ones is drawn with u[s][tokens]: from max(p_t - q_t, 0)
+ *   at the first refused t (from p_t if nothing is left of it), from p_tokens behind the
+ *   last; the first by index at which the running sum exceeds u times the whole.
+ * The tokens are then distributed as drawn from p one by one, if the drafted ones were
+ * from q.  A drafted token outside [0, vocab) is no draft: the sequence's next token is
+ * drawn from p there (so sequences may have fewer drafts).  token int64 [seqs, tokens +
+ * 1]: the accepted ones, the one drawn, then -1; accepted int64 [seqs]: their number,
+ * 0 .. tokens.  Greedy (temperature 0 or top_k 1): the drafts that are the target's
+ * largest logits are accepted, draft_logits and u are not read.  A row with nothing to
+ * choose from accepts nothing and gives token 0.  tokens >= 0; logits, types and filters
+ * as dip_sample's; seqs * (2 tokens + 1) below 2^22.  What is left of p is summed in whole
+ * numbers of 2^-51.  The workspace needs no clearing; calls that may run at once need
+ * one each.  The reference has no counterpart.
+ */
+size_t dip_verify_workspace_size(int64_t seqs, int64_t tokens, int64_t vocab, int draft_logits);
+int dip_verify(const void* logits, int dtype, int64_t seqs, int64_t tokens, int64_t vocab,
+               int64_t row_stride, const int64_t* drafted, const void* draft_logits,
+               int64_t draft_row_stride, const float* u, double temperature, int64_t top_k,
+               double top_p, double min_p, int64_t* token, int64_t* accepted, void* workspace,
+               size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }  // extern "C"
