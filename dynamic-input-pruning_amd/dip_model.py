@@ -9,7 +9,8 @@ model_int4.safetensors.  One MI355X holds the whole model in HBM, so every
 tensor goes to one device; there is no offload map.
 
 ``DIPDecoder`` decodes, greedily or drawing tokens (temperature, top-k, top-p,
-min-p), with its keys and values in bf16 or in 4 bits.  The prompt runs like the HF forward (the
+min-p), with its keys and values in bf16, in 8 or in 4 bits, one token a step or
+with tokens that the pruned step drafts and the dense route verifies.  The prompt runs like the HF forward (the
 reference's prefill: the DIP modules take their dense route for sequences
 longer than one token), on this library's kernels around the projections and
 MLPs where the model fits them, and leaves its keys and values in a static
@@ -243,10 +244,13 @@ class DIPDecoder:
                  prompt's attention then reads the 4-bit rows too, so it sees
                  what later tokens see (through the HF forward, where the model
                  has other modules, hooks or modes, it does not).
+      kv_dtype:  torch.float8_e4m3fn: keys and values in 8 bits with a scale per 64
+                 positions of a head (257 bytes per row and kv head), in pages; the
+                 same needs as kv_bits=4.  None: as kv_bits says.
     """
 
     def __init__(self, model: nn.Module, max_len: int = 1024, use_graph: bool = True,
-                 fused=None, kv_bits: int = 16):
+                 fused=None, kv_bits: int = 16, kv_dtype=None):
         inner = model.model
         cfg = model.config
         self.model = model
@@ -264,13 +268,26 @@ class DIPDecoder:
             raise ValueError(f"rope type {rot.rope_type!r}: frequencies change with length")
         self.max_len = int(max_len)
         if kv_bits not in (4, 16):
-            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
+            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits} (8 bits are "
+                             "kv_dtype=torch.float8_e4m3fn)")
+        if kv_dtype is not None:
+            if kv_dtype is not torch.float8_e4m3fn or kv_bits != 16:
+                raise ValueError("kv_dtype must be torch.float8_e4m3fn, without kv_bits")
+            kv_bits = 8
         self.kv_bits = kv_bits
         supported = self._fused_supported()
-        if kv_bits == 4 and (not supported or (fused is not None and not fused)):
-            raise ValueError("a 4-bit cache needs the fused decode: a GPU, bf16 weights, head_dim "
-                             "128, int4 attention projections and a supported head grouping")
+        if kv_bits < 16 and (not supported or (fused is not None and not fused)):
+            raise ValueError(f"a {kv_bits}-bit cache needs the fused decode: a GPU, bf16 weights, "
+                             "head_dim 128, int4 attention projections and a supported head "
+                             "grouping")
         rows = self.max_len
+        if kv_bits == 8:
+            import _dip_hip as K
+            pages = -(-self.max_len // K.KV8_PAGE)
+            self.kv8 = K.kv8_cache(self.nkv, pages, self.device, layers=len(self.layers))
+            self._kv8 = [self.kv8.layer(i) for i in range(len(self.layers))]
+            self._table = torch.arange(pages, dtype=torch.int32, device=self.device)[None]
+            rows = pages * K.KV8_PAGE
         if kv_bits == 4:
             import _dip_hip as K
             self.kv4 = K.kv4_cache(self.nkv, self.max_len, self.device, layers=len(self.layers))
@@ -289,6 +306,7 @@ class DIPDecoder:
         self.tok = torch.zeros(1, dtype=torch.long, device=self.device)
         self.pos = torch.zeros(1, dtype=torch.long, device=self.device)
         self._draw = None  # how generate draws its tokens; None: greedy
+        self.drafts = (0, 0)  # accepted and made in the last generate that drafted
         if fused and not supported:
             raise ValueError("fused decode needs a GPU, bf16 weights, head_dim 128, int4 "
                              "attention projections and a supported head grouping")
@@ -366,6 +384,9 @@ class DIPDecoder:
         self._o = torch.empty(self.nh * self.hd, dtype=bf, device=dev)
         nbytes = (K.kv4_decode_attention_workspace_bytes(self.nh, self.nkv, self.kv4.max_len)
                   if self.kv_bits == 4 else
+                  K.kv8_decode_attention_workspace_bytes(1, 1, self.nh, self.nkv,
+                                                         self._table.shape[1])
+                  if self.kv_bits == 8 else
                   K.decode_attention_workspace_bytes(self.nh, self.hd, self.max_len))
         self._attn_ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
         # short caches: norm + rotary + cache write + attention in one launch
@@ -400,6 +421,13 @@ class DIPDecoder:
                                    a.q_norm.variance_epsilon)
                 K.kv4_decode_attention(self._q, self._kv4[i], self.pos, self._o, a.scaling,
                                        ws=self._attn_ws)
+            elif self.kv_bits == 8:
+                q = self._q.view(1, 1, -1)
+                K.qk_norm_rope_kv8(self._qkv.view(1, 1, -1), a.q_norm.weight, a.k_norm.weight,
+                                   self.cos, self.sin, self.pos, q, self._kv8[i], self._table,
+                                   self.nh, self.nkv, a.q_norm.variance_epsilon)
+                K.kv8_decode_attention(q, self._kv8[i], self._table, self.pos,
+                                       self._o.view(1, 1, -1), a.scaling, ws=self._attn_ws)
             elif self._attn_one_launch:
                 K.decode_attention_fused(self._qkv, a.q_norm.weight, a.k_norm.weight, self.cos,
                                          self.sin, self.pos, self.k_cache[i], self.v_cache[i],
@@ -509,7 +537,7 @@ class DIPDecoder:
         """prefill with the decode kernels' prompt forms around the
         projections: one q|k|v product; q/k norm, rotary embedding and the
         static cache's rows in one launch; residual add and RMSNorm in one; and
-        the head for the last token alone.  With a 4-bit cache the prompt goes
+        the head for the last token alone.  With a quantised cache the prompt goes
         through the layers in parts of even length."""
         K, plen = self._K, ids.shape[1]
         parts = 1 if self.kv_bits == 16 else -(-plen // _PROMPT_CHUNK)
@@ -524,14 +552,15 @@ class DIPDecoder:
         return logits
 
     def _prefill_part(self, ids: torch.Tensor, start: int):
-        """The tokens of a prompt from position `start` through every layer
-        (start 0 with a bf16 cache); (residual, last MLP's output)."""
+        """The tokens of a prompt, or more than one behind it, from position `start`
+        through every layer (start 0 with a bf16 cache); (residual, last MLP's output)."""
         from qlinear import int4_linear
         K, inner, hd, nh = self._K, self.model.model, self.hd, self.nh
         plen = ids.shape[1]
         h = inner.embed_tokens(ids).view(plen, self.hidden)  # from here on the residual, in place
         q = torch.empty(plen, nh * hd, dtype=self.dtype, device=self.device)
         x = y = None
+        at = torch.full((1,), start, device=self.device) if self.kv_bits == 8 else None
         for i, L in enumerate(self.layers):
             a, n_in, pn = L.self_attn, L.input_layernorm, L.post_attention_layernorm
             # a layer's own, as who calls its MLP may keep it; else the same memory again
@@ -544,6 +573,13 @@ class DIPDecoder:
                                         q, self._kv4[i], nh, self.nkv, a.q_norm.variance_epsilon,
                                         start=start)
                 o = K.kv4_prompt_attention(q, self._kv4[i], start, None, a.scaling)
+                o = a.o_proj(o.view(1, plen, nh * hd))
+            elif self.kv_bits == 8:
+                K.qk_norm_rope_kv8(qkv.view(1, plen, -1), a.q_norm.weight, a.k_norm.weight,
+                                   self.cos, self.sin, at, q.view(1, plen, -1), self._kv8[i],
+                                   self._table, nh, self.nkv, a.q_norm.variance_epsilon)
+                o = K.kv8_prompt_attention(q, self._kv8[i], self._table[0], start, None,
+                                           a.scaling)
                 o = a.o_proj(o.view(1, plen, nh * hd))
             else:
                 kc, vc = self.k_cache[i], self.v_cache[i]
@@ -659,6 +695,10 @@ class DIPDecoder:
                 self._K.kv4_write(layer.keys[0].transpose(0, 1), layer.values[0].transpose(0, 1),
                                   self._kv4[i])
                 continue
+            if self.kv_bits == 8:
+                self._K.kv8_write(layer.keys.transpose(1, 2), layer.values.transpose(1, 2),
+                                  self._kv8[i], self._table, torch.zeros_like(self.pos))
+                continue
             self.k_cache[i, :, :plen].copy_(layer.keys[0])
             self.v_cache[i, :, :plen].copy_(layer.values[0])
         logits = out.logits[0, -1]
@@ -669,7 +709,8 @@ class DIPDecoder:
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id=None,
                  return_logits: bool = False, do_sample: bool = False, temperature: float = 1.0,
-                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, generator=None):
+                 top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, generator=None,
+                 draft: int = 0):
         """Continuation of `input_ids` [1, P]: the prompt followed by up to
         `max_new_tokens` tokens (cut after the first `eos_token_id`), as HF's
         generate returns it for batch 1.  Greedy, or with `do_sample` drawn with
@@ -677,7 +718,20 @@ class DIPDecoder:
         `temperature`, of the `top_k` likeliest tokens (0: all) the fewest that
         reach `top_p` of the probability, of those the ones with at least
         `min_p` of the largest (_dip_hip.sample).  With `return_logits` also the
-        logits of every generated token, before any of these."""
+        logits of every generated token, before any of these.
+
+        With `draft` n > 0 the tokens are the dense model's, as prompts run through
+        it: n pruned steps draft a token each, drawn as the settings say, one pass of
+        n + 1 tokens through the dense route gives their logits, and _dip_hip.verify
+        accepts those that are the dense model's too and chooses the one behind them.
+        `self.drafts` then has the numbers of accepted and of drafted tokens.  It needs
+        a cache of 4 or 8 bits, which a pass of several tokens can go on from, with
+        room for `draft` tokens behind the last."""
+        if draft:
+            return self._generate_drafted(input_ids, max_new_tokens, eos_token_id, return_logits,
+                                          int(draft), do_sample,
+                                          dict(temperature=temperature, top_k=top_k, top_p=top_p,
+                                               min_p=min_p), generator)
         if not do_sample:
             return self._generate(input_ids, max_new_tokens, eos_token_id, return_logits)
         if self.device.type != "cuda":
@@ -693,6 +747,78 @@ class DIPDecoder:
         finally:
             self._draw = None
 
+    def _reset_speculation(self) -> None:
+        """Every generation starts from fresh speculation keys, so the same
+        prompt gives the same tokens and logits bit for bit."""
+        for m in self.model.modules():
+            if hasattr(m, "reset_speculation"):
+                m.reset_speculation()
+
+    def _generate_drafted(self, input_ids, max_new_tokens: int, eos_token_id, return_logits: bool,
+                          draft: int, do_sample: bool, how: dict, generator):
+        """generate with drafted tokens (see there).  Every pass of the dense route has
+        draft + 1 tokens, of which the ones behind the last wanted are dropped: a single
+        token would take the pruned step."""
+        if draft < 0 or self.kv_bits == 16 or not self._prefill_fusible():
+            raise ValueError(f"draft must not be negative: {draft}" if draft < 0 else
+                             "drafting needs a cache of 4 or 8 bits, and prompts on the fused "
+                             "kernels")
+        K, dev = self._K, self.device
+        if not do_sample:
+            how = dict(how, temperature=0.0)
+        K.check_sampling(**how)
+        ids = input_ids.to(dev).view(1, -1)
+        plen = ids.shape[1]
+        if plen + max_new_tokens + draft > self.max_len:
+            raise ValueError(f"{plen} + {max_new_tokens} tokens and {draft} drafted ones exceed "
+                             f"max_len {self.max_len}")
+        eos = set(() if eos_token_id is None else eos_token_id
+                  if isinstance(eos_token_id, (list, tuple)) else [eos_token_id])
+        on = dev if generator is None else generator.device
+        rand = lambda n: torch.rand(n, generator=generator, device=on).to(dev)
+        norm = self.model.model.norm
+        tokens, logs, accepted, made = [], [], 0, 0
+        self._reset_speculation()
+        try:
+            if do_sample:
+                self._draw = iter(rand(1).split(1)), how
+            last = self.prefill(ids)
+            if max_new_tokens > 0:
+                tokens.append(int(self.tok))
+                logs.append(last.view(-1).float())
+            while 0 < len(tokens) < max_new_tokens and tokens[-1] not in eos:
+                start = plen + len(tokens) - 1  # of the last token, which no pass has had
+                part = torch.empty(1, draft + 1, dtype=torch.long, device=dev)
+                part[0, :1].copy_(self.tok)
+                if do_sample:
+                    self._draw = iter(rand(draft).split(1)), how
+                drawn_from = []
+                for j in range(draft):
+                    logits = self.step()
+                    part[0, j + 1:j + 2].copy_(self.tok)
+                    if do_sample:
+                        drawn_from.append(logits.view(-1))
+                h, y = self._prefill_part(part, start)
+                x = torch.empty_like(h)
+                K.add_rmsnorm_rows(h, y, norm.weight, x, norm.variance_epsilon)
+                logits = self.model.lm_head(x).view(1, draft + 1, -1)
+                u = rand(draft + 1) if do_sample else torch.zeros(draft + 1, device=dev)
+                new, _ = K.verify(logits, part[:, 1:], u.view(1, -1),
+                                  torch.stack(drawn_from)[None] if do_sample else None, **how)
+                new = [t for t in new[0].tolist() if t >= 0]
+                accepted, made = accepted + len(new) - 1, made + draft
+                new = new[:max_new_tokens - len(tokens)]
+                new = new[:next((j + 1 for j, t in enumerate(new) if t in eos), len(new))]
+                tokens += new
+                logs += list(logits[0, :len(new)].float())
+                self.tok.fill_(tokens[-1])
+                self.pos.fill_(plen + len(tokens) - 1)
+        finally:
+            self._draw = None
+        self.drafts = (accepted, made)
+        seq = torch.cat([ids[0].cpu(), torch.tensor(tokens, dtype=torch.long)]).view(1, -1)
+        return (seq, torch.stack(logs)) if return_logits else seq
+
     def _generate(self, input_ids: torch.Tensor, max_new_tokens: int, eos_token_id,
                   return_logits: bool):
         ids = input_ids.to(self.device).view(1, -1)
@@ -701,11 +827,7 @@ class DIPDecoder:
             raise ValueError(f"{plen} + {max_new_tokens} tokens exceed max_len {self.max_len}")
         toks = torch.empty(max_new_tokens, dtype=torch.long, device=self.device)
         logs = []
-        # every generation starts from fresh speculation keys, so the same
-        # prompt gives the same tokens and logits bit for bit
-        for m in self.model.modules():
-            if hasattr(m, "reset_speculation"):
-                m.reset_speculation()
+        self._reset_speculation()
         last = self.prefill(ids)
         for t in range(max_new_tokens):
             if return_logits:
