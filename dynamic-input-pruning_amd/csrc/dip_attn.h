@@ -127,4 +127,45 @@ DIP_DEV void combine_splits(const float* base, size_t stride, int ns, uint16_t* 
   }
 }
 
+// The same of up to 64 splits by kWaves waves (a workgroup's), each of which takes every
+// kWaves-th split, lane l dimensions 2 l and 2 l + 1.  `red`: LDS for the waves' sums.
+template <int kWaves>
+DIP_DEV void combine_splits_waves(const float* base, size_t stride, int ns, int wave, int l,
+                                  float2 (*red)[64], uint16_t* out) {
+  // lane s the weight of split s, then 16 splits' sums in flight
+  const float2 ml = l < ns ? *reinterpret_cast<const float2*>(base + l * stride)
+                           : make_float2(-INFINITY, 0.f);
+  const float mx = group_max<64>(ml.x);
+  // (a split without a score above -inf has sums of 0, or NaN, which must count)
+  const float f = l >= ns ? 0.f : ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - mx);
+  const float sum = group_sum<64>(f * ml.y);
+  float o0 = 0.f, o1 = 0.f;
+  for (int s0 = wave; s0 < ns; s0 += 16 * kWaves) {
+    float2 v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u)
+      v[u] = *reinterpret_cast<const float2*>(base + min(s0 + kWaves * u, ns - 1) * stride + 2 +
+                                              2 * l);
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      if (s0 + kWaves * u >= ns) break;
+      const float w = __shfl(f, s0 + kWaves * u, 64);
+      o0 = fmaf(w, v[u].x, o0);
+      o1 = fmaf(w, v[u].y, o1);
+    }
+  }
+  if (kWaves > 1) {
+    red[wave][l] = make_float2(o0, o1);
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+      o0 += red[w][l].x;
+      o1 += red[w][l].y;
+    }
+  }
+  const float inv = ns == 0 ? 0.f : 1.f / sum;  // (no rows: zeros)
+  reinterpret_cast<uint32_t*>(out)[l] = cvt_bf16x2(o0 * inv, o1 * inv);
+}
+
 }  // namespace dip

@@ -339,30 +339,9 @@ __global__ __launch_bounds__(256) void prompt_combine_kernel(PromptArgs a) {
   const float* base = a.part + ((size_t)(tile * a.nkv + kvh) * a.splits * kTileCols +
                                 cc % kTileCols) * kKvPart;
   const size_t stride = (size_t)kTileCols * kKvPart;
-  // lane s the weight of split s (64 at most), then 8 splits' sums in flight
-  const float2 ml = l < ns ? *reinterpret_cast<const float2*>(base + l * stride)
-                           : make_float2(-INFINITY, 0.f);
-  const float mx = group_max<64>(ml.x);
-  const float f = l >= ns ? 0.f : ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - mx);
-  const float sum = group_sum<64>(f * ml.y);
-  float o0 = 0.f, o1 = 0.f;
-  for (int s0 = 0; s0 < ns; s0 += 8) {
-    float2 v[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u)
-      v[u] = *reinterpret_cast<const float2*>(base + min(s0 + u, ns - 1) * stride + 2 + 2 * l);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (s0 + u >= ns) break;
-      const float w = __shfl(f, s0 + u, 64);
-      o0 = fmaf(w, v[u].x, o0);
-      o1 = fmaf(w, v[u].y, o1);
-    }
-  }
-  const float inv = 1.f / sum;
-  reinterpret_cast<uint32_t*>(a.out)[((size_t)(cc / a.group) * a.nkv * a.group +
-                                      kvh * a.group + cc % a.group) * 64 + l] =
-      cvt_bf16x2(o0 * inv, o1 * inv);
+  combine_splits_waves<1>(base, stride, ns, 0, l, nullptr,
+                          a.out + ((size_t)(cc / a.group) * a.nkv * a.group + kvh * a.group +
+                                   cc % a.group) * kKvHeadDim);
 }
 
 struct Plan {

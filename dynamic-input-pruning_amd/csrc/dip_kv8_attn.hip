@@ -16,7 +16,7 @@ struct Kv8AttnArgs {
   int64_t start;
   int seqs, tokens, group, width;
   int tiles;   // of columns
-  int per;     // pages of a split
+  int per;     // pages of a split, at least
   int splits;
   float scale;
 };
@@ -33,273 +33,294 @@ DIP_DEV int tile_pages(const Kv8AttnArgs& a, int64_t first, int tile, int cols) 
   return (rows + kPageRows - 1) / kPageRows;
 }
 
-// A tile of 16 CT columns, each a (token, query head) of one kv head of a sequence,
-// over the pages of one split, in turn by the W waves of the workgroup.  Per page a
-// wave computes, all in registers:
-//   scores^T: A = 16 keys, B = the columns' queries, 16x16x32 MFMAs; lane (c, col) ends
-//     up with the scores of rows 16 t + 4 c + r;
-//   softmax against a base that follows the running maximum (the columns' lanes agree
-//     on it by two lane swaps) in fp32;
-//   values^T: A = 16 dimensions of 32 rows, B = the weights rounded to bf16 (off by
-//     2^-8 of each at most) where the scores are.
-// Keys and values become bf16 times their page's scale on the way, two to an
-// instruction.
-template <int W, int CT>
-__global__ __launch_bounds__(W * 64) void kv8_attn_kernel(Kv8AttnArgs a) {
-  constexpr int kCols = 16 * CT;
-  __shared__ float wm[W][kCols], wl[W][kCols];
-  __shared__ __align__(16) float wacc[W][kCols][kKvHeadDim + 4];
-  const int nkv = a.c.nkv;
-  const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % nkv;
-  const int tile = blockIdx.x / a.splits / nkv % a.tiles;
-  const int seq = blockIdx.x / a.splits / nkv / a.tiles;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
-  const int l16 = l & 15, c = l >> 4;
-  const int64_t first = first_of(a, seq);
-  const int pages = tile_pages(a, first, tile, kCols);
-  const bool direct = a.splits == 1;
-  if (!direct && split * a.per >= pages) return;
-  const int p0 = split * a.per + wave, p1 = min(split * a.per + a.per, pages);
+// The pages of a split of a sequence that has `pages`.
+DIP_DEV int pages_per_split(const Kv8AttnArgs& a, int pages) {
+  return max(a.per, (pages + a.splits - 1) / a.splits);
+}
 
-  bf16x8_t bq[CT][4];
-  int limit[CT];  // rows that the lane's columns attend
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int col = tile * kCols + 16 * ct + l16;
-    const int tok = col / a.group, head = kvh * a.group + col % a.group;
+// A workgroup's share.  Workgroups go to the 8 XCDs in turn: the heads of a split come
+// one after the other, so that an XCD gets all splits alike, of which the later ones have
+// less to do where lengths differ.  (By splits first, 32 sequences of up to 16384 rows,
+// four splits: 138 us.)
+struct Task {
+  int split, kvh, tile, seq;
+  DIP_DEV explicit Task(const Kv8AttnArgs& a) {
+    const int heads = a.seqs * a.tiles * a.c.nkv, head = blockIdx.x % heads;
+    split = blockIdx.x / heads;
+    kvh = head % a.c.nkv;
+    tile = head / a.c.nkv % a.tiles;
+    seq = head / a.c.nkv / a.tiles;
+  }
+  DIP_DEV size_t part(const Kv8AttnArgs& a) const {
+    return (((size_t)seq * a.tiles + tile) * a.c.nkv + kvh) * a.splits + split;
+  }
+};
+
+// What a wave has of 16 columns, each a (token, query head) of one kv head of a
+// sequence: lane (c, l16) of column l16 the queries' operand, the sums of dimensions 16 t
+// + 4 c + r, and the softmax's base and sum.
+struct Columns {
+  bf16x8_t q[4];
+  floatx4 acc[8];
+  float m, den;  // m: the base; den: this lane's rows only
+  int limit;     // rows that the column attends
+  int sure;      // rows that every column attends
+  float scale2;  // to scores in powers of 2
+
+  DIP_DEV Columns(const Kv8AttnArgs& a, int seq, int kvh, int64_t first, int col0, int l16, int c) {
+    const int nkv = a.c.nkv, col = col0 + l16, tok = col / a.group;
+    const int head = kvh * a.group + col % a.group;
     const bool on = tok < a.tokens && first >= 0;
-    limit[ct] = on ? rows_at(first + tok, a.width * kPageRows) : 0;
+    limit = on ? rows_at(first + tok, a.width * kPageRows) : 0;
+    // (columns without a token, whose queries are 0, take them too: nothing reads
+    // their sums)
+    sure = rows_at(first + col0 / a.group, a.width * kPageRows);
+    scale2 = a.scale * kLog2e;
     const uint4* qp = reinterpret_cast<const uint4*>(
         a.q + (((size_t)seq * a.tokens + tok) * nkv * a.group + head) * kKvHeadDim);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const uint4 w = on ? qp[8 * (g >> 1) + 2 * c + (g & 1)] : make_uint4(0, 0, 0, 0);
-      bq[ct][g] = __builtin_bit_cast(bf16x8_t, u32x4_t{w.x, w.y, w.z, w.w});
+      q[g] = __builtin_bit_cast(bf16x8_t, u32x4_t{w.x, w.y, w.z, w.w});
+    }
+    m = -INFINITY;
+    den = 0.f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // Whether some column of the wave does not attend all of a page.
+  DIP_DEV bool masks(int page) const { return (page + 1) * kPageRows > sure; }
+
+  // Adds a page's rows, kMasked if it masks some.  keys(t, i) and values(t): the lane's 16
+  // bytes of the page, of row 16 t + l16 from dimension 64 i + 16 c on, and of dimension
+  // 16 t + l16.
+  //   scores^T: A = 16 keys, B = the columns' queries, 16x16x32 MFMAs; lane (c, col) ends
+  //     up with the scores of rows 16 t + 4 c + r;
+  //   softmax against a base that follows the running maximum (the columns' lanes agree
+  //     on it by two lane swaps) in fp32;
+  //   values^T: A = 16 dimensions of 32 rows, B = the weights rounded to bf16 (off by
+  //     2^-8 of each at most) where the scores are.
+  // Keys and values become bf16 times their page's scale on the way, two to an
+  // instruction.
+  template <bool kMasked, typename K, typename V>
+  DIP_DEV void add(K keys, V values, float2 scale, int page, int c) {
+    float s[4][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint4 lo = keys(t, 0), hi = keys(t, 1);
+      floatx4 d{0.f, 0.f, 0.f, 0.f};
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(lo.x, lo.y, scale.x), q[0], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(lo.z, lo.w, scale.x), q[1], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(hi.x, hi.y, scale.x), q[2], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(hi.z, hi.w, scale.x), q[3], d, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[t][r] = d[r] * scale2;
+    }
+    const int row = page * kPageRows + 4 * c;  // of s[0][0]
+    if (kMasked) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (row + 16 * (e >> 2) + (e & 3) >= limit) s[e >> 2][e & 3] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e >> 2][e & 3]);
+    mx = fmaxf(m, row_pair_max32(row_pair_max16(mx)) + kDown);
+    if (__any(mx > m + kSlack)) {
+      const float f = m == -INFINITY ? 0.f : fast_exp2(m - mx);  // what the sums so far are worth
+      den *= f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[t][r] *= f;
+      m = mx;
+    }
+    const float base = m == -INFINITY ? 0.f : m;  // (no score above -inf yet: weights 0, or NaN)
+    {
+      // Not one multiply-add from the sum: the base comes from the rounded scores, and
+      // beyond 2^31 the rounding alone is further than weights reach.
+#pragma clang fp contract(off)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e >> 2][e & 3] = fast_exp2(s[e >> 2][e & 3] - base);
+    }
+    if (kMasked) {
+      // weights of 0, whatever a base of +inf or NaN made of them
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (row + 16 * (e >> 2) + (e & 3) >= limit) s[e >> 2][e & 3] = 0.f;
+    }
+    bf16x8_t p[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float(&x)[4] = s[2 * h], (&y)[4] = s[2 * h + 1];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) den += x[r] + y[r];
+      p[h] = __builtin_bit_cast(bf16x8_t,
+                                u32x4_t{cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]),
+                                        cvt_bf16x2(y[0], y[1]), cvt_bf16x2(y[2], y[3])});
+    }
+    if (!kMasked) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) product(t, values(t), p, scale.y);
+      return;
+    }
+    // A NaN counts for the columns that attend its row alone: it is taken out of the values,
+    // and a product of ones where NaN is with ones where a column attends says which sums
+    // it belongs to.
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const uint4 w = values(t), n = nans(w);
+      product(t, make_uint4(w.x & ~n.x, w.y & ~n.y, w.z & ~n.z, w.w & ~n.w), p, scale.y);
+      if (!__any((n.x | n.y | n.z | n.w) != 0u)) continue;
+      bf16x8_t there[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = row + 32 * h + 16 * (e >> 1) + 2 * (e & 1);
+          o[e] = (r < limit ? 0x3F80u : 0u) | (r + 1 < limit ? 0x3F800000u : 0u);
+        }
+        there[h] = __builtin_bit_cast(bf16x8_t, o);
+      }
+      constexpr uint32_t kOne = 0x38383838u;
+      floatx4 d{0.f, 0.f, 0.f, 0.f};
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(n.x & kOne, n.y & kOne, 1.f),
+                                                  there[0], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(n.z & kOne, n.w & kOne, 1.f),
+                                                  there[1], d, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[t][r] = d[r] > 0.f ? NAN : acc[t][r];
     }
   }
-  // rows that every column of the tile attends (columns without a token, whose
-  // queries are 0, take them too: nothing reads their sums)
-  const int sure = rows_at(first + tile * kCols / a.group, a.width * kPageRows);
-  const float sc2 = a.scale * kLog2e;
-  const int32_t* table = a.table + (size_t)seq * a.width;
 
-  floatx4 acc[CT][8];
-  float m[CT], den[CT];  // m: the base; den: this lane's rows only
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    m[ct] = -INFINITY;
-    den[ct] = 0.f;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) acc[ct][t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  DIP_DEV static uint4 nans(uint4 w) {
+    return make_uint4(kv8_nan_bytes(w.x), kv8_nan_bytes(w.y), kv8_nan_bytes(w.z),
+                      kv8_nan_bytes(w.w));
   }
+  DIP_DEV void product(int t, uint4 w, const bf16x8_t (&p)[2], float scale) {
+    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(w.x, w.y, scale), p[0], acc[t], 0,
+                                                     0, 0);
+    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(w.z, w.w, scale), p[1], acc[t], 0,
+                                                     0, 0);
+  }
+};
+
+// The 16-byte pieces of a page's keys (of values behind them) that an operand takes.
+DIP_DEV int key_piece(int t, int i, int l16, int c) { return (16 * t + l16) * 8 + 4 * i + c; }
+DIP_DEV int value_piece(int t, int l16, int c) { return (16 * t + l16) * 4 + c; }
+constexpr int kPagePieces = kPageBytes / 16;
+
+constexpr int kRawBuffer = 0x00027000;  // a buffer of bytes, bounds checked
+DIP_DEV uint4 buffer_piece(__amdgpu_buffer_rsrc_t b, int piece) {
+  const u32x4_t w =
+      __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, 16 * piece, 0, 0));
+  return make_uint4(w.x, w.y, w.z, w.w);
+}
+
+// Up to 16 columns: a workgroup of W waves takes a split's pages in turn, each wave
+// with all columns, from memory into registers, 32 KB of a wave in flight.  Bound by
+// memory: 32 sequences of up to 16384 rows (547 MB) 114 us, 4.8 TB/s; one of 131071 (268
+// MB) 44.  One of 701 rows, in one launch of 8 waves: 8.8 us of waits in a row.
+template <int W>
+__global__ __launch_bounds__(W * 64) void kv8_attn_kernel(Kv8AttnArgs a) {
+  __shared__ float wm[W][16], wl[W][16];
+  __shared__ __align__(16) float wacc[W][16][kKvHeadDim + 4];
+  const int nkv = a.c.nkv;
+  const Task task(a);
+  const int split = task.split, kvh = task.kvh, seq = task.seq;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+  const int l16 = l & 15, c = l >> 4;
+  const int64_t first = first_of(a, seq);
+  const int pages = tile_pages(a, first, 0, 16);
+  const bool direct = a.splits == 1;
+  const int per = pages_per_split(a, pages);
+  if (!direct && split * per >= pages) return;
+  const int p0 = split * per + wave, p1 = min(split * per + per, pages);
+  const int32_t* table = a.table + (size_t)seq * a.width;
+  Columns x(a, seq, kvh, first, 0, l16, c);
 
   struct Raw {
     uint4 k[8], v[8];
     float2 scale;
   };
-  auto load = [&](Raw& x, int id) {
+  // Page number id, or zeros where that is negative: the bounds of the buffer say so,
+  // so the loads are behind no branch, which would have them all waited for where it ends.
+  auto load = [&](Raw& r, int id) {
     const size_t at = (size_t)max(id, 0) * nkv + kvh;
-    const uint4* kp = reinterpret_cast<const uint4*>(a.c.k + at * kPageBytes) + 8 * l16 + c;
-    const uint4* vp = reinterpret_cast<const uint4*>(a.c.v + at * kPageBytes) + 4 * l16 + c;
+    const int bytes = id < 0 ? 0 : kPageBytes;
+    const auto kp = __builtin_amdgcn_make_buffer_rsrc(a.c.k + at * kPageBytes, 0, bytes, kRawBuffer);
+    const auto vp = __builtin_amdgcn_make_buffer_rsrc(a.c.v + at * kPageBytes, 0, bytes, kRawBuffer);
 #pragma unroll
-    for (int t = 0; t < 8; ++t) x.k[t] = kp[128 * (t >> 1) + 4 * (t & 1)];
+    for (int t = 0; t < 8; ++t) r.k[t] = buffer_piece(kp, key_piece(t >> 1, t & 1, l16, c));
 #pragma unroll
-    for (int t = 0; t < 8; ++t) x.v[t] = vp[64 * t];
-    x.scale = *reinterpret_cast<const float2*>(a.c.scales + 2 * at);
+    for (int t = 0; t < 8; ++t) r.v[t] = buffer_piece(vp, value_piece(t, l16, c));
+    r.scale = *reinterpret_cast<const float2*>(a.c.scales + 2 * at);
   };
   auto number = [&](int p) {
-    return __builtin_amdgcn_readfirstlane(page_number(table, min(p, p1 - 1), a.c.pages));
-  };
-  auto page = [&](Raw& x, int id, int p) {
-    if (id < 0) {  // rows of no page: zeros
-#pragma unroll
-      for (int t = 0; t < 8; ++t) x.k[t] = x.v[t] = make_uint4(0, 0, 0, 0);
-    }
-    float s[CT][4][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint4 lo = x.k[2 * t], hi = x.k[2 * t + 1];
-      const bf16x8_t ka[4] = {
-          kv8_operand(lo.x, lo.y, x.scale.x), kv8_operand(lo.z, lo.w, x.scale.x),
-          kv8_operand(hi.x, hi.y, x.scale.x), kv8_operand(hi.z, hi.w, x.scale.x)};
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        floatx4 d{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[g], bq[ct][g], d, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[ct][t][r] = d[r] * sc2;
-      }
-    }
-    const bool masked = (p + 1) * kPageRows > sure;
-    const int row = p * kPageRows + 4 * c;  // of s[..][0][0]
-    if (masked) {
-      asm volatile("");  // a branch: comparisons and selections that most pages skip
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (row + 16 * (e >> 2) + (e & 3) >= limit[ct]) s[ct][e >> 2][e & 3] = -INFINITY;
-    }
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[ct][e >> 2][e & 3]);
-      mx = fmaxf(m[ct], row_pair_max32(row_pair_max16(mx)) + kDown);
-      if (__any(mx > m[ct] + kSlack)) {
-        // what the sums so far are worth
-        const float f = m[ct] == -INFINITY ? 0.f : fast_exp2(m[ct] - mx);
-        den[ct] *= f;
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[ct][t][r] *= f;
-        m[ct] = mx;
-      }
-      // (no score above -inf yet: weights 0, or NaN)
-      const float base = m[ct] == -INFINITY ? 0.f : m[ct];
-      {
-        // Not one multiply-add from the sum: the base comes from the rounded scores, and
-        // beyond 2^31 the rounding alone is further than weights reach.
-#pragma clang fp contract(off)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          s[ct][e >> 2][e & 3] = fast_exp2(s[ct][e >> 2][e & 3] - base);
-      }
-    }
-    if (masked) {
-      asm volatile("");
-      uint32_t some = 0u;
-      // weights of 0, whatever a base of +inf or NaN made of them
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (row + 16 * (e >> 2) + (e & 3) >= limit[ct]) s[ct][e >> 2][e & 3] = 0.f;
-#pragma unroll
-      for (int t = 0; t < 8; ++t)
-        some |= kv8_nan_bytes(x.v[t].x) | kv8_nan_bytes(x.v[t].y) | kv8_nan_bytes(x.v[t].z) |
-                kv8_nan_bytes(x.v[t].w);
-      if (__any(some != 0u)) {
-        // A NaN counts for the columns that attend its row alone: it is taken out of the
-        // values, and a product of ones where NaN is with ones where a column attends
-        // says which sums it belongs to.
-        bf16x8_t there[CT][2];
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            u32x4_t w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = row + 32 * h + 16 * (e >> 1) + 2 * (e & 1);
-              w[e] = (r < limit[ct] ? 0x3F80u : 0u) | (r + 1 < limit[ct] ? 0x3F800000u : 0u);
-            }
-            there[ct][h] = __builtin_bit_cast(bf16x8_t, w);
-          }
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const uint4 w = x.v[t];
-          const uint4 n = make_uint4(kv8_nan_bytes(w.x), kv8_nan_bytes(w.y), kv8_nan_bytes(w.z),
-                                     kv8_nan_bytes(w.w));
-          x.v[t] = make_uint4(w.x & ~n.x, w.y & ~n.y, w.z & ~n.z, w.w & ~n.w);
-          const uint32_t one = 0x38383838u;  // 1.0
-          const bf16x8_t a0 = kv8_operand(n.x & one, n.y & one, 1.f);
-          const bf16x8_t a1 = kv8_operand(n.z & one, n.w & one, 1.f);
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            floatx4 d{0.f, 0.f, 0.f, 0.f};
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, there[ct][0], d, 0, 0, 0);
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, there[ct][1], d, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[ct][t][r] = d[r] > 0.f ? NAN : acc[ct][t][r];
-          }
-        }
-      }
-    }
-    bf16x8_t bp[CT][2];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float(&p)[4] = s[ct][2 * h], (&q)[4] = s[ct][2 * h + 1];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) den[ct] += p[r] + q[r];
-        bp[ct][h] = __builtin_bit_cast(
-            bf16x8_t, u32x4_t{cvt_bf16x2(p[0], p[1]), cvt_bf16x2(p[2], p[3]),
-                              cvt_bf16x2(q[0], q[1]), cvt_bf16x2(q[2], q[3])});
-      }
-#pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const bf16x8_t a0 = kv8_operand(x.v[t].x, x.v[t].y, x.scale.y);
-      const bf16x8_t a1 = kv8_operand(x.v[t].z, x.v[t].w, x.scale.y);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        acc[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, bp[ct][0], acc[ct][t], 0, 0, 0);
-        acc[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, bp[ct][1], acc[ct][t], 0, 0, 0);
-      }
-    }
+    const int id = page_number(table, min(p, p1 - 1), a.c.pages);
+    return __builtin_amdgcn_readfirstlane(p < p1 ? id : -1);
   };
   // the next page's loads in flight behind this one's work, its number read before
   if (p0 < p1) {
-    Raw x, y;
-    int id = number(p0), next = number(p0 + W), p = p0;
-    load(x, id);
-    for (; p + W < p1; p += W) {
-      load(y, next);
-      const int after = number(p + 2 * W);
-      page(x, id, p);
-      x = y;
-      id = next;
-      next = after;
+    Raw r, s;
+    int next = number(p0 + W), p = p0;
+    load(r, number(p0));
+    auto key = [&](int t, int i) { return r.k[2 * t + i]; };
+    auto value = [&](int t) { return r.v[t]; };
+    for (; p < p1 && !x.masks(p); p += W) {
+      load(s, next);
+      next = number(p + 2 * W);
+      x.add<false>(key, value, r.scale, p, c);
+      r = s;
     }
-    page(x, id, p);
+    for (; p < p1; p += W) {
+      load(s, next);
+      next = number(p + 2 * W);
+      x.add<true>(key, value, r.scale, p, c);
+      r = s;
+    }
   }
 
-  // the waves' sums: lane (c, col) has dimensions 16 t + 4 c + r of its columns
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const float sum = row_pair_sum32(row_pair_sum16(den[ct]));
-    if (c == 0) {
-      wm[wave][16 * ct + l16] = m[ct];
-      wl[wave][16 * ct + l16] = sum;
-    }
-#pragma unroll
-    for (int t = 0; t < 8; ++t)
-      *reinterpret_cast<float4*>(&wacc[wave][16 * ct + l16][16 * t + 4 * c]) =
-          make_float4(acc[ct][t][0], acc[ct][t][1], acc[ct][t][2], acc[ct][t][3]);
+  // the waves' sums
+  const float sum = row_pair_sum32(row_pair_sum16(x.den));
+  if (c == 0) {
+    wm[wave][l16] = x.m;
+    wl[wave][l16] = sum;
   }
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+    *reinterpret_cast<float4*>(&wacc[wave][l16][16 * t + 4 * c]) =
+        make_float4(x.acc[t][0], x.acc[t][1], x.acc[t][2], x.acc[t][3]);
   __syncthreads();
-  for (int e = threadIdx.x; e < kCols * kKvHeadDim / 2; e += W * 64) {
+  for (int e = threadIdx.x; e < 16 * kKvHeadDim / 2; e += W * 64) {
     const int cl = e / (kKvHeadDim / 2), d = e % (kKvHeadDim / 2) * 2;
-    const int cc = tile * kCols + cl;
-    if (cc >= a.tokens * a.group) break;
+    if (cl >= a.tokens * a.group) break;
     float mx = -INFINITY;
 #pragma unroll
     for (int w = 0; w < W; ++w) mx = fmaxf(mx, wm[w][cl]);
-    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+    float all = 0.f, o0 = 0.f, o1 = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       // a wave without rows has m = -inf and sums 0; one whose scores are all NaN
       // has m = -inf and NaN sums, which must count
       const float f = wm[w][cl] == -INFINITY ? 1.f : fast_exp2(wm[w][cl] - mx);
-      sum = fmaf(f, wl[w][cl], sum);
+      all = fmaf(f, wl[w][cl], all);
       o0 = fmaf(f, wacc[w][cl][d], o0);
       o1 = fmaf(f, wacc[w][cl][d + 1], o1);
     }
     if (direct) {
-      const float inv = pages == 0 ? 0.f : 1.f / sum;  // (a sum of 0: every score is -inf)
+      const float inv = pages == 0 ? 0.f : 1.f / all;  // (a sum of 0: every score is -inf)
       reinterpret_cast<uint32_t*>(
-          a.out)[(((size_t)seq * a.tokens + cc / a.group) * nkv * a.group + kvh * a.group +
-                  cc % a.group) * (kKvHeadDim / 2) + d / 2] =
+          a.out)[(((size_t)seq * a.tokens + cl / a.group) * nkv * a.group + kvh * a.group +
+                  cl % a.group) * (kKvHeadDim / 2) + d / 2] =
           f32_to_bf16(o0 * inv) | (f32_to_bf16(o1 * inv) << 16);
     } else {
-      float* o = a.part + ((size_t)blockIdx.x * kCols + cl) * kKvPart;
+      float* o = a.part + (task.part(a) * 16 + cl) * kKvPart;
       if (d == 0) {
         o[0] = mx;
-        o[1] = sum;
+        o[1] = all;
       }
       o[2 + d] = o0;
       o[3 + d] = o1;
@@ -307,18 +328,156 @@ __global__ __launch_bounds__(W * 64) void kv8_attn_kernel(Kv8AttnArgs a) {
   }
 }
 
-// The splits of a column added up: a workgroup per (sequence, column, kv head).
-__global__ __launch_bounds__(kCombine * kKvHeadDim) void kv8_combine_kernel(Kv8AttnArgs a,
-                                                                            int cols) {
+constexpr int kWideWaves = 3;  // waves of a SIMD
+typedef __attribute__((address_space(3))) void lds_void;
+typedef const __attribute__((address_space(1))) void global_void;
+
+// More columns: a workgroup of W waves takes a split's pages one after the other, each
+// wave with 16 columns of its own.  A page goes straight from memory to LDS, the next one
+// while this one is worked on; its 16-byte pieces lie there in an order in which eight
+// neighbouring lanes' are in different banks.  6 sequences of up to 20011 rows with 40
+// columns (135 MB): 38 us, 3.5 TB/s, bound by the wait for a page, of which three or four
+// workgroups of a CU have one each under way.  (Each wave with all 40 columns, padded to
+// 64, in registers: 68 us; two waves to a SIMD, without a spill: 44.)
+template <int W>
+__global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArgs a) {
+  __shared__ uint4 buf_a[2 * kPagePieces], buf_b[2 * kPagePieces];
+  const int nkv = a.c.nkv;
+  const Task task(a);
+  const int split = task.split, kvh = task.kvh, tile = task.tile, seq = task.seq;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+  const int l16 = l & 15, c = l >> 4;
+  const int64_t first = first_of(a, seq);
+  const int pages = tile_pages(a, first, tile, 16 * W);
+  const bool direct = a.splits == 1;
+  const int per = pages_per_split(a, pages);
+  const int p0 = split * per, p1 = min(p0 + per, pages);
+  if (!direct && p0 >= pages) return;
+  const int32_t* table = a.table + (size_t)seq * a.width;
+  const int col0 = tile * 16 * W + 16 * wave;
+  Columns x(a, seq, kvh, first, col0, l16, c);
+
+  // piece s of a buffer: keys of row s / 8, then values of dimension (s - 512) / 4
+  constexpr int kLoads = (2 * kPagePieces / 64 + W - 1) / W;  // of a wave
+  auto fetch = [&](uint4* buf, int id) {
+    const size_t at = (size_t)max(id, 0) * nkv + kvh;
+    const uint4* kp = reinterpret_cast<const uint4*>(a.c.k + at * kPageBytes);
+    const uint4* vp = reinterpret_cast<const uint4*>(a.c.v + at * kPageBytes);
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const int at64 = min(n * W + wave, 2 * kPagePieces / 64 - 1);  // (the last one more than once)
+      const int s = at64 * 64 + l;
+      const uint4* src = at64 < kPagePieces / 64
+                             ? kp + (s & ~7) + ((s ^ (s >> 3)) & 7)
+                             : vp + ((s & ~3) - kPagePieces) + ((s ^ (s >> 3)) & 3);
+      __builtin_amdgcn_global_load_lds((global_void*)src, (lds_void*)(buf + at64 * 64), 16, 0, 0);
+    }
+  };
+  auto number = [&](int p) {
+    return __builtin_amdgcn_readfirstlane(page_number(table, min(p, p1 - 1), a.c.pages));
+  };
+  auto scales = [&](int id) {
+    return id < 0 ? make_float2(0.f, 0.f)
+                  : *reinterpret_cast<const float2*>(a.c.scales + 2 * ((size_t)id * nkv + kvh));
+  };
+  auto add = [&](const uint4* buf, int id, float2 scale, int p) {
+    const uint32_t there = id < 0 ? 0u : ~0u;  // (rows of no page: zeros)
+    auto key = [&](int t, int i) {
+      const int s = key_piece(t, i, l16, c);
+      return buf[(s & ~7) + ((s ^ (s >> 3)) & 7)];
+    };
+    auto value = [&](int t) {
+      const int s = kPagePieces + value_piece(t, l16, c);
+      return buf[(s & ~3) + ((s ^ (s >> 3)) & 3)];
+    };
+    auto masked = [&](uint4 w) {
+      return make_uint4(w.x & there, w.y & there, w.z & there, w.w & there);
+    };
+    if (!x.masks(p) && id >= 0)
+      x.add<false>(key, value, scale, p, c);
+    else
+      x.add<true>([&](int t, int i) { return masked(key(t, i)); },
+                  [&](int t) { return masked(value(t)); }, scale, p, c);
+  };
+  // this wave's pieces have landed, then everybody's, and the other buffer's readers
+  // are through
+  auto landed = [&] {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if (p0 < p1) {
+    int id = number(p0), next = number(p0 + 1);
+    float2 scale = scales(id);
+    fetch(buf_a, id);
+    for (int p = p0; p < p1; p += 2) {
+      landed();
+      float2 after = scales(next);
+      int then = number(p + 2);
+      if (p + 1 < p1) fetch(buf_b, next);
+      add(buf_a, id, scale, p);
+      if (p + 1 >= p1) break;
+      landed();
+      id = then;
+      scale = scales(id);
+      then = number(p + 3);
+      if (p + 2 < p1) fetch(buf_a, id);
+      add(buf_b, next, after, p + 1);
+      next = then;
+    }
+  }
+
+  const float sum = row_pair_sum32(row_pair_sum16(x.den));
+  const int cc = col0 + l16;
+  if (cc >= a.tokens * a.group) return;
+  if (direct) {
+    const float inv = pages == 0 ? 0.f : 1.f / sum;  // (a sum of 0: every score is -inf)
+    uint2* o = reinterpret_cast<uint2*>(
+        a.out + (((size_t)seq * a.tokens + cc / a.group) * nkv * a.group + kvh * a.group +
+                 cc % a.group) * kKvHeadDim);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      o[4 * t + c] = make_uint2(cvt_bf16x2(x.acc[t][0] * inv, x.acc[t][1] * inv),
+                                cvt_bf16x2(x.acc[t][2] * inv, x.acc[t][3] * inv));
+    return;
+  }
+  float* o = a.part + (task.part(a) * 16 * W + 16 * wave + l16) * kKvPart;
+  if (c == 0) {
+    o[0] = x.m;
+    o[1] = sum;
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      *reinterpret_cast<float2*>(o + 2 + 16 * t + 4 * c + 2 * r) =
+          make_float2(x.acc[t][2 * r], x.acc[t][2 * r + 1]);
+}
+
+// The splits of a column (of a sequence and kv head) added up: by a wave where there are
+// few of them, by four, or by a workgroup of 16.  (1920 columns of 21 splits: 6.4 us by
+// four waves each, 9.3 by one, 17 by 16; 40 of 64: 10 by four, 6 by 16.)
+template <int kWaves>
+__global__ __launch_bounds__(kWaves == 16 ? 1024 : 256) void kv8_combine_kernel(Kv8AttnArgs a,
+                                                                                int cols) {
+  __shared__ float2 red[kWaves == 4 ? 4 : 1][64];
   const int nkv = a.c.nkv, all = a.tokens * a.group;
-  const int kvh = blockIdx.x % nkv, cc = blockIdx.x / nkv % all, seq = blockIdx.x / nkv / all;
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
+  const int64_t at = kWaves == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (kWaves == 1 && at >= (int64_t)a.seqs * all * nkv) return;
+  const int kvh = (int)(at % nkv), cc = (int)(at / nkv % all), seq = (int)(at / nkv / all);
   const int tile = cc / cols, cl = cc % cols;
-  const int pages = tile_pages(a, first_of(a, seq), tile, cols);
-  combine_splits(
-      a.part + ((((size_t)seq * a.tiles + tile) * nkv + kvh) * a.splits * cols + cl) * kKvPart,
-      (size_t)cols * kKvPart, (pages + a.per - 1) / a.per,
-      a.out + (((size_t)seq * a.tokens + cc / a.group) * nkv * a.group + kvh * a.group +
-               cc % a.group) * kKvHeadDim);
+  const int pages = tile_pages(a, first_of(a, seq), tile, cols), per = pages_per_split(a, pages);
+  const int ns = (pages + per - 1) / per;
+  const float* base =
+      a.part + ((((size_t)seq * a.tiles + tile) * nkv + kvh) * a.splits * cols + cl) * kKvPart;
+  uint16_t* out = a.out + (((size_t)seq * a.tokens + cc / a.group) * nkv * a.group +
+                           kvh * a.group + cc % a.group) * kKvHeadDim;
+  const size_t stride = (size_t)cols * kKvPart;
+  if (kWaves == 16)
+    combine_splits(base, stride, ns, out);
+  else
+    combine_splits_waves<kWaves == 16 ? 4 : kWaves>(base, stride, ns, kWaves == 1 ? 0 : wave, l,
+                                                    red, out);
 }
 
 // A page of a head expanded for a prompt (dip_attn.h), two blocks of 32 rows: a
@@ -378,28 +537,48 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8Pages a, const int32
     bad[2 * blockIdx.x + tid] = found[tid][0] | found[tid][1] | found[tid][2] | found[tid][3];
 }
 
-// How a launch cuts its work: columns in tiles of 16 ct, a sequence's pages into
-// splits of `per`.
+// How a launch cuts its work: columns in tiles of 16 `waves` (0: up to 16 columns, with
+// the waves taking pages in turn), a sequence's pages into splits of `per` at least.
+//
+// A single sequence's splits are one round of the workgroups that run at once, each with
+// an even share of the pages there are.  Of several sequences, whose lengths only the
+// device knows, a split is a share of the table's width that makes half as many
+// workgroups again as run at once (narrow ones: three times as many), of which those
+// behind a sequence's end leave at once: 32 of up to 16384 rows 118 us, with a round and
+// a third 125; 6 of up to 20011 with 5 tokens each 49, with one round 57, with two 60.
+// Below 8 pages (4 where waves share them) a split costs more for its sums than it saves.
 struct Cut {
-  int ct, tiles, per, splits;
+  int waves, tiles, per, splits;
+  int cols() const { return waves ? 16 * waves : 16; }
   size_t part_bytes(int64_t seqs, int64_t nkv) const {
     return splits == 1 ? 0
-                       : (size_t)seqs * tiles * nkv * splits * 16 * ct * kKvPart * sizeof(float);
+                       : (size_t)seqs * tiles * nkv * splits * cols() * kKvPart * sizeof(float);
   }
 };
+
+constexpr int kMaxWide = 8;
 
 inline Cut cut_for(int64_t seqs, int64_t tokens, int64_t nkv, int64_t group, int64_t width) {
   Cut c;
   const int64_t cols = tokens * group;
-  c.ct = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-  c.tiles = (int)((cols + 16 * c.ct - 1) / (16 * c.ct));
+  c.waves = cols <= 16 ? 0 : (int)min((cols + 15) / 16, (int64_t)kMaxWide);
+  c.tiles = (int)((cols + c.cols() - 1) / c.cols());
   const int64_t heads = seqs * c.tiles * nkv;
-  int64_t per = (width * heads + 1023) / 1024;
-  per = max(min(per, (int64_t)64), (int64_t)4);
-  per = max(per, (width + kMaxSplits - 1) / kMaxSplits);
-  if (width <= 16) per = width;
+  const int64_t cus = device_cus();
+  // workgroups that run at once
+  const int64_t slots = cus * (c.waves ? min(4 * kWideWaves / c.waves, 5) : 2);
+  int64_t per = c.waves ? 4 : 8, splits;
+  if (seqs == 1) {
+    splits = min(max(slots / heads, (int64_t)1), (width + per - 1) / per);
+  } else {
+    const int64_t want = c.waves ? slots * 3 / 2 : 6 * cus;
+    per = max((width * heads + want - 1) / want, per);
+    splits = (width + per - 1) / per;
+  }
+  splits = min(splits, (int64_t)kMaxSplits);
+  if (width <= 16) splits = 1;
   c.per = (int)per;
-  c.splits = (int)((width + per - 1) / per);
+  c.splits = (int)splits;
   return c;
 }
 
@@ -413,31 +592,39 @@ int check_attn(const void* q, const void* out, int64_t seqs, int64_t tokens, int
   return DIP_OK;
 }
 
-template <int W, int CT>
-void launch_tiles(const Kv8AttnArgs& a, int64_t grid, hipStream_t stream) {
-  hipLaunchKernelGGL((kv8_attn_kernel<W, CT>), dim3((unsigned)grid), dim3(64 * W), 0, stream, a);
-}
-
 int launch_attn(Kv8AttnArgs a, const Cut& cut, hipStream_t stream) {
   a.tiles = cut.tiles;
   a.per = cut.per;
   a.splits = cut.splits;
   const int64_t grid = (int64_t)a.seqs * cut.tiles * a.c.nkv * cut.splits;
   const int64_t cols = (int64_t)a.seqs * a.tokens * a.group * a.c.nkv;
-  if (!launch_fits(grid, 512) ||
-      (cut.splits > 1 && !launch_fits(cols, kCombine * kKvHeadDim)))
+  if (!launch_fits(grid, 512) || (cut.splits > 1 && !launch_fits(cols, kCombine * kKvHeadDim)))
     return DIP_ERR_SHAPE;
-  if (cut.ct == 1 && cut.splits == 1)
-    launch_tiles<8, 1>(a, grid, stream);
-  else if (cut.ct == 1)
-    launch_tiles<4, 1>(a, grid, stream);
-  else if (cut.ct == 2)
-    launch_tiles<4, 2>(a, grid, stream);
-  else
-    launch_tiles<4, 4>(a, grid, stream);
-  if (cut.splits > 1)
-    hipLaunchKernelGGL(kv8_combine_kernel, dim3((unsigned)cols), dim3(kCombine * kKvHeadDim), 0,
-                       stream, a, 16 * cut.ct);
+  const dim3 g((unsigned)grid);
+  switch (cut.waves) {
+    case 0:
+      if (cut.splits == 1)
+        hipLaunchKernelGGL(kv8_attn_kernel<8>, g, dim3(512), 0, stream, a);
+      else
+        hipLaunchKernelGGL(kv8_attn_kernel<4>, g, dim3(256), 0, stream, a);
+      break;
+    case 2: hipLaunchKernelGGL(kv8_wide_kernel<2>, g, dim3(128), 0, stream, a); break;
+    case 3: hipLaunchKernelGGL(kv8_wide_kernel<3>, g, dim3(192), 0, stream, a); break;
+    case 4: hipLaunchKernelGGL(kv8_wide_kernel<4>, g, dim3(256), 0, stream, a); break;
+    case 5: hipLaunchKernelGGL(kv8_wide_kernel<5>, g, dim3(320), 0, stream, a); break;
+    case 6: hipLaunchKernelGGL(kv8_wide_kernel<6>, g, dim3(384), 0, stream, a); break;
+    case 7: hipLaunchKernelGGL(kv8_wide_kernel<7>, g, dim3(448), 0, stream, a); break;
+    default: hipLaunchKernelGGL(kv8_wide_kernel<8>, g, dim3(512), 0, stream, a);
+  }
+  if (cut.splits > 32)
+    hipLaunchKernelGGL(kv8_combine_kernel<16>, dim3((unsigned)cols), dim3(1024), 0, stream, a,
+                       cut.cols());
+  else if (cut.splits > 16)
+    hipLaunchKernelGGL(kv8_combine_kernel<4>, dim3((unsigned)cols), dim3(256), 0, stream, a,
+                       cut.cols());
+  else if (cut.splits > 1)
+    hipLaunchKernelGGL(kv8_combine_kernel<1>, dim3((unsigned)((cols + 3) / 4)), dim3(256), 0,
+                       stream, a, cut.cols());
   return hip_status(hipGetLastError());
 }
 
