@@ -1147,7 +1147,7 @@ class KV8Cache:
     its first row, before it is read.  The arrays are checked here, once, so that a call
     need not."""
 
-    __slots__ = ("k", "v", "scales", "device", "n_kv_heads", "pages", "one_layer")
+    __slots__ = ("k", "v", "scales", "device", "n_kv_heads", "pages", "one_layer", "_args")
 
     def __init__(self, k, v, scales):
         dev = _dev(k, v, scales)
@@ -1162,6 +1162,7 @@ class KV8Cache:
         self.k, self.v, self.scales = k, v, scales
         self.device, self.n_kv_heads, self.pages = dev, nkv, pages
         self.one_layer = not lead
+        self._args = (k.data_ptr(), v.data_ptr(), scales.data_ptr(), pages)  # of every call
 
     def layer(self, i: int) -> "KV8Cache":
         return KV8Cache(self.k[i], self.v[i], self.scales[i])
@@ -1180,24 +1181,38 @@ def kv8_cache(n_kv_heads: int, pages: int, device="cuda", layers=None) -> KV8Cac
                     torch.zeros(*lead, 2, dtype=torch.float32, device=device))
 
 
-def _kv8(cache: KV8Cache, table, *ts):
-    """(device, table, its width) of a call over one layer's cache; the tensors must be
-    on the cache's device."""
+def _kv8(cache: KV8Cache, table, pos=None):
+    """(device, table and pos as the library takes them) of a call over one layer's
+    cache; without pos the table is one sequence's."""
     if not isinstance(cache, KV8Cache) or not cache.one_layer:
         raise RuntimeError("cache must be one layer's KV8Cache")
     dev = cache.device
-    for t in (table, *ts):
+    for t in (table,) if pos is None else (table, pos):
         if t.device != dev:
             raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
-    if table.dtype is not torch.int32 or table.dim() not in (1, 2) or not table.shape[-1]:
-        raise RuntimeError("table must be int32 [seqs, pages of a sequence]")
-    return dev, table.contiguous(), table.shape[-1]
+    shape = table.shape
+    if table.dtype is not torch.int32 or len(shape) != (1 if pos is None else 2) or not shape[-1]:
+        raise RuntimeError("table must be int32, " + ("[pages] of one sequence" if pos is None else
+                                                      "[seqs, pages of a sequence]"))
+    if pos is not None:
+        if pos.dtype is not torch.int64 or pos.numel() != shape[0]:
+            raise RuntimeError("pos must be int64, a position for each row of table")
+        pos = pos.contiguous()
+    return dev, table.contiguous(), pos
 
 
-def _positions(pos, table) -> torch.Tensor:
-    if table.dim() != 2 or pos.dtype is not torch.int64 or pos.numel() != table.shape[0]:
-        raise RuntimeError("table must be [seqs, pages], pos int64 with a position for each")
-    return pos.contiguous()
+def _dense_on(dev, *wanted):
+    """_dense of each (tensor, values, name), on that device too."""
+    ptrs = []
+    for t, n, name in wanted:
+        p = t.data_ptr()
+        if t.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
+        if t.dtype is not torch.bfloat16 or t.numel() != n or not t.is_contiguous() or p & 15:
+            raise RuntimeError(f"{name} must be a contiguous, 16-byte aligned bf16 tensor of {n} "
+                               "values")
+        ptrs.append(p)
+    return ptrs
 
 
 def kv8_write(k, v, cache: KV8Cache, table, pos) -> None:
@@ -1206,8 +1221,9 @@ def kv8_write(k, v, cache: KV8Cache, table, pos) -> None:
     of the sequences whose pages table (int32 [seqs, ..]) has.  A negative position
     leaves a sequence out; no two may write to one page.  Rows of a page behind the last
     written no longer stand for anything."""
-    dev, table, width = _kv8(cache, table, k, v, pos)
-    pos, nkv = _positions(pos, table), cache.n_kv_heads
+    (dev, table, pos), nkv = _kv8(cache, table, pos), cache.n_kv_heads
+    if k.device != dev or v.device != dev:
+        raise RuntimeError(f"tensors on different devices: {dev}, {k.device} and {v.device}")
     if k.dim() != 4 or k.shape != v.shape or k.shape[0] != table.shape[0] \
             or tuple(k.shape[2:]) != (nkv, 128) \
             or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
@@ -1220,28 +1236,25 @@ def kv8_write(k, v, cache: KV8Cache, table, pos) -> None:
             for t in (k, v))
     with _on(dev):
         _check(lib.dip_kv8_write(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                 cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
-                                 cache.pages, table.data_ptr(), width, pos.data_ptr(), k.shape[0],
-                                 k.shape[1], nkv, 128, _stream(dev)), "dip_kv8_write")
+                                 *cache._args, table.data_ptr(), table.shape[1], pos.data_ptr(),
+                                 k.shape[0], k.shape[1], nkv, 128, _stream(dev)), "dip_kv8_write")
 
 
 def kv8_read(cache: KV8Cache, table, pos, tokens: int):
     """(k, v) bf16 [seqs, tokens, n_kv_heads, 128]: what the rows of the positions from
     pos (int64 [seqs]) on stand for in one layer's cache, exactly; 0 where a sequence has
     no page, or pos is negative."""
-    dev, table, width = _kv8(cache, table, pos)
-    pos, nkv, tokens = _positions(pos, table), cache.n_kv_heads, int(tokens)
+    (dev, table, pos), nkv, tokens = _kv8(cache, table, pos), cache.n_kv_heads, int(tokens)
     if tokens < 0:
         raise RuntimeError("tokens must not be negative")
-    k, v = torch.empty(2, table.shape[0], tokens, nkv, 128, dtype=torch.bfloat16,
-                       device=dev).unbind(0)
-    if k.numel() == 0:
+    seqs, width = table.shape
+    k, v = torch.empty((2, seqs, tokens, nkv, 128), dtype=torch.bfloat16, device=dev).unbind(0)
+    if seqs * tokens == 0:
         return k, v
     with _on(dev):
-        _check(lib.dip_kv8_read(cache.k.data_ptr(), cache.v.data_ptr(), cache.scales.data_ptr(),
-                                cache.pages, table.data_ptr(), width, pos.data_ptr(),
-                                k.data_ptr(), v.data_ptr(), table.shape[0], tokens, nkv, 128,
-                                _stream(dev)), "dip_kv8_read")
+        _check(lib.dip_kv8_read(*cache._args, table.data_ptr(), width, pos.data_ptr(),
+                                k.data_ptr(), v.data_ptr(), seqs, tokens, nkv, 128, _stream(dev)),
+               "dip_kv8_read")
     return k, v
 
 
@@ -1252,25 +1265,24 @@ def qk_norm_rope_kv8(qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out, cache: KV8Ca
     in pos (int64 [seqs], on the device), q to q_out [seqs, tokens, n_heads * 128].  A
     token at a position that the tables of pages or of cos and sin do not have is left
     out, as is a sequence whose position is negative: its row of q_out stays as it is."""
-    dev, table, width = _kv8(cache, table, qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out)
-    pos, nkv = _positions(pos, table), cache.n_kv_heads
+    (dev, table, pos), nkv = _kv8(cache, table, pos), cache.n_kv_heads
     if n_kv_heads != nkv or n_heads < 1:
         raise RuntimeError(f"the cache has {nkv} kv heads, the call {n_kv_heads}")
-    if qkv.dim() != 3 or qkv.shape[0] != table.shape[0]:
-        raise RuntimeError(f"qkv must be [{table.shape[0]}, tokens, ..]")
-    rows = cos.numel() // 128
+    shape, (seqs, width) = qkv.shape, table.shape
+    if len(shape) != 3 or shape[0] != seqs:
+        raise RuntimeError(f"qkv must be [{seqs}, tokens, ..]")
     if cos.shape != sin.shape or cos.shape[-1] != 128:
         raise RuntimeError("cos and sin must be tables of as many rows of 128 values")
-    seqs, tokens = qkv.shape[:2]
-    ptrs = (_dense(qkv, seqs * tokens * (n_heads + 2 * nkv) * 128, "qkv"),
-            _dense(q_norm_w, 128, "q_norm_w"), _dense(k_norm_w, 128, "k_norm_w"),
-            _dense(cos, rows * 128, "cos"), _dense(sin, rows * 128, "sin"))
-    q_p = _dense(q_out, seqs * tokens * n_heads * 128, "q_out")
-    if seqs * tokens == 0:
+    tokens, values = shape[1], cos.numel()
+    n = seqs * tokens * 128
+    *ptrs, q_p = _dense_on(dev, (qkv, n * (n_heads + 2 * nkv), "qkv"),
+                           (q_norm_w, 128, "q_norm_w"), (k_norm_w, 128, "k_norm_w"),
+                           (cos, values, "cos"), (sin, values, "sin"),
+                           (q_out, n * n_heads, "q_out"))
+    if n == 0:
         return q_out
     with _on(dev):
-        _check(lib.dip_qk_norm_rope_kv8(*ptrs, rows, pos.data_ptr(), q_p, cache.k.data_ptr(),
-                                        cache.v.data_ptr(), cache.scales.data_ptr(), cache.pages,
+        _check(lib.dip_qk_norm_rope_kv8(*ptrs, values // 128, pos.data_ptr(), q_p, *cache._args,
                                         table.data_ptr(), width, seqs, tokens, n_heads, nkv, 128,
                                         eps, _stream(dev)), "dip_qk_norm_rope_kv8")
     return q_out
@@ -1290,28 +1302,25 @@ def kv8_decode_attention(q, cache: KV8Cache, table, pos, out, scale: float, ws=N
     longest sequence's pages is the fastest.  ws: a workspace of
     kv8_decode_attention_workspace_bytes, one for each call that may run at once (None:
     the call's own)."""
-    dev, table, width = _kv8(cache, table, q, pos)
-    pos, nkv, n = _positions(pos, table), cache.n_kv_heads, q.numel()
-    if q.dim() != 3 or q.shape[0] != table.shape[0] or q.shape[2] % (128 * nkv) or not q.shape[2]:
-        raise RuntimeError(f"q must be [{table.shape[0]}, tokens, a multiple of {nkv} heads of "
-                           "128 values]")
-    seqs, tokens, nh = q.shape[0], q.shape[1], q.shape[2] // 128
+    (dev, table, pos), nkv = _kv8(cache, table, pos), cache.n_kv_heads
+    shape, (seqs, width) = q.shape, table.shape
+    if len(shape) != 3 or shape[0] != seqs or shape[2] % (128 * nkv) or not shape[2]:
+        raise RuntimeError(f"q must be [{seqs}, tokens, a multiple of {nkv} heads of 128 values]")
+    tokens, nh = shape[1], shape[2] // 128
+    n = seqs * tokens * nh * 128
     if out is None:
         out = torch.empty_like(q)
-    elif out.device != dev:
-        raise RuntimeError("out must be on q's device")
-    q_p, out_p = _dense(q, n, "q"), _dense(out, n, "out")
+    q_p, out_p = _dense_on(dev, (q, n, "q"), (out, n, "out"))
     if n == 0:
         return out
     with _on(dev):
         ws_p, nbytes, ws = _scratch(
             lib.dip_kv8_decode_attention_workspace_size(seqs, tokens, nh, nkv, 128, width), ws,
             dev, "attention")
-        _check(lib.dip_kv8_decode_attention(q_p, cache.k.data_ptr(), cache.v.data_ptr(),
-                                            cache.scales.data_ptr(), cache.pages,
-                                            table.data_ptr(), width, pos.data_ptr(), out_p, seqs,
-                                            tokens, nh, nkv, 128, scale, ws_p, nbytes,
-                                            _stream(dev)), "dip_kv8_decode_attention")
+        _check(lib.dip_kv8_decode_attention(q_p, *cache._args, table.data_ptr(), width,
+                                            pos.data_ptr(), out_p, seqs, tokens, nh, nkv, 128,
+                                            scale, ws_p, nbytes, _stream(dev)),
+               "dip_kv8_decode_attention")
     return out
 
 
@@ -1320,30 +1329,24 @@ def kv8_prompt_attention(q, cache: KV8Cache, table, start: int, out, scale: floa
     positions start ..), token t over rows 0 .. start + t of the pages in table (int32
     [pages]) of one layer's 8-bit cache -> out (new if None).  ws: as in
     kv8_decode_attention; its size depends on start and the number of tokens."""
-    dev, table, width = _kv8(cache, table, q)
-    nkv, n = cache.n_kv_heads, q.numel()
-    if table.dim() != 1:
-        raise RuntimeError("table must be one sequence's, int32 [pages]")
+    (dev, table, _), nkv = _kv8(cache, table), cache.n_kv_heads
+    width, n = table.shape[0], q.numel()
     if q.dim() != 2 or q.shape[1] % (128 * nkv) or not q.shape[1]:
         raise RuntimeError(f"q must be [tokens, a multiple of {nkv} heads of 128 values]")
     nh = q.shape[1] // 128
     start, tokens = _rows_in(start, q.shape[0], width * KV8_PAGE)
     if out is None:
         out = torch.empty_like(q)
-    elif out.device != dev:
-        raise RuntimeError("out must be on q's device")
-    q_p, out_p = _dense(q, n, "q"), _dense(out, n, "out")
+    q_p, out_p = _dense_on(dev, (q, n, "q"), (out, n, "out"))
     if tokens == 0:
         return out
     with _on(dev):
         ws_p, nbytes, ws = _scratch(
             lib.dip_kv8_prompt_attention_workspace_size(tokens, start, nh, nkv, 128), ws, dev,
             "attention")
-        _check(lib.dip_kv8_prompt_attention(q_p, cache.k.data_ptr(), cache.v.data_ptr(),
-                                            cache.scales.data_ptr(), cache.pages,
-                                            table.data_ptr(), width, start, out_p, tokens, nh,
-                                            nkv, 128, scale, ws_p, nbytes, _stream(dev)),
-               "dip_kv8_prompt_attention")
+        _check(lib.dip_kv8_prompt_attention(q_p, *cache._args, table.data_ptr(), width, start,
+                                            out_p, tokens, nh, nkv, 128, scale, ws_p, nbytes,
+                                            _stream(dev)), "dip_kv8_prompt_attention")
     return out
 
 

@@ -129,6 +129,18 @@ struct Piece {
           f(first + i, load_logit<kType>(row, first + i));
     }
   }
+  // f(index, logit of p's row, logit of q's row) of two rows' pieces at the same place.
+  template <typename F>
+  DIP_DEV static void pairs(const Piece& p, const Piece& q, const char* row, const char* other,
+                            int64_t vocab, F f) {
+    if (p.inside) {
+      float y[kVec];
+      q.tokens(other, vocab, [&](int64_t i, float v) { y[i - q.first] = v; });
+      p.tokens(row, vocab, [&](int64_t i, float x) { f(i, x, y[i - p.first]); });
+    } else {
+      p.tokens(row, vocab, [&](int64_t i, float x) { f(i, x, load_logit<kType>(other, i)); });
+    }
+  }
 };
 
 // f(index, logit) of the tokens in the pieces [v0, v1) by the workgroup's threads,
@@ -189,9 +201,15 @@ struct Weigher {
 
   // The workgroup's `lds` gets the roots; a barrier must follow before their use.
   DIP_DEV Weigher(const SampleArgs& a, uint32_t top_key, uint32_t least_key, double* lds)
-      : per_hi(a.per_hi), per_lo(a.per_lo), least(a.least), roots(lds) {
+      : Weigher(a, put_roots(a, lds), top_key, least_key) {}
+  DIP_DEV static const double* put_roots(const SampleArgs& a, double* lds) {
     if (threadIdx.x < 64)
       lds[threadIdx.x] = __builtin_amdgcn_ldexp(kRoots.v[threadIdx.x], a.shift);
+    return lds;
+  }
+  // `lds` has the roots.
+  DIP_DEV Weigher(const SampleArgs& a, const double* lds, uint32_t top_key, uint32_t least_key)
+      : per_hi(a.per_hi), per_lo(a.per_lo), least(a.least), roots(lds) {
     most = key_value(top_key);
     inf = most == INFINITY;
     if (inf) most = 0.f;
