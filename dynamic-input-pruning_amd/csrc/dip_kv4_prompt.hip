@@ -112,14 +112,17 @@ typedef const __attribute__((address_space(1))) void global_void;
 //     l ^ 32 share a column);
 //   out^T += V^T P^T, the weights rounded to bf16 in place: they are the operand
 //     as they lie.  (Off by 2^-8 of itself at most, as any bf16 weight is.)
-// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 294 us a call, the
-// 4-bit cache's expansion of 8 with it, 0.94 PFLOP/s, where a large product of matrices
-// reaches 1.15 to 1.37 (a trace of 30 calls alone has this launch at 297 to 334).  The
-// MFMAs are busy 49 % of the time and the VALU, the softmax mostly, 56 %; without the
+// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 284 us a call, the
+// 8-bit cache's expansion of 7 with it, 0.97 PFLOP/s, where a large product of matrices
+// reaches 1.2 to 1.37 (a trace of 30 calls alone has this launch longer).  Of 298 the
+// MFMAs were busy 49 % of the time and the VALU, the softmax mostly, 56 %; without the
 // fetch it took 240 us, without the exponentials 336, without the second product 290 (of
 // 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
 // buffers 353; rows through registers into LDS 493; 32 rows to a step and three
-// workgroups to a CU 340 to 346.)
+// workgroups to a CU 340 to 346; 256 columns to a workgroup of 8 waves, four of which
+// multiply while four weigh, a meeting at each change of turns: 278 of then 290, for as
+// much code again; the multiplying waves at a higher priority, or the weighing ones,
+// 289 to 291 for 286.)
 template <bool kSplit>
 __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void prompt_kernel(PromptArgs a) {
   __shared__ uint4 buf_a[kStepBlocks * kBlockVecs], buf_b[kStepBlocks * kBlockVecs];
@@ -196,12 +199,16 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void prompt_kernel(Prom
     // does not attend
     const int behind = t * kTileRows + 4 * h - limit;
     if (masked) {
-      asm volatile("");  // a branch: 64 comparisons and selections that most steps skip
+      int at = behind;
+      // Compared with a value made here, as the compiler takes the comparisons before the
+      // branch otherwise, into every step: 4096 tokens of 64 / 8 heads from 8-bit pages
+      // 286 us for 298, 509 behind 16003 rows 292 for 308.
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int b = 0; b < kStepBlocks; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (behind + 32 * b + 8 * (r >> 2) + (r & 3) >= 0) s[b][r] = -INFINITY;
+          if (at + 32 * b + 8 * (r >> 2) + (r & 3) >= 0) s[b][r] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -243,12 +250,13 @@ __global__ __launch_bounds__(kPromptWaves * 64, kMinWgs) void prompt_kernel(Prom
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[b][r] = fast_exp2(fmaf(s[b][r], by, -base));
     if (masked) {  // weights of 0, whatever a base of +inf or NaN made of them
-      asm volatile("");
+      int at = behind;
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int b = 0; b < kStepBlocks; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (behind + 32 * b + 8 * (r >> 2) + (r & 3) >= 0) s[b][r] = 0.f;
+          if (at + 32 * b + 8 * (r >> 2) + (r & 3) >= 0) s[b][r] = 0.f;
     }
 #pragma unroll
     for (int b = 0; b < kStepBlocks; ++b)
