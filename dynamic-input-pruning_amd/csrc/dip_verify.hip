@@ -26,9 +26,9 @@
 //
 // 5 rows of 151936 bf16 logits, top-k 20 and top-p: 6, 8 and 4.5 us, all waits in a row
 // (by the histogram's launches 39 in all).  16 sequences of 5 drafts over 151936 fp32 with
-// the draft's logits, top-p and min-p (107 MB): 19 for max, the memory; 34 for hist, the
-// weights' instructions; 26 for gather, which reads the rows again for their borders'
-// tokens; 5, 9 and 8 for the rest.  50 of 3 over 32003 bf16, no filter: 16 for the sums, 15
+// the draft's logits, top-p and min-p (107 MB): 18 for max, the memory; 31 for hist, the
+// weights' instructions; 21 for gather, which reads the rows again for their borders'
+// tokens; 5, 10 and 8 for the rest.  50 of 3 over 32003 bf16, no filter: 16 for the sums, 15
 // and 10 (in one workgroup a row 27, 12 and 12, as 350 of them go unevenly onto 256 CUs).
 #include "dip_sample.h"
 
