@@ -136,8 +136,8 @@ def whole_model(args) -> int:
           f"keep={args.keep}", file=sys.stderr, flush=True)
     model, mods = synthetic_model(cfg, args.keep, dev, seed=0)
     plen, gen_new = 32, 64
-    dec = DIPDecoder(model, max_len=plen + max(args.warmup + args.steps, gen_new) + 1,
-                     kv_bits=args.kv_bits)
+    cache = {"kv_dtype": torch.float8_e4m3fn} if args.kv_bits == 8 else {"kv_bits": args.kv_bits}
+    dec = DIPDecoder(model, max_len=plen + max(args.warmup + args.steps, gen_new) + 1, **cache)
     prompt = torch.randint(0, cfg.vocab_size, (1, plen), generator=torch.Generator().manual_seed(0))
     print("[bench] model built; prefill + warmup", file=sys.stderr, flush=True)
     dec.prefill(prompt)
@@ -613,7 +613,7 @@ def main(argv=None):
     ap.add_argument("--eager", action="store_true",
                     help="launch every kernel eagerly instead of replaying the captured graph "
                          "(for counter collection, which profiles each dispatch)")
-    ap.add_argument("--kv-bits", type=int, choices=(4, 16), default=16,
+    ap.add_argument("--kv-bits", type=int, choices=(4, 8, 16), default=16,
                     help="with --whole-model: bits of the cached keys and values")
     ap.add_argument("--whole-model", action="store_true",
                     help="instead of the MLP stack, time greedy decode of a whole synthetic "
