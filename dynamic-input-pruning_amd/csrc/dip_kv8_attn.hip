@@ -454,8 +454,10 @@ __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArg
 }
 
 // The splits of a column (of a sequence and kv head) added up: by a wave where there are
-// few of them, by four, or by a workgroup of 16.  (1920 columns of 21 splits: 6.4 us by
-// four waves each, 9.3 by one, 17 by 16; 40 of 64: 10 by four, 6 by 16.)
+// few of them, by four, or by a workgroup of 16, which fewer splits are worth where all of
+// these run at once, two to a CU.  (1920 columns of 21 splits: 6.4 us by four waves each,
+// 9.3 by one, 17 by 16; 40 of 64: 10 by four, 6 by 16; 64 of 16: 9.1 by one, 4.7 by 16; a
+// whole call with 512 of 4: 14.8 by one, 16 by 16.)
 template <int kWaves>
 __global__ __launch_bounds__(kWaves == 16 ? 1024 : 256) void kv8_combine_kernel(Kv8AttnArgs a,
                                                                                 int cols) {
@@ -546,7 +548,8 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8Pages a, const int32
 // workgroups again as run at once (narrow ones: three times as many), of which those
 // behind a sequence's end leave at once: 32 of up to 16384 rows 118 us, with a round and
 // a third 125; 6 of up to 20011 with 5 tokens each 49, with one round 57, with two 60.
-// Below 8 pages (4 where waves share them) a split costs more for its sums than it saves.
+// A split has a page for each wave at least, of several sequences 8: 4000 rows of one 12.9
+// us with 4 for 14.4 with 8, 20011 rows 17.1 for 18.8; 8 sequences of 2000 17.0 for 14.8.
 struct Cut {
   int waves, tiles, per, splits;
   int cols() const { return waves ? 16 * waves : 16; }
@@ -567,7 +570,7 @@ inline Cut cut_for(int64_t seqs, int64_t tokens, int64_t nkv, int64_t group, int
   const int64_t cus = device_cus();
   // workgroups that run at once
   const int64_t slots = cus * (c.waves ? min(4 * kWideWaves / c.waves, 5) : 2);
-  int64_t per = c.waves ? 4 : 8, splits;
+  int64_t per = c.waves || seqs == 1 ? 4 : 8, splits;
   if (seqs == 1) {
     splits = min(max(slots / heads, (int64_t)1), (width + per - 1) / per);
   } else {
@@ -616,7 +619,7 @@ int launch_attn(Kv8AttnArgs a, const Cut& cut, hipStream_t stream) {
     case 7: hipLaunchKernelGGL(kv8_wide_kernel<7>, g, dim3(448), 0, stream, a); break;
     default: hipLaunchKernelGGL(kv8_wide_kernel<8>, g, dim3(512), 0, stream, a);
   }
-  if (cut.splits > 32)
+  if (cut.splits > 32 || (cut.splits > 8 && cols <= 2 * device_cus()))
     hipLaunchKernelGGL(kv8_combine_kernel<16>, dim3((unsigned)cols), dim3(1024), 0, stream, a,
                        cut.cols());
   else if (cut.splits > 16)
