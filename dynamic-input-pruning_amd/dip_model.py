@@ -726,7 +726,9 @@ class DIPDecoder:
         accepts those that are the dense model's too and chooses the one behind them.
         `self.drafts` then has the numbers of accepted and of drafted tokens.  It needs
         a cache of 4 or 8 bits, which a pass of several tokens can go on from, with
-        room for `draft` tokens behind the last."""
+        room for `draft` tokens behind the last.  (A page of 8 bits keeps the scale that
+        refused drafts' keys or values may have raised, and with it the rounding of its
+        numbers below 2^-14 of the largest.)"""
         if draft:
             return self._generate_drafted(input_ids, max_new_tokens, eos_token_id, return_logits,
                                           int(draft), do_sample,
