@@ -3,6 +3,8 @@
 // the device, and of a prompt's tokens.
 #include "dip_kv8.h"
 
+#include <type_traits>
+
 namespace dip {
 namespace {
 
@@ -336,9 +338,10 @@ typedef const __attribute__((address_space(1))) void global_void;
 // wave with 16 columns of its own.  A page goes straight from memory to LDS, the next one
 // while this one is worked on; its 16-byte pieces lie there in an order in which eight
 // neighbouring lanes' are in different banks.  6 sequences of up to 20011 rows with 40
-// columns (135 MB): 38 us, 3.5 TB/s, bound by the wait for a page, of which three or four
+// columns (135 MB): 37 us, 3.6 TB/s, bound by the wait for a page, of which three or four
 // workgroups of a CU have one each under way.  (Each wave with all 40 columns, padded to
-// 64, in registers: 68 us; two waves to a SIMD, without a spill: 44.)
+// 64, in registers: 68 us; masked pages and others in one loop, which spills: 39, a
+// whole call 49 for 43; two pages under way, whose three buffers leave room for fewer workgroups: 10 us more.)
 template <int W>
 __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArgs a) {
   __shared__ uint4 buf_a[2 * kPagePieces], buf_b[2 * kPagePieces];
@@ -380,8 +383,7 @@ __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArg
     return id < 0 ? make_float2(0.f, 0.f)
                   : *reinterpret_cast<const float2*>(a.c.scales + 2 * ((size_t)id * nkv + kvh));
   };
-  auto add = [&](const uint4* buf, int id, float2 scale, int p) {
-    const uint32_t there = id < 0 ? 0u : ~0u;  // (rows of no page: zeros)
+  auto add = [&](auto masked, const uint4* buf, int id, float2 scale, int p) {
     auto key = [&](int t, int i) {
       const int s = key_piece(t, i, l16, c);
       return buf[(s & ~7) + ((s ^ (s >> 3)) & 7)];
@@ -390,14 +392,16 @@ __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArg
       const int s = kPagePieces + value_piece(t, l16, c);
       return buf[(s & ~3) + ((s ^ (s >> 3)) & 3)];
     };
-    auto masked = [&](uint4 w) {
-      return make_uint4(w.x & there, w.y & there, w.z & there, w.w & there);
-    };
-    if (!x.masks(p) && id >= 0)
+    if constexpr (decltype(masked)::value) {
+      const uint32_t there = id < 0 ? 0u : ~0u;  // (rows of no page: zeros)
+      auto kept = [&](uint4 w) {
+        return make_uint4(w.x & there, w.y & there, w.z & there, w.w & there);
+      };
+      x.add<true>([&](int t, int i) { return kept(key(t, i)); },
+                  [&](int t) { return kept(value(t)); }, scale, p, c);
+    } else {
       x.add<false>(key, value, scale, p, c);
-    else
-      x.add<true>([&](int t, int i) { return masked(key(t, i)); },
-                  [&](int t) { return masked(value(t)); }, scale, p, c);
+    }
   };
   // this wave's pieces have landed, then everybody's, and the other buffer's readers
   // are through
@@ -409,20 +413,27 @@ __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArg
     int id = number(p0), next = number(p0 + 1);
     float2 scale = scales(id);
     fetch(buf_a, id);
-    for (int p = p0; p < p1; p += 2) {
+    int p = p0, at = 0;  // a page, and the buffer that it is in
+    auto turn = [&](auto masked, const uint4* cur, uint4* free) {
+      if (p >= p1 || (!decltype(masked)::value && (x.masks(p) || id < 0))) return false;
       landed();
-      float2 after = scales(next);
-      int then = number(p + 2);
-      if (p + 1 < p1) fetch(buf_b, next);
-      add(buf_a, id, scale, p);
-      if (p + 1 >= p1) break;
-      landed();
-      id = then;
-      scale = scales(id);
-      then = number(p + 3);
-      if (p + 2 < p1) fetch(buf_a, id);
-      add(buf_b, next, after, p + 1);
-      next = then;
+      const float2 after = scales(next);
+      const int then = number(p + 2);
+      if (p + 1 < p1) fetch(free, next);
+      add(masked, cur, id, scale, p);
+      id = next, next = then, scale = after;
+      ++p;
+      return true;
+    };
+    // The pages that all of the wave's columns attend, then the others.  (A wave changes
+    // loops by itself: each meets the others once a page in both.)
+    while (turn(std::false_type{}, buf_a, buf_b) && (at = 1, turn(std::false_type{}, buf_b, buf_a)))
+      at = 0;
+    for (; p < p1; at ^= 1) {
+      if (at == 0)
+        turn(std::true_type{}, buf_a, buf_b);
+      else
+        turn(std::true_type{}, buf_b, buf_a);
     }
   }
 
@@ -547,7 +558,9 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8Pages a, const int32
 // device knows, a split is a share of the table's width that makes half as many
 // workgroups again as run at once (narrow ones: three times as many), of which those
 // behind a sequence's end leave at once: 32 of up to 16384 rows 118 us, with a round and
-// a third 125; 6 of up to 20011 with 5 tokens each 49, with one round 57, with two 60.
+// a third 125; 6 of up to 20011 with 5 tokens each 45, with one round 54, with two 64; with
+// 3 tokens each 40, 42 and 56 (of two waves' workgroups five fit a CU, four are counted:
+// with five 55).
 // A split has a page for each wave at least, of several sequences 8: 4000 rows of one 12.9
 // us with 4 for 14.4 with 8, 20011 rows 17.1 for 18.8; 8 sequences of 2000 17.0 for 14.8.
 struct Cut {
@@ -569,7 +582,7 @@ inline Cut cut_for(int64_t seqs, int64_t tokens, int64_t nkv, int64_t group, int
   const int64_t heads = seqs * c.tiles * nkv;
   const int64_t cus = device_cus();
   // workgroups that run at once
-  const int64_t slots = cus * (c.waves ? min(4 * kWideWaves / c.waves, 5) : 2);
+  const int64_t slots = cus * (c.waves ? min(4 * kWideWaves / c.waves, 4) : 2);
   int64_t per = c.waves || seqs == 1 ? 4 : 8, splits;
   if (seqs == 1) {
     splits = min(max(slots / heads, (int64_t)1), (width + per - 1) / per);
