@@ -341,7 +341,8 @@ typedef const __attribute__((address_space(1))) void global_void;
 // columns (135 MB): 37 us, 3.6 TB/s, bound by the wait for a page, of which three or four
 // workgroups of a CU have one each under way.  (Each wave with all 40 columns, padded to
 // 64, in registers: 68 us; masked pages and others in one loop, which spills: 39, a
-// whole call 49 for 43; two pages under way, whose three buffers leave room for fewer workgroups: 10 us more.)
+// whole call 49 for 43; two pages under way, whose three buffers leave room for fewer
+// workgroups: 10 more.)
 template <int W>
 __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArgs a) {
   __shared__ uint4 buf_a[2 * kPagePieces], buf_b[2 * kPagePieces];
