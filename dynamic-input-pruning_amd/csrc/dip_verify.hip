@@ -831,16 +831,9 @@ inline bool sizes_ok(int64_t seqs, int64_t tokens, int64_t vocab) {
          vocab <= (1 << 30) && launch_fits(seqs * (2 * tokens + 1), 1024);
 }
 
-}  // namespace
-}  // namespace dip
-
-using namespace dip;
-
-// For fp32 logits, which take the most slices, and any filters.
-extern "C" size_t dip_verify_workspace_size(int64_t seqs, int64_t tokens, int64_t vocab,
-                                            int draft_logits) {
-  if (!sizes_ok(seqs, tokens, vocab) || seqs == 0) return 0;
-  const int64_t rows = rows_of(seqs, tokens, draft_logits != 0), vecs = max_vecs(vocab, 4);
+// For `rows` rows of any type (fp32 rows take the most slices) and any filters.
+inline size_t workspace_of(int64_t seqs, int64_t rows, int64_t vocab) {
+  const int64_t vecs = max_vecs(vocab, 4);
   size_t n = (size_t)seqs * slices_for(seqs, vecs) * 16;
   if (vecs > kOneLaunch)
     n += (size_t)rows *
@@ -852,6 +845,20 @@ extern "C" size_t dip_verify_workspace_size(int64_t seqs, int64_t tokens, int64_
                    (size_t)rows * sum_slices(rows, w) * sizeof(Part));
   }
   return up16(rows * sizeof(Border)) + up16(seqs * sizeof(Decided)) + n;
+}
+
+}  // namespace
+}  // namespace dip
+
+using namespace dip;
+
+extern "C" size_t dip_verify_workspace_size(int64_t seqs, int64_t tokens, int64_t vocab,
+                                            int draft_logits) {
+  if (!sizes_ok(seqs, tokens, vocab) || seqs == 0) return 0;
+  // fewer rows may be cut finer, and greedy calls do without the draft's
+  size_t n = workspace_of(seqs, rows_of(seqs, tokens, false), vocab);
+  if (draft_logits) n = max(n, workspace_of(seqs, rows_of(seqs, tokens, true), vocab));
+  return n;
 }
 
 extern "C" int dip_verify(const void* logits, int dtype, int64_t seqs, int64_t tokens,
