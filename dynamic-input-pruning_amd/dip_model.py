@@ -533,17 +533,17 @@ class DIPDecoder:
             out.append(q.as_strided((sum(t.shape[0] for t in ts), q.shape[1]), q.stride()))
         return tuple(out)
 
-    def _prefill_fused(self, ids: torch.Tensor) -> torch.Tensor:
+    def _prefill_fused(self, ids: torch.Tensor, dense: bool = False) -> torch.Tensor:
         """prefill with the decode kernels' prompt forms around the
         projections: one q|k|v product; q/k norm, rotary embedding and the
         static cache's rows in one launch; residual add and RMSNorm in one; and
         the head for the last token alone.  With a quantised cache the prompt goes
-        through the layers in parts of even length."""
+        through the layers in parts of even length.  `dense`: as in _prefill_part."""
         K, plen = self._K, ids.shape[1]
         parts = 1 if self.kv_bits == 16 else -(-plen // _PROMPT_CHUNK)
         ends = [plen * (j + 1) // parts for j in range(parts)]
         for start, end in zip([0] + ends, ends):
-            h, y = self._prefill_part(ids[:, start:end], start)
+            h, y = self._prefill_part(ids[:, start:end], start, dense)
         n = self.model.model.norm
         last = torch.empty(self.hidden, dtype=self.dtype, device=self.device)
         K.add_rmsnorm(h[-1], y[-1], n.weight, last, n.variance_epsilon)
@@ -551,9 +551,10 @@ class DIPDecoder:
         self.pos.fill_(plen)
         return logits
 
-    def _prefill_part(self, ids: torch.Tensor, start: int):
+    def _prefill_part(self, ids: torch.Tensor, start: int, dense: bool = False):
         """The tokens of a prompt, or more than one behind it, from position `start`
-        through every layer (start 0 with a bf16 cache); (residual, last MLP's output)."""
+        through every layer (start 0 with a bf16 cache); (residual, last MLP's output).
+        The MLPs take a single token for a step's and prune it; `dense`: not here."""
         from qlinear import int4_linear
         K, inner, hd, nh = self._K, self.model.model, self.hd, self.nh
         plen = ids.shape[1]
@@ -592,7 +593,8 @@ class DIPDecoder:
                     enable_gqa=nh != self.nkv)
                 o = a.o_proj(o.transpose(1, 2).reshape(1, plen, nh * hd))
             K.add_rmsnorm_rows(h, o.reshape(plen, -1), pn.weight, x, pn.variance_epsilon)
-            y = L.mlp(x.view(1, plen, -1)).reshape(plen, -1)
+            # (the pruned route is for [.., 1, hidden] alone)
+            y = L.mlp(x if dense and plen == 1 else x.view(1, plen, -1)).reshape(plen, -1)
         return h, y
 
     # -- one decode step (device-side token and position) ---------------------
@@ -721,7 +723,7 @@ class DIPDecoder:
         logits of every generated token, before any of these.
 
         With `draft` n > 0 the tokens are the dense model's, as prompts run through
-        it: n pruned steps draft a token each, drawn as the settings say, one pass of
+        it (here one of a single token too): n pruned steps draft a token each, drawn as the settings say, one pass of
         n + 1 tokens through the dense route gives their logits, and _dip_hip.verify
         accepts those that are the dense model's too and chooses the one behind them.
         `self.drafts` then has the numbers of accepted and of drafted tokens.  It needs
@@ -758,9 +760,9 @@ class DIPDecoder:
 
     def _generate_drafted(self, input_ids, max_new_tokens: int, eos_token_id, return_logits: bool,
                           draft: int, do_sample: bool, how: dict, generator):
-        """generate with drafted tokens (see there).  Every pass of the dense route has
-        draft + 1 tokens, of which the ones behind the last wanted are dropped: a single
-        token would take the pruned step."""
+        """generate with drafted tokens (see there).  Every pass of the dense route behind
+        the prompt has draft + 1 tokens, of which the ones behind the last wanted are
+        dropped."""
         if draft < 0 or self.kv_bits == 16 or not self._prefill_fusible():
             raise ValueError(f"draft must not be negative: {draft}" if draft < 0 else
                              "drafting needs a cache of 4 or 8 bits, and prompts on the fused "
@@ -771,6 +773,8 @@ class DIPDecoder:
         K.check_sampling(**how)
         ids = input_ids.to(dev).view(1, -1)
         plen = ids.shape[1]
+        if plen < 1:
+            raise ValueError("an empty prompt")
         if plen + max_new_tokens + draft > self.max_len:
             raise ValueError(f"{plen} + {max_new_tokens} tokens and {draft} drafted ones exceed "
                              f"max_len {self.max_len}")
@@ -784,7 +788,7 @@ class DIPDecoder:
         try:
             if do_sample:
                 self._draw = iter(rand(1).split(1)), how
-            last = self.prefill(ids)
+            last = self._prefill_fused(ids, dense=True)
             if max_new_tokens > 0:
                 tokens.append(int(self.tok))
                 logs.append(last.view(-1).float())
