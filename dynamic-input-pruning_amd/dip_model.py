@@ -27,6 +27,7 @@ The step uses the model's own modules, so the decode math is the HF model's
 """
 from __future__ import annotations
 
+import math
 from pathlib import Path
 
 import torch
@@ -722,16 +723,18 @@ class DIPDecoder:
         `min_p` of the largest (_dip_hip.sample).  With `return_logits` also the
         logits of every generated token, before any of these.
 
-        With `draft` n > 0 the tokens are the dense model's, as prompts run through
-        it (here one of a single token too): n pruned steps draft a token each, drawn as the settings say, one pass of
-        n + 1 tokens through the dense route gives their logits, and _dip_hip.verify
-        accepts those that are the dense model's too and chooses the one behind them.
-        `self.drafts` then has the numbers of accepted and of drafted tokens.  It needs
-        a cache of 4 or 8 bits, which a pass of several tokens can go on from, with
-        room for `draft` tokens behind the last.  (A page of 8 bits keeps the scale that
-        refused drafts' keys or values may have raised, and with it the rounding of its
-        numbers below 2^-14 of the largest.)"""
+        With `draft` n > 0, a whole number, the tokens are the dense model's, as prompts
+        run through it (here one of a single token too): n pruned steps draft a token
+        each, drawn as the settings say, one pass of n + 1 tokens through the dense route
+        gives their logits, and _dip_hip.verify accepts those that are the dense model's
+        too and chooses the one behind them.  `self.drafts` then has the numbers of
+        accepted and of drafted tokens.  It needs a cache of 4 or 8 bits, which a pass of
+        several tokens can go on from, with room for `draft` tokens behind the last.  (A
+        page of 8 bits keeps the scale that refused drafts' keys or values may have
+        raised, and with it the rounding of its numbers below 2^-14 of the largest.)"""
         if draft:
+            if not math.isfinite(draft) or draft < 0 or int(draft) != draft:
+                raise ValueError(f"draft must be a whole number >= 0, got {draft}")
             return self._generate_drafted(input_ids, max_new_tokens, eos_token_id, return_logits,
                                           int(draft), do_sample,
                                           dict(temperature=temperature, top_k=top_k, top_p=top_p,
@@ -763,9 +766,8 @@ class DIPDecoder:
         """generate with drafted tokens (see there).  Every pass of the dense route behind
         the prompt has draft + 1 tokens, of which the ones behind the last wanted are
         dropped."""
-        if draft < 0 or self.kv_bits == 16 or not self._prefill_fusible():
-            raise ValueError(f"draft must not be negative: {draft}" if draft < 0 else
-                             "drafting needs a cache of 4 or 8 bits, and prompts on the fused "
+        if self.kv_bits == 16 or not self._prefill_fusible():
+            raise ValueError("drafting needs a cache of 4 or 8 bits, and prompts on the fused "
                              "kernels")
         K, dev = self._K, self.device
         if not do_sample:
