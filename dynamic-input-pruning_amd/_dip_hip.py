@@ -1263,8 +1263,9 @@ def qk_norm_rope_kv8(qkv, q_norm_w, k_norm_w, cos, sin, pos, q_out, cache: KV8Ca
     """qk_norm_rope_cache for the tokens of several sequences, into their pages of one
     layer's 8-bit cache: qkv [seqs, tokens, ..], the first token of each at the position
     in pos (int64 [seqs], on the device), q to q_out [seqs, tokens, n_heads * 128].  A
-    token at a position that the tables of pages or of cos and sin do not have is left
-    out, as is a sequence whose position is negative: its row of q_out stays as it is."""
+    token at a position that the table of cos and sin does not have, or in a page that the
+    table of pages does not, is left out, as is a sequence whose position is negative: its
+    row of q_out stays as it is."""
     (dev, table, pos), nkv = _kv8(cache, table, pos), cache.n_kv_heads
     if n_kv_heads != nkv or n_heads < 1:
         raise RuntimeError(f"the cache has {nkv} kv heads, the call {n_kv_heads}")

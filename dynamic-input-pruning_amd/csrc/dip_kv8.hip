@@ -111,10 +111,12 @@ __global__ __launch_bounds__(64 * kWriteWaves) void kv8_write_kernel(Kv8WriteArg
     if (tok >= (int64_t)a.seqs * a.tokens) return;
     const int64_t s = tok / a.tokens, t = tok % a.tokens, first = a.pos[s];
     if (first < 0 || first >= a.rows - t) return;
+    // (read beside the token's values, for the write behind them)
+    const int id = page_number(a.table + s * a.width, (first + t) / kPageRows, a.c.pages);
     uint32_t x[4] = {0u, 0u, 0u, 0u};
     if (head < a.nh) load_head(x, a.k + s * a.k_seq + t * a.k_tok + head * kKvHeadDim + 8 * i, true);
     head_norm_rope(x, a.q_w, a.cos_t, a.sin_t, first + t, i, a.eps);
-    if (head < a.nh)
+    if (head < a.nh && id >= 0)
       reinterpret_cast<uint4*>(a.q_out)[(tok * a.nh + head) * 16 + i] =
           make_uint4(x[0], x[1], x[2], x[3]);
     return;
