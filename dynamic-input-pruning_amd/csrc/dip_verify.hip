@@ -10,9 +10,17 @@
 //   with u_n; behind n accepted ones from p_n.
 // The tokens are then distributed as if each had been drawn from p.
 //
-// A row's weights are dip_sample's whole numbers, exact in sum, so the share of a token
-// is a quotient of two of them.  What is left of p where q is taken away is held in whole
-// numbers of 2^-51.
+// A row's weights are dip_sample's whole numbers, so a token's share is a quotient: its
+// weight over the row's sum.  With filters the sum is exact, in any order.  Without any it
+// is put together of the slices' sums, each of weights by the slice's own largest logit,
+// in 64-bit floating point: off by 2^-30 of itself as a weight and a slice's factor are
+// (4e-10 each), and by what the weights' rounding to whole numbers does, which is finer
+// against a smaller largest logit (half a unit of 2^-43 for each of 2^19 tokens, the most
+// that go this way: 2^-25).  By that much the sum may be another one where the call's
+// number of rows cuts them otherwise, and a draft whose u q lies that near to p taken or
+// refused.  (Exact here too would take the largest logit of the whole row first, a launch
+// and a reading of the rows more.)  What is left of p where q is taken away is held in
+// whole numbers of 2^-51.
 //
 // Launches: the border and the sum of the weights that the filters keep, for every row
 // at once (in one launch where rows fit a workgroup's registers, else in slices, as

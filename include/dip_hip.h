@@ -837,7 +837,10 @@ int dip_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64
  * largest logits are accepted, draft_logits and u are not read.  A row with nothing to
  * choose from accepts nothing and gives token 0.  tokens >= 0; logits, types and filters
  * as dip_sample's; seqs * (2 tokens + 1) below 2^22.  What is left of p is summed in whole
- * numbers of 2^-51.  The workspace needs no clearing; calls that may run at once need
+ * numbers of 2^-51.  Without filters a row's sum is put together of
+ * parts, which the call's number of rows cuts: it may depend on that by 2^-30 of itself
+ * (2^-24 at the very most, where thousands of tokens are hardly likelier than none), and
+ * so may a draft whose u * q_t lies that near to p_t.  The workspace needs no clearing; calls that may run at once need
  * one each.  The reference has no counterpart.
  */
 size_t dip_verify_workspace_size(int64_t seqs, int64_t tokens, int64_t vocab, int draft_logits);
