@@ -61,6 +61,16 @@ struct Task {
 // What a wave has of 16 columns, each a (token, query head) of one kv head of a
 // sequence: lane (c, l16) of column l16 the queries' operand, the sums of dimensions 16 t
 // + 4 c + r, and the softmax's base and sum.
+//
+// kFine: the weights in two bf16 parts, off by 2^-17 of each, for a second product of
+// each 32 rows; else in one, off by 2^-8 of each at most.  Where memory bounds the kernel
+// the second product is hidden: 1 token over 701 rows 9.6 us for 9.3, of 32 sequences of up
+// to 16384 118.7 for 118.1, over 131071 57.4 for 56.7, and the results are those of 32-bit
+// weights but for some of the result's own roundings.  Where the products and the softmax
+// bound it it is not: 5 tokens of 6 sequences of up to 20011 47.9 for 43.1, a prompt of
+// 4096 379 for 284, 509 tokens behind 16003 386 for 292.  Those keep one part, as the
+// attention over the 4-bit cache does.
+template <bool kFine>
 struct Columns {
   bf16x8_t q[4];
   floatx4 acc[8];
@@ -101,8 +111,8 @@ struct Columns {
   //     up with the scores of rows 16 t + 4 c + r;
   //   softmax against a base that follows the running maximum (the columns' lanes agree
   //     on it by two lane swaps) in fp32;
-  //   values^T: A = 16 dimensions of 32 rows, B = the weights rounded to bf16 (off by
-  //     2^-8 of each at most) where the scores are.
+  //   values^T: A = 16 dimensions of 32 rows, B = the weights in bf16 parts where the
+  //     scores are.
   // Keys and values become bf16 times their page's scale on the way, two to an
   // instruction.
   template <bool kMasked, typename K, typename V>
@@ -152,19 +162,23 @@ struct Columns {
       for (int e = 0; e < 16; ++e)
         if (row + 16 * (e >> 2) + (e & 3) >= limit) s[e >> 2][e & 3] = 0.f;
     }
-    bf16x8_t p[2];
+    bf16x8_t p[2], rest[2] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float(&x)[4] = s[2 * h], (&y)[4] = s[2 * h + 1];
 #pragma unroll
       for (int r = 0; r < 4; ++r) den += x[r] + y[r];
-      p[h] = __builtin_bit_cast(bf16x8_t,
-                                u32x4_t{cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]),
-                                        cvt_bf16x2(y[0], y[1]), cvt_bf16x2(y[2], y[3])});
+      const u32x4_t w{cvt_bf16x2(x[0], x[1]), cvt_bf16x2(x[2], x[3]), cvt_bf16x2(y[0], y[1]),
+                      cvt_bf16x2(y[2], y[3])};
+      p[h] = __builtin_bit_cast(bf16x8_t, w);
+      if (kFine)
+        rest[h] = __builtin_bit_cast(bf16x8_t,
+                                     u32x4_t{left_of(x[0], x[1], w[0]), left_of(x[2], x[3], w[1]),
+                                             left_of(y[0], y[1], w[2]), left_of(y[2], y[3], w[3])});
     }
     if (!kMasked) {
 #pragma unroll
-      for (int t = 0; t < 8; ++t) product(t, values(t), p, scale.y);
+      for (int t = 0; t < 8; ++t) product(t, values(t), p, rest, scale.y);
       return;
     }
     // A NaN counts for the columns that attend its row alone: it is taken out of the values,
@@ -173,7 +187,7 @@ struct Columns {
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       const uint4 w = values(t), n = nans(w);
-      product(t, make_uint4(w.x & ~n.x, w.y & ~n.y, w.z & ~n.z, w.w & ~n.w), p, scale.y);
+      product(t, make_uint4(w.x & ~n.x, w.y & ~n.y, w.z & ~n.z, w.w & ~n.w), p, rest, scale.y);
       if (!__any((n.x | n.y | n.z | n.w) != 0u)) continue;
       bf16x8_t there[2];
 #pragma unroll
@@ -201,11 +215,18 @@ struct Columns {
     return make_uint4(kv8_nan_bytes(w.x), kv8_nan_bytes(w.y), kv8_nan_bytes(w.z),
                       kv8_nan_bytes(w.w));
   }
-  DIP_DEV void product(int t, uint4 w, const bf16x8_t (&p)[2], float scale) {
-    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(w.x, w.y, scale), p[0], acc[t], 0,
-                                                     0, 0);
-    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kv8_operand(w.z, w.w, scale), p[1], acc[t], 0,
-                                                     0, 0);
+  // What rounding to bf16 (a pair, in w) leaves of x and y, as bf16 too.
+  DIP_DEV static uint32_t left_of(float x, float y, uint32_t w) {
+    return cvt_bf16x2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xFFFF0000u));
+  }
+  DIP_DEV void product(int t, uint4 w, const bf16x8_t (&p)[2], const bf16x8_t (&rest)[2],
+                       float scale) {
+    const bf16x8_t lo = kv8_operand(w.x, w.y, scale), hi = kv8_operand(w.z, w.w, scale);
+    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[0], acc[t], 0, 0, 0);
+    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[1], acc[t], 0, 0, 0);
+    if (!kFine) return;
+    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[0], acc[t], 0, 0, 0);
+    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[1], acc[t], 0, 0, 0);
   }
 };
 
@@ -241,7 +262,7 @@ __global__ __launch_bounds__(W * 64) void kv8_attn_kernel(Kv8AttnArgs a) {
   if (!direct && split * per >= pages) return;
   const int p0 = split * per + wave, p1 = min(split * per + per, pages);
   const int32_t* table = a.table + (size_t)seq * a.width;
-  Columns x(a, seq, kvh, first, 0, l16, c);
+  Columns<true> x(a, seq, kvh, first, 0, l16, c);
 
   struct Raw {
     uint4 k[8], v[8];
@@ -359,7 +380,7 @@ __global__ __launch_bounds__(W * 64, kWideWaves) void kv8_wide_kernel(Kv8AttnArg
   if (!direct && p0 >= pages) return;
   const int32_t* table = a.table + (size_t)seq * a.width;
   const int col0 = tile * 16 * W + 16 * wave;
-  Columns x(a, seq, kvh, first, col0, l16, c);
+  Columns<false> x(a, seq, kvh, first, col0, l16, c);
 
   // piece s of a buffer: keys of row s / 8, then values of dimension (s - 512) / 4
   constexpr int kLoads = (2 * kPagePieces / 64 + W - 1) / W;  // of a wave

@@ -772,7 +772,8 @@ int dip_qk_norm_rope_kv8(const uint16_t* qkv, const uint16_t* q_norm_w, const ui
  * table [table_width]) at positions start .. start + tokens - 1, which the table must
  * have, token t over rows 0 .. start + t.
  * Types, sums and what is not finite as with dip_kv4_decode_attention, but for the
- * weights: they are rounded to bf16 without the values' scales.  Workspaces need no
+ * weights.  Of up to 16 columns (tokens * n_heads / n_kv_heads) they are two bf16 numbers
+ * each, off by 2^-17 of it, else one, without the values' scales, off by 2^-8 at most.  Workspaces need no
  * clearing; calls that may run at once need one each.
  */
 size_t dip_kv8_decode_attention_workspace_size(int64_t seqs, int64_t tokens, int64_t n_heads,
