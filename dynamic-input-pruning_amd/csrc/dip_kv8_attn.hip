@@ -594,7 +594,13 @@ struct Cut {
   }
 };
 
-constexpr int kMaxWide = 8;
+// More waves share a page's fetch, and fewer such workgroups fit a CU and wait for pages
+// by turns: of 4 waves at most, and of 8, 80 columns of 1 sequence of 20000 rows of 64 / 8
+// heads 33 us and 35, 128 35 and 33, 256 50 and 54; of 6 sequences of up to 20000 rows 79 and
+// 90, 80 and 91, 142 and 174; of 32 of up to 6000 119 and 136, 127 and 143, 193 and 197; of
+// 16 / 2 heads 6 sequences 35 and 47, 40 and 46, 50 and 87.  (Of 3 at most 64 columns 70 for
+// 51 and 96 for 70 in the second and third.)
+constexpr int kMaxWide = 4;
 
 inline Cut cut_for(int64_t seqs, int64_t tokens, int64_t nkv, int64_t group, int64_t width) {
   Cut c;
@@ -648,11 +654,7 @@ int launch_attn(Kv8AttnArgs a, const Cut& cut, hipStream_t stream) {
       break;
     case 2: hipLaunchKernelGGL(kv8_wide_kernel<2>, g, dim3(128), 0, stream, a); break;
     case 3: hipLaunchKernelGGL(kv8_wide_kernel<3>, g, dim3(192), 0, stream, a); break;
-    case 4: hipLaunchKernelGGL(kv8_wide_kernel<4>, g, dim3(256), 0, stream, a); break;
-    case 5: hipLaunchKernelGGL(kv8_wide_kernel<5>, g, dim3(320), 0, stream, a); break;
-    case 6: hipLaunchKernelGGL(kv8_wide_kernel<6>, g, dim3(384), 0, stream, a); break;
-    case 7: hipLaunchKernelGGL(kv8_wide_kernel<7>, g, dim3(448), 0, stream, a); break;
-    default: hipLaunchKernelGGL(kv8_wide_kernel<8>, g, dim3(512), 0, stream, a);
+    default: hipLaunchKernelGGL(kv8_wide_kernel<4>, g, dim3(256), 0, stream, a);
   }
   if (cut.splits > 32 || (cut.splits > 8 && cols <= 2 * device_cus()))
     hipLaunchKernelGGL(kv8_combine_kernel<16>, dim3((unsigned)cols), dim3(1024), 0, stream, a,
