@@ -713,8 +713,21 @@ extern "C" int dip_kv8_decode_attention(const uint16_t* q, const uint8_t* k_cach
 }
 
 namespace {
-// Whether a prompt goes over the cache expanded to bf16, in tiles of 128 columns.
-inline bool by_tiles(int64_t tokens, int64_t group) { return tokens * group > 256; }
+// Whether a prompt goes over the cache expanded to bf16, in tiles of 128 columns: where
+// the columns of a kv head are worth the expansion of all rows before, which the kernels
+// above do without.  Those take a page again for every 64 columns, but cut it into splits
+// that fill the card from fewer columns where there are fewer heads.  Columns of a kv
+// head, us by pages and by tiles, in a row:
+//   64 / 8 heads, 16000 rows before  256 42 59, 512 67 71, 640 83 77, 1024 117 99
+//                 6000               256 27 37, 512 40 42, 640 46 43, 1024 57 52
+//                 500                128 19 17, 512 19 21, 1024 21 26 (none 7 10, 7 10, 8 12)
+//   32 / 32       6000               256 57 73, 512 101 100, 640 142 114
+//   32 / 4        16000              512 43 50, 768 55 56, 1024 67 62, 1536 92 76
+//   16 / 2        16000              512 34 45, 1024 42 46, 1536 55 52, 2048 68 58
+//   8 / 1         16000              512 23 39, 1024 34 43, 2048 43 45, 4096 68 56
+inline bool by_tiles(int64_t tokens, int64_t group, int64_t nkv) {
+  return tokens * group > max((int64_t)512, min(4096 / nkv, (int64_t)1536));
+}
 }  // namespace
 
 extern "C" size_t dip_kv8_prompt_attention_workspace_size(int64_t tokens, int64_t start,
@@ -725,7 +738,8 @@ extern "C" size_t dip_kv8_prompt_attention_workspace_size(int64_t tokens, int64_
       tokens * n_heads > INT32_MAX)
     return 0;
   const int64_t group = n_heads / n_kv_heads;
-  if (by_tiles(tokens, group)) return prompt_tiles_workspace(tokens, start, n_kv_heads, group);
+  if (by_tiles(tokens, group, n_kv_heads))
+    return prompt_tiles_workspace(tokens, start, n_kv_heads, group);
   return cut_for(1, tokens, n_kv_heads, group, (start + tokens + kPageRows - 1) / kPageRows)
       .part_bytes(1, n_kv_heads);
 }
@@ -752,7 +766,7 @@ extern "C" int dip_kv8_prompt_attention(const uint16_t* q, const uint8_t* k_cach
   const Kv8Pages c{const_cast<uint8_t*>(k_cache), const_cast<uint8_t*>(v_cache),
                    const_cast<float*>(kv_scales), (int)pages, (int)n_kv_heads};
   hipStream_t s = (hipStream_t)stream;
-  if (by_tiles(tokens, group)) {
+  if (by_tiles(tokens, group, n_kv_heads)) {
     PromptArgs p{q, out, start, (int)tokens, (int)n_kv_heads, (int)group, scale};
     if (int st = prompt_tiles_plan(p, workspace)) return st;
     hipLaunchKernelGGL(kv8_expand_kernel, dim3((unsigned)(n_kv_heads * (p.blocks / 2))), dim3(256),
