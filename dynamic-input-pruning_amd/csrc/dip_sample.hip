@@ -39,6 +39,158 @@
 namespace dip {
 namespace {
 
+// kIndex: of equal ones the first, for greedy draws.
+template <int kType, bool kIndex>
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
+  const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
+  const char* row = row_of(a, r);
+  RowState& st = row_state(a, r);
+  float most = -INFINITY, low = INFINITY;
+  int64_t at = 0;  // a thread's tokens come in ascending order
+  each_token<kType>(row, a.vocab, s * a.slice_vecs,
+                    min((s + 1) * a.slice_vecs, row_vecs<kType>(row, a.vocab)),
+                    [&](int64_t i, float x) {
+                      if (kIndex) at = x > most ? i : at;
+                      most = fmaxf(most, x);
+                      if (!kIndex) low = fminf(low, x == -INFINITY ? INFINITY : x);
+                    });
+  uint64_t best = (uint64_t)order_key(most) << 32 | (uint32_t)~(uint32_t)at;
+  best = block_reduce(best, [](uint64_t x, uint64_t y) { return max(x, y); }, lds);
+  const uint32_t least = block_reduce(order_key(low), [](uint32_t x, uint32_t y) { return min(x, y); },
+                                      reinterpret_cast<uint32_t*>(lds));
+  if (threadIdx.x == 0) {
+    st.best[s] = best;
+    st.least[s] = least;
+    if (s == 0) st.listed = 0;
+  }
+  if (kIndex) return;
+  for (int b = s * kThreads + threadIdx.x; b < kBins; b += a.slices * kThreads) {
+    st.hn[b] = 0;
+    st.hw[b] = 0;
+  }
+}
+
+// kCount: top-k needs the number of tokens in the bins too.
+template <int kType, bool kCount>
+__global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
+  __shared__ double roots[64];
+  __shared__ uint32_t hn[kCount ? kBins : 1];
+  __shared__ unsigned long long hw[kBins];
+  const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
+  const char* row = row_of(a, r);
+  RowState& st = row_state(a, r);
+  const int64_t v0 = s * a.slice_vecs;
+  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
+  const Piece<kType> head(row, a.vocab, v0 + threadIdx.x);
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    if (kCount) hn[b] = 0;
+    hw[b] = 0;
+  }
+  uint64_t best;
+  uint32_t least;
+  row_ends(a, st, lds, best, least);
+  const uint32_t top = (uint32_t)(best >> 32);
+  if (top <= kKeyMinusInf) return;
+  const Weigher wt(a, top, least, roots);
+  __syncthreads();
+  const auto add = [&](int64_t, float x) {
+    const unsigned long long w = wt.whole_of(x);
+    if (w == 0) return;
+    const int b = wt.bin(x);
+    if (kCount) atomicAdd(&hn[b], 1u);
+    atomicAdd(&hw[b], w);
+  };
+  if (wt.inf)
+    each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) { add(i, wt.value(x)); });
+  else
+    each_token<kType>(head, row, a.vocab, v0, v1, add);
+  __syncthreads();
+  unsigned long long* own = slice_hist(a, r, s);
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    own[b] = hw[b];
+    if (!hw[b]) continue;
+    if (kCount) atomicAdd(&st.hn[b], hn[b]);
+    atomicAdd(&st.hw[b], hw[b]);
+  }
+}
+
+// kHist: the histogram has been made.
+template <int kType, bool kHist>
+__global__ __launch_bounds__(kThreads) void sample_gather_kernel(SampleArgs a) {
+  __shared__ uint64_t lds[kLdsWords];
+  __shared__ double roots[64];
+  const int r = blockIdx.x / a.slices, s = blockIdx.x % a.slices;
+  const char* row = row_of(a, r);
+  RowState& st = row_state(a, r);
+  const int64_t v0 = s * a.slice_vecs;
+  const int64_t v1 = min(v0 + a.slice_vecs, row_vecs<kType>(row, a.vocab));
+  // a short slice's tokens are fetched at once; a long one's only if some of them lie
+  // in the bins to list, which its own histogram tells
+  const bool early = !kHist || a.slice_vecs <= kThreads;
+  Piece<kType> head(row, a.vocab, early ? v0 + threadIdx.x : INT32_MAX);
+  uint64_t best;
+  uint32_t least;
+  row_ends(a, st, lds, best, least);
+  const uint32_t top = (uint32_t)(best >> 32);
+  Plan p{top, least, kBins, kBins, 0, 0, 0, 0, 0};
+  if (top <= kKeyMinusInf) {
+    if (s == 0 && threadIdx.x == 0) st.plan = p;
+    return;
+  }
+  const Weigher wt(a, top, least, roots);
+  __syncthreads();
+  uint64_t sure = 0;
+  if (kHist) {
+    p = make_plan(a, st.hn, st.hw, wt, p, lds);
+    const unsigned long long* own = slice_hist(a, r, s);
+    int some = 0;
+    for (int b = threadIdx.x; b <= min(p.hi, kBins - 1); b += kThreads) {
+      if (b < p.lo)
+        sure += own[b];
+      else
+        some |= own[b] != 0;
+    }
+    if (p.lo < kBins && __syncthreads_or(some)) {
+      if (!early) head = Piece<kType>(row, a.vocab, v0 + threadIdx.x);
+      each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) {
+        const float y = wt.value(x);
+        const int b = wt.bin(y);
+        if (b < p.lo || b > p.hi || wt.whole_of(y) == 0) return;
+        const uint32_t at = atomicAdd(&st.listed, 1u);
+        if (at < kListMax) st.list[at] = (uint64_t)order_key(x) << 32 | (uint32_t)~(uint32_t)i;
+      });
+    }
+  } else {
+    const auto add = [&](int64_t, float x) { sure += wt.kept_whole(x); };
+    if (wt.inf)
+      each_token<kType>(head, row, a.vocab, v0, v1, [&](int64_t i, float x) { add(i, wt.value(x)); });
+    else
+      each_token<kType>(head, row, a.vocab, v0, v1, add);
+  }
+  sure = block_reduce(sure, [](uint64_t x, uint64_t y) { return x + y; }, lds);
+  if (threadIdx.x == 0) {
+    st.sure[s] = sure;
+    if (s == 0) st.plan = p;
+  }
+}
+
+template <int kType>
+void launch_slices_of(const SampleArgs& a, int rows, hipStream_t s) {
+  const dim3 slices((unsigned)rows * a.slices), block(kThreads);
+  hipLaunchKernelGGL((sample_max_kernel<kType, false>), slices, block, 0, s, a);
+  if (!counts(a)) {
+    hipLaunchKernelGGL((sample_gather_kernel<kType, false>), slices, block, 0, s, a);
+    return;
+  }
+  if (a.top_k > 0 && a.top_k < a.vocab)
+    hipLaunchKernelGGL((sample_hist_kernel<kType, true>), slices, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((sample_hist_kernel<kType, false>), slices, block, 0, s, a);
+  hipLaunchKernelGGL((sample_gather_kernel<kType, true>), slices, block, 0, s, a);
+}
+
 __global__ __launch_bounds__(kThreads) void sample_greedy_kernel(SampleArgs a) {
   __shared__ uint64_t lds[kLdsWords];
   uint64_t best;
@@ -233,12 +385,11 @@ int launch_sample(const SampleArgs& a, int rows, int64_t vecs, hipStream_t s) {
   if (threads) return launch_row<kType, 1024>(a, rows, s);
   const dim3 each(rows), draw(kDrawThreads);
   if (a.per_64th == 0) {
-    hipLaunchKernelGGL((sample_max_kernel<kType, true>), dim3((unsigned)rows * a.slices),
-                       dim3(kThreads), 0, s, a);
+    launch_slices_max(kType, a, rows, s);
     hipLaunchKernelGGL(sample_greedy_kernel, each, dim3(kThreads), 0, s, a);
     return hip_status(hipGetLastError());
   }
-  launch_slices<kType>(a, rows, s);
+  launch_slices(kType, a, rows, s);
   if (counts(a))
     hipLaunchKernelGGL((sample_draw_kernel<kType, true>), each, draw, 0, s, a);
   else
@@ -247,6 +398,23 @@ int launch_sample(const SampleArgs& a, int rows, int64_t vecs, hipStream_t s) {
 }
 
 }  // namespace
+
+void launch_slices(int dtype, const SampleArgs& a, int rows, hipStream_t s) {
+  if (dtype == DIP_F32) return launch_slices_of<DIP_F32>(a, rows, s);
+  if (dtype == DIP_F16) return launch_slices_of<DIP_F16>(a, rows, s);
+  launch_slices_of<DIP_BF16>(a, rows, s);
+}
+
+void launch_slices_max(int dtype, const SampleArgs& a, int rows, hipStream_t s) {
+  const dim3 slices((unsigned)rows * a.slices), block(kThreads);
+  if (dtype == DIP_F32)
+    hipLaunchKernelGGL((sample_max_kernel<DIP_F32, true>), slices, block, 0, s, a);
+  else if (dtype == DIP_F16)
+    hipLaunchKernelGGL((sample_max_kernel<DIP_F16, true>), slices, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((sample_max_kernel<DIP_BF16, true>), slices, block, 0, s, a);
+}
+
 }  // namespace dip
 
 using namespace dip;

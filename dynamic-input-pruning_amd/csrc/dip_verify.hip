@@ -794,10 +794,9 @@ int launch_verify(const VerifyArgs& v, int rows, int64_t vecs, hipStream_t s) {
   } else if (threads) {
     launch_rows<kType, 1024>(v, rows, s);
   } else if (greedy) {
-    hipLaunchKernelGGL((sample_max_kernel<kType, true>), dim3((unsigned)rows * v.s.slices),
-                       dim3(kThreads), 0, s, v.s);
+    launch_slices_max(kType, v.s, rows, s);
   } else {
-    launch_slices<kType>(v.s, rows, s);
+    launch_slices(kType, v.s, rows, s);
     if (counts(v.s))
       hipLaunchKernelGGL((verify_slices_kernel<kType, true>), dim3(rows), dim3(kDrawThreads), 0,
                          s, v);
