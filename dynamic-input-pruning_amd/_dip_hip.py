@@ -1299,8 +1299,9 @@ def kv8_decode_attention(q, cache: KV8Cache, table, pos, out, scale: float, ws=N
     """Grouped-query attention of one or a few tokens of each of several sequences: q
     [seqs, tokens, n_heads * 128], token t of sequence s over rows 0 .. pos[s] + t of its
     pages in one layer's 8-bit cache -> out (new if None).  A sequence whose position is
-    negative gives zeros.  The work is cut by the table's width: one no wider than the
-    longest sequence's pages is the fastest.  ws: a workspace of
+    negative gives zeros.  The work of several is cut by the table's width: one no wider
+    than the longest sequence's pages is the fastest (four times as wide up to twice, sixteen
+    times up to five times as long).  ws: a workspace of
     kv8_decode_attention_workspace_bytes, one for each call that may run at once (None:
     the call's own)."""
     (dev, table, pos), nkv = _kv8(cache, table, pos), cache.n_kv_heads

@@ -112,12 +112,11 @@ typedef const __attribute__((address_space(1))) void global_void;
 //     l ^ 32 share a column);
 //   out^T += V^T P^T, the weights rounded to bf16 in place: they are the operand
 //     as they lie.  (Off by 2^-8 of itself at most, as any bf16 weight is.)
-// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 284 us a call, the
-// 8-bit cache's expansion of 7 with it, 0.97 PFLOP/s, where a large product of matrices
-// reaches 1.2 to 1.37 (a trace of 30 calls alone has this launch longer).  Of 298 the
-// MFMAs were busy 49 % of the time and the VALU, the softmax mostly, 56 %; without the
-// fetch it took 240 us, without the exponentials 336, without the second product 290 (of
-// 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
+// 4096 tokens of 64 / 8 heads, 275 GFLOP without the masked half: 274 to 292 us a call,
+// card to card, the 8-bit cache's expansion of 7 with it, 0.94 to 1 PFLOP/s, where a large
+// product of matrices reaches 1.2 to 1.37.  The MFMAs are busy 50 % of the time and the VALU,
+// the softmax mostly, 48 %.  Earlier forms: without the fetch 240 us of then 298, without
+// the exponentials 336, without the second product 290 (of 350).  (8 waves to a workgroup 341 of then 352, but 72 for 43 at 1024 tokens; three
 // buffers 353; rows through registers into LDS 493; 32 rows to a step and three
 // workgroups to a CU 340 to 346; 256 columns to a workgroup of 8 waves, four of which
 // multiply while four weigh, a meeting at each change of turns: 278 of then 290, for as

@@ -98,6 +98,10 @@ DIP_DEV uint32_t row_bytes(int t, int c, int lo, int hi) {
 // and nothing is exchanged between them but the largest magnitudes.  All of a page's
 // rows are in registers before any is written, as they share a scale.  Then, with the
 // norm, the q heads, a wave per four heads of a token.
+// A prompt of 4099 tokens of 64 / 8 heads: 42 us, 187 MB at 3.7 to 3.9 TB/s, VALU 76 % busy
+// with the norm, in 64 bits; 40000 tokens' keys and values without it at 5.8 TB/s.  One
+// token: 5.5 us of waits in a row, 5.0 for 4.1 where the page's 63 earlier rows are rounded
+// again to a larger scale.
 template <bool kNorm>
 __global__ __launch_bounds__(64 * kWriteWaves) void kv8_write_kernel(Kv8WriteArgs a) {
   __shared__ uint32_t most[2][kWriteWaves];

@@ -244,8 +244,9 @@ DIP_DEV uint4 buffer_piece(__amdgpu_buffer_rsrc_t b, int piece) {
 
 // Up to 16 columns: a workgroup of W waves takes a split's pages in turn, each wave
 // with all columns, from memory into registers, 32 KB of a wave in flight.  Bound by
-// memory: 32 sequences of up to 16384 rows (547 MB) 114 us, 4.8 TB/s; one of 131071 (268
-// MB) 44.  One of 701 rows, in one launch of 8 waves: 8.8 us of waits in a row.
+// memory: 32 sequences of up to 16384 rows (547 MB) 113 us, 4.9 TB/s, MFMA 12 % and VALU 35
+// % busy; one of 131071 (268 MB) 53, 5.1 TB/s.  One of 701 rows, in one launch of 8 waves:
+// 9.6 us of waits in a row.
 template <int W>
 __global__ __launch_bounds__(W * 64) void kv8_attn_kernel(Kv8AttnArgs a) {
   __shared__ float wm[W][16], wl[W][16];
@@ -359,8 +360,9 @@ typedef const __attribute__((address_space(1))) void global_void;
 // wave with 16 columns of its own.  A page goes straight from memory to LDS, the next one
 // while this one is worked on; its 16-byte pieces lie there in an order in which eight
 // neighbouring lanes' are in different banks.  6 sequences of up to 20011 rows with 40
-// columns (135 MB): 37 us, 3.6 TB/s, bound by the wait for a page, of which three or four
-// workgroups of a CU have one each under way.  (Each wave with all 40 columns, padded to
+// columns (135 MB): 37 us, 3.8 TB/s, VALU 53 % and MFMA 18 % busy: the conversion and the
+// softmax, and the wait for a page, of which three or four workgroups of a CU have one each
+// under way.  (Each wave with all 40 columns, padded to
 // 64, in registers: 68 us; masked pages and others in one loop, which spills: 39, a
 // whole call 49 for 43; two pages under way, whose three buffers leave room for fewer
 // workgroups: 10 more.)
@@ -579,12 +581,15 @@ __global__ __launch_bounds__(256) void kv8_expand_kernel(Kv8Pages a, const int32
 // an even share of the pages there are.  Of several sequences, whose lengths only the
 // device knows, a split is a share of the table's width that makes half as many
 // workgroups again as run at once (narrow ones: three times as many), of which those
-// behind a sequence's end leave at once: 32 of up to 16384 rows 118 us, with a round and
-// a third 125; 6 of up to 20011 with 5 tokens each 45, with one round 54, with two 64; with
-// 3 tokens each 40, 42 and 56 (of two waves' workgroups five fit a CU, four are counted:
-// with five 55).
-// A split has a page for each wave at least, of several sequences 8: 4000 rows of one 12.9
-// us with 4 for 14.4 with 8, 20011 rows 17.1 for 18.8; 8 sequences of 2000 17.0 for 14.8.
+// behind a sequence's end leave at once.  In a graph, states in turn: 32 of up to 16384
+// rows 120 us, with one round 134, with a round and a third 118, with two 130; 6 of up to
+// 20011 with 5 tokens each 46, with one round 53, a third more 49, with two 67; with 3
+// tokens each 41, 42, 44 and 57 (of two waves' workgroups five fit a CU, four are counted:
+// with five 56).  Where the table is wider than the longest sequence's pages splits are
+// longer and more workgroups leave: four times as wide the first takes 137 us for 120,
+// the second 82 for 42 (one state).
+// A split has a page for each wave at least, of several sequences 8: 4000 rows of one 10.8
+// us with 4 for 14.0 with 8, 20011 rows 17.3 for 19.4; 8 sequences of 2000 15.8 for 13.9.
 struct Cut {
   int waves, tiles, per, splits;
   int cols() const { return waves ? 16 * waves : 16; }

@@ -246,7 +246,7 @@ class DIPDecoder:
                  what later tokens see (through the HF forward, where the model
                  has other modules, hooks or modes, it does not).
       kv_dtype:  torch.float8_e4m3fn: keys and values in 8 bits with a scale per 64
-                 positions of a head (257 bytes per row and kv head), in pages; the
+                 positions of a head (256 bytes per row and kv head), in pages; the
                  same needs as kv_bits=4.  None: as kv_bits says.
     """
 
@@ -731,7 +731,11 @@ class DIPDecoder:
         accepted and of drafted tokens.  It needs a cache of 4 or 8 bits, which a pass of
         several tokens can go on from, with room for `draft` tokens behind the last.  (A
         page of 8 bits keeps the scale that refused drafts' keys or values may have
-        raised, and with it the rounding of its numbers below 2^-14 of the largest.)"""
+        raised, and with it the rounding of its numbers below 2^-14 of the largest.)
+        It is for the dense model's tokens from a pruned model's steps, not for speed:
+        steps of every channel (keep_ratio 1) take less where, as with 64 layers of the
+        32B shape at keep 0.6, a pruned step takes 4.7 ms, one of every channel 5.5 and
+        the dense pass 8.2."""
         if draft:
             if not math.isfinite(draft) or draft < 0 or int(draft) != draft:
                 raise ValueError(f"draft must be a whole number >= 0, got {draft}")

@@ -714,7 +714,7 @@ int dip_kv4_prompt_attention(const uint16_t* q, const int8_t* k_cache, const int
  *   k_cache   [pages, n_kv_heads, 64 * 128] bytes
  *   v_cache   [pages, n_kv_heads, 64 * 128] bytes
  *   kv_scales fp32 [pages, n_kv_heads, 2]
- * 257 bytes per position and kv head, where bf16 takes 512.  table int32
+ * 256 bytes per position and kv head, 8 more per page, where bf16 takes 512.  table int32
  * [seqs, table_width] (on the device): the number of the page that holds the positions
  * 64 j .. 64 j + 63 of sequence s at [s][j].  pos int64 [seqs] (on the device): the
  * position of a sequence's first token of the call, its others follow it.  A negative
