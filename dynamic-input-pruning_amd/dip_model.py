@@ -781,7 +781,7 @@ class DIPDecoder:
         plen = ids.shape[1]
         if plen < 1:
             raise ValueError("an empty prompt")
-        if plen + max_new_tokens + draft > self.max_len:
+        if plen + max(max_new_tokens, 0) + draft > self.max_len:
             raise ValueError(f"{plen} + {max_new_tokens} tokens and {draft} drafted ones exceed "
                              f"max_len {self.max_len}")
         eos = set(() if eos_token_id is None else eos_token_id

@@ -773,8 +773,8 @@ int dip_qk_norm_rope_kv8(const uint16_t* qkv, const uint16_t* q_norm_w, const ui
  * have, token t over rows 0 .. start + t.
  * Types, sums and what is not finite as with dip_kv4_decode_attention, but for the
  * weights.  Of up to 16 columns (tokens * n_heads / n_kv_heads) they are two bf16 numbers
- * each, off by 2^-17 of it, else one, without the values' scales, off by 2^-8 at most.  Workspaces need no
- * clearing; calls that may run at once need one each.
+ * each, off by 2^-17 of it, else one, without the values' scales, off by 2^-8 at most.
+ * Workspaces need no clearing; calls that may run at once need one each.
  */
 size_t dip_kv8_decode_attention_workspace_size(int64_t seqs, int64_t tokens, int64_t n_heads,
                                                int64_t n_kv_heads, int64_t head_dim,
@@ -838,11 +838,11 @@ int dip_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64
  * largest logits are accepted, draft_logits and u are not read.  A row with nothing to
  * choose from accepts nothing and gives token 0.  tokens >= 0; logits, types and filters
  * as dip_sample's; seqs * (2 tokens + 1) below 2^22.  What is left of p is summed in whole
- * numbers of 2^-51.  Without filters a row's sum is put together of
- * parts, which the call's number of rows cuts: it may depend on that by 2^-30 of itself
- * (2^-24 at the very most, where thousands of tokens are hardly likelier than none), and
- * so may a draft whose u * q_t lies that near to p_t.  The workspace needs no clearing; calls that may run at once need
- * one each.  The reference has no counterpart.
+ * numbers of 2^-51.  Without filters a row's sum is put together of the sums of its parts,
+ * and how many there are depends on the call's number of rows: it may change by 2^-30 of
+ * itself with them (2^-24 at the very most), and so a draft whose u * q_t lies that near to
+ * p_t may be accepted in one call and refused in another.  The workspace needs no
+ * clearing; calls that may run at once need one each.  The reference has no counterpart.
  */
 size_t dip_verify_workspace_size(int64_t seqs, int64_t tokens, int64_t vocab, int draft_logits);
 int dip_verify(const void* logits, int dtype, int64_t seqs, int64_t tokens, int64_t vocab,

@@ -79,3 +79,12 @@ def test_an_empty_prompt_is_refused(pruned):
     for draft in (0, 2):
         with pytest.raises(ValueError):
             dec.generate(torch.zeros(1, 0, dtype=torch.long), 2, draft=draft)
+
+
+def test_a_prompt_longer_than_the_cache_is_refused(pruned):
+    """Whatever the number of new tokens, one that is negative among them."""
+    from dip_model import DIPDecoder
+    dec = DIPDecoder(pruned, 64, kv_dtype=E4M3)
+    for new in (2, 0, -10):
+        with pytest.raises(ValueError):
+            dec.generate(_prompt(70), new, draft=2)
